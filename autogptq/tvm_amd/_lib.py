@@ -49,6 +49,10 @@ ABI_SYMBOLS = (
     "gptq_hip_gemm_tiled_transposed",
     "gptq_hip_gemm_tiled",
     "gptq_hip_dequant",
+    "gptq_hip_cache_tables",
+    "gptq_hip_cache_write",
+    "gptq_hip_attention_workspace_bytes",
+    "gptq_hip_attend",
     "gptq_hip_probe",
     "gptq_hip_strerror",
     "gptq_hip_abi_version",
@@ -94,6 +98,28 @@ class Route(ctypes.Structure):
     """Mirror of ``gptq_hip_route``."""
 
     _fields_ = [("copy", ctypes.c_int), ("reserved", ctypes.c_int), ("plan", Plan)]
+
+
+TYPE_FP16, TYPE_BF16 = 0, 1
+CACHE_MAX_REQUESTS = 16384
+
+
+class Cache(ctypes.Structure):
+    """Mirror of ``gptq_hip_cache``."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + [
+        (name, ctypes.c_int) for name in ("type", "blocks", "block_size", "heads", "dim")] + [
+        (name, ctypes.c_longlong) for name in ("block_stride", "slot_stride", "head_stride")]
+
+
+class Attention(ctypes.Structure):
+    """Mirror of ``gptq_hip_attention``."""
+
+    _fields_ = [("cache", Cache)] + [
+        (name, ctypes.c_void_p) for name in ("q", "out", "tables", "starts", "contexts", "prefix_blocks")] + [
+        (name, ctypes.c_int) for name in ("tokens", "requests", "heads", "table_width", "max_context", "window", "sinks",
+                                          "prefix_length")] + [
+        (name, ctypes.c_longlong) for name in ("q_token_stride", "q_head_stride", "table_stride")] + [("scale", ctypes.c_float)]
 
 
 class GptqHipError(RuntimeError):
@@ -185,6 +211,15 @@ def lib() -> ctypes.CDLL:
     l.gptq_hip_select_tiled_transposed.argtypes = [i, i, i, i, i, ctypes.POINTER(Plan)]
     l.gptq_hip_gemm_tiled_transposed.restype = i
     l.gptq_hip_gemm_tiled_transposed.argtypes = [vp, vp, vp, vp, vp, vp, sz, i, i, i, i, i, ctypes.POINTER(Plan), vp]
+    ll = ctypes.c_longlong
+    l.gptq_hip_cache_tables.restype = i
+    l.gptq_hip_cache_tables.argtypes = [vp, vp, vp, ll, i, vp, i, i, i, i, vp, vp, vp, vp, vp, vp]
+    l.gptq_hip_cache_write.restype = i
+    l.gptq_hip_cache_write.argtypes = [ctypes.POINTER(Cache), vp, vp, ll, ll, ll, ll, vp, i, vp]
+    l.gptq_hip_attention_workspace_bytes.restype = sz
+    l.gptq_hip_attention_workspace_bytes.argtypes = [ctypes.POINTER(Attention)]
+    l.gptq_hip_attend.restype = i
+    l.gptq_hip_attend.argtypes = [ctypes.POINTER(Attention), vp, sz, vp]
     l.gptq_hip_probe.restype = i
     l.gptq_hip_probe.argtypes = [i, vp, sz, vp, sz, i, i, i, i, vp, vp, vp]
     l.gptq_hip_dequant.restype = i

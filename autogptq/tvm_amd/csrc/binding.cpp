@@ -41,6 +41,7 @@ void raise(int rc, const char *what, int64_t M, int64_t K, int64_t N, int64_t bi
 // kind 1: the decode plans of the tiled family with halved tiles, whose kernel keeps their bytes zero between launches
 // (the slots of the halves): nothing else may write there, so they do not share the workspace the other plans pack x
 // or partial sums into.
+// kind 2: the attention's, whose counters and parts lie elsewhere than a product's (kAttentionWorkspace).
 static std::mutex g_ws_mutex;   // of the map; its entries stay where they are
 static std::map<std::tuple<int, void *, int>, Workspace> g_ws;
 
@@ -59,7 +60,7 @@ WorkspaceLease::WorkspaceLease(const Tensor &like, size_t nbytes, void *stream, 
         void *stream = nullptr;
         Workspace *ws = nullptr;
     };
-    static thread_local Last last[2];
+    static thread_local Last last[3];
     Last &l = last[kind];
     const int device = (int)like.get_device();
     if (!l.ws || l.device != device || l.stream != stream) {

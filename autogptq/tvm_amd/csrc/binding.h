@@ -22,6 +22,7 @@ inline Tensor aligned(const Tensor &x) { return (uintptr_t)x.data_ptr() % 16 == 
 
 void raise(int rc, const char *what, int64_t M, int64_t K, int64_t N, int64_t bits, int64_t gs);
 
+constexpr int kAttentionWorkspace = 2;
 int workspace_kind(const gptq_hip_plan &plan);
 
 // The workspace of a stream for the launches of one call (none for nbytes = 0).  Held over all of them: a call is up to three

@@ -356,4 +356,7 @@ int launch_tiled(const void *x, const void *qtile, const uint32_t *sz, const int
                  char *xpack, float *partial, int M, int K, int N, int bits, int group_size,
                  const gptq_hip_plan &plan, void *stream);
 
+// the cache's shape and strides are ones the cache kernels take (gptq_attention_plan.cpp)
+int check_cache(const gptq_hip_cache *cache);
+
 }  // namespace gptq

@@ -352,6 +352,78 @@ enum { GPTQ_HIP_PROBE_EMPTY = 0, GPTQ_HIP_PROBE_STREAM = 1, GPTQ_HIP_PROBE_MIXED
 int gptq_hip_probe(int kind, const void *buf, size_t bytes, const void *hot, size_t hot_bytes, int workgroups, int iters,
                    int mode, int depth, unsigned long long *ticks, void *scratch, void *stream);
 
+/*
+ * Serving: a paged key/value cache next to the quantised layers, and the attention that reads it.  No counterpart in the
+ * reference, whose models keep torch's attention.
+ *
+ * A cache holds `blocks` blocks of `block_size` token slots (any size), each slot with the keys (or values) of `heads` heads of `dim`
+ * elements.  Strides are in elements; dim is a multiple of 8 up to 256 whose elements lie side by side, strides are
+ * multiples of 8, k and v are 16-byte aligned and share shape and strides.  Slot s is slot s % block_size of block
+ * s / block_size.  A request's block table names, for each block_size tokens of its context, the block that holds them.
+ */
+enum { GPTQ_HIP_TYPE_FP16 = 0, GPTQ_HIP_TYPE_BF16 = 1 };
+typedef struct gptq_hip_cache {
+    void *k, *v;
+    int type;                 /* GPTQ_HIP_TYPE_* */
+    int blocks, block_size, heads, dim;
+    long long block_stride, slot_stride, head_stride;
+} gptq_hip_cache;
+
+/*
+ * The bookkeeping of a step.  Request b has lengths[b] tokens in the cache and gets counts[b] more; the blocks it needs
+ * for them are taken from the front of free_blocks, requests in order, and entered into its table row.
+ *   lengths, counts int32 [requests]   tokens in the cache, new tokens (0 or less: none)
+ *   tables int32 [requests, table_width], rows table_stride apart: read, and new entries written
+ *   starts int32 [requests + 1]        out: new tokens before each request, and all of them
+ *   contexts int32 [requests]          out: lengths + counts
+ *   slots, positions int32 [tokens]    out: cache slot and position of every new token; tokens = the room in the two (a caller
+ *                                      who knows the lengths knows the sum); entries past the last new token are -1
+ *   taken int32 [1]                    out: blocks needed.  More than free_count: the tokens without a block got slot -1
+ * Tokens that lie past a table's width get slot -1 too.  Up to GPTQ_HIP_CACHE_MAX_REQUESTS requests
+ * (GPTQ_HIP_ERR_UNSUPPORTED beyond).  One launch; the same inputs give the same results however often it runs.
+ */
+#define GPTQ_HIP_CACHE_MAX_REQUESTS 16384
+int gptq_hip_cache_tables(const int32_t *lengths, const int32_t *counts, int32_t *tables, long long table_stride,
+                          int table_width, const int32_t *free_blocks, int free_count, int requests, int tokens,
+                          int block_size, int32_t *starts, int32_t *contexts, int32_t *slots, int32_t *positions,
+                          int32_t *taken, void *stream);
+
+/* Keys and values [tokens, heads, dim] (16-byte aligned, strides in elements and multiples of 8) into their slots; slots
+ * below 0 or outside of the cache are skipped.  One launch. */
+int gptq_hip_cache_write(const gptq_hip_cache *cache, const void *k, const void *v, long long k_token_stride,
+                         long long k_head_stride, long long v_token_stride, long long v_head_stride,
+                         const int32_t *slots, int tokens, void *stream);
+
+/*
+ * Causal attention of a step's tokens over their requests' blocks.  starts and contexts as gptq_hip_cache_tables gives
+ * them: request b has the tokens starts[b] .. starts[b + 1] - 1, the last of them at position contexts[b] - 1, and the
+ * query at position i sees the keys j <= i; with window > 0 only those with j > i - window or j < sinks (first tokens that
+ * stay visible).  Query head n reads key/value head n / (heads / cache.heads).
+ *   out[t, n] = sum_j softmax_j(scale q[t, n] . k[j]) v[j], zeros for a token that sees nothing
+ * q [tokens, heads, dim] in the cache's type (16-byte aligned, strides in elements, multiples of 8), out [tokens, heads,
+ * dim] contiguous, 16-byte aligned.  scale > 0.  Scores, softmax and sums are fp32; shares of the softmax are rounded to the cache's
+ * type for the product with v, the result once.  Table entries of blocks that no token of a request sees are
+ * not read (blocks that a window has left behind may be given back), nor are slots past a context.
+ *   prefix_length > 0: every token sees prefix_length more keys before its own context, those of the blocks
+ *     prefix_blocks int32 [ceil(prefix_length / block_size)], shared by all requests and read once for all of them;
+ *     contexts count a request's own tokens only.  window must be 0.
+ *   max_context: the longest context, as the host knows it: it sets how the work is divided, not what is computed (0: the
+ *     tables' width)
+ * workspace: gptq_hip_attention_workspace_bytes, zeroed once; every call leaves its counters at zero, so calls on one
+ * stream may share it, but no other entry point may write to it.  One launch, two with a prefix.
+ */
+typedef struct gptq_hip_attention {
+    gptq_hip_cache cache;
+    const void *q;
+    void *out;
+    const int32_t *tables, *starts, *contexts, *prefix_blocks;
+    int tokens, requests, heads, table_width, max_context, window, sinks, prefix_length;
+    long long q_token_stride, q_head_stride, table_stride;
+    float scale;
+} gptq_hip_attention;
+size_t gptq_hip_attention_workspace_bytes(const gptq_hip_attention *a);
+int gptq_hip_attend(const gptq_hip_attention *a, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Human-readable text for a gptq_hip_status. */
 const char *gptq_hip_strerror(int status);
 

@@ -1,0 +1,296 @@
+"""The attention over a paged cache against the same sums in 64 bits."""
+import ctypes
+
+import pytest
+import torch
+
+from autogptq.tvm_amd import _lib, attention
+from tests.attention_util import Step, assert_attention
+
+HALF, BF16 = torch.float16, torch.bfloat16
+
+
+def attend(s, **more):
+    more = {"max_context": s.most, **more}
+    if s.prefix:
+        return attention.shared_prefix_attention(s.q, s.k_cache, s.v_cache, s.prefix_blocks, s.prefix, s.tables, s.starts,
+                                                 s.contexts, **more)
+    return attention.paged_attention(s.q, s.k_cache, s.v_cache, s.tables, s.starts, s.contexts, window=s.window, sinks=s.sinks,
+                                     **more)
+
+
+# (requests, heads, kv_heads, dim, block_size, dtype, layout, window, sinks)
+CASES = {
+    "one token of one": ([(1, 1)], 1, 1, 64, 16, HALF, "token", 0, 0),
+    "single tokens": ([(1, 1), (2, 1), (63, 1), (64, 1), (65, 1), (700, 1)], 8, 2, 128, 16, HALF, "token", 0, 0),
+    "single tokens, no shared heads": ([(33, 1), (257, 1), (1030, 1)], 4, 4, 128, 32, BF16, "head", 0, 0),
+    "single tokens, sevens": ([(33, 1), (257, 1), (1030, 1)], 14, 2, 128, 7, HALF, "token", 0, 0),
+    "sixteen heads share": ([(129, 1), (5, 1)], 16, 1, 128, 16, HALF, "head", 0, 0),
+    "twenty-four heads share": ([(129, 1), (500, 1)], 24, 1, 128, 16, HALF, "token", 0, 0),
+    "seventy-one heads share": ([(129, 1), (300, 1)], 71, 1, 64, 16, BF16, "token", 0, 0),
+    "requests without tokens": ([(5, 0), (9, 1), (0, 0), (40, 2), (7, 0)], 4, 2, 64, 8, HALF, "token", 0, 0),
+    "drafts": ([(130, 3), (7, 7), (64, 5), (400, 1)], 8, 4, 128, 16, HALF, "head", 0, 0),
+    "drafts of many heads": ([(130, 3), (7, 7), (64, 5), (400, 1)], 16, 2, 128, 16, BF16, "token", 0, 0),
+    "window": ([(300, 1), (100, 1), (65, 1), (64, 1)], 8, 2, 128, 16, HALF, "token", 64, 0),
+    "window and sinks": ([(300, 1), (100, 1), (65, 1), (66, 1), (3, 1)], 8, 2, 128, 16, HALF, "token", 64, 4),
+    "window of one": ([(300, 2), (100, 1), (1, 1)], 4, 2, 64, 16, HALF, "token", 1, 0),
+    "more sinks than context": ([(30, 2), (400, 3)], 4, 2, 128, 16, HALF, "token", 9, 50),
+    "drafts under a window": ([(300, 5), (70, 9), (20, 20)], 4, 2, 128, 24, HALF, "token", 32, 3),
+    "dim 8": ([(300, 1), (70, 40)], 4, 2, 8, 16, HALF, "token", 0, 0),
+    "dim 72": ([(300, 1), (70, 3)], 4, 2, 72, 16, HALF, "head", 0, 0),
+    "dim 80": ([(300, 1), (90, 1)], 4, 2, 80, 16, BF16, "token", 0, 0),
+    "dim 256": ([(300, 1), (90, 2)], 4, 2, 256, 16, HALF, "token", 0, 0),
+    "dim 200": ([(300, 1), (90, 2)], 4, 2, 200, 16, BF16, "token", 70, 2),
+    "blocks of one": ([(90, 1), (33, 2)], 4, 2, 64, 1, HALF, "token", 0, 0),
+    "prompt": ([(200, 200)], 4, 2, 128, 16, HALF, "token", 0, 0),
+    "prompts, ragged": ([(1, 1), (129, 129), (64, 64), (333, 200), (17, 3)], 8, 2, 128, 16, BF16, "head", 0, 0),
+    "prompts, blocks of 24": ([(500, 250), (33, 33)], 7, 1, 64, 24, HALF, "token", 0, 0),
+    "prompts under a window": ([(500, 500), (700, 90), (40, 40)], 4, 2, 128, 16, HALF, "token", 100, 0),
+    "prompts under a window with sinks": ([(500, 500), (700, 90), (40, 40)], 4, 1, 128, 16, BF16, "token", 70, 5),
+    "prompt under a window with many sinks": ([(600, 600)], 2, 1, 64, 16, HALF, "token", 30, 100),
+    "prompt, dim 80": ([(200, 150), (77, 77)], 4, 2, 80, 16, HALF, "token", 0, 0),
+    "prompt, dim 256": ([(300, 150), (77, 77)], 4, 2, 256, 16, HALF, "token", 0, 0),
+    "prompt, dim 136": ([(300, 150), (77, 77)], 4, 2, 136, 16, BF16, "head", 64, 1),
+    "prompts of many heads": ([(70, 70), (9, 9)], 40, 8, 128, 64, HALF, "token", 0, 0),
+    "a piece behind a long context": ([(5000, 40)], 4, 1, 128, 16, HALF, "token", 0, 0),
+    "one prompt among single tokens": ([(700, 1), (400, 400), (90, 1), (1200, 1)], 4, 1, 128, 16, HALF, "token", 0, 0),
+    "long": ([(9000, 1)], 8, 2, 128, 16, HALF, "token", 0, 0),
+    "long and short": ([(6000, 1), (3, 1), (900, 1), (1, 1)], 4, 2, 64, 16, BF16, "token", 0, 0),
+    "many requests": ([(1 + 7 * i % 50, i % 3) for i in range(200)], 4, 2, 64, 16, HALF, "token", 0, 0),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(CASES))
+def test_attention(name):
+    requests, heads, kv_heads, dim, block, dtype, layout, window, sinks = CASES[name]
+    s = Step(11, requests, heads, kv_heads, dim, block, dtype, layout, window, sinks)
+    got = attend(s)
+    assert_attention(got, s, name)
+    assert torch.equal(got, attend(s)), "a second call on the same inputs differs"
+
+
+# (requests, heads, kv_heads, dim, block_size, dtype, prefix)
+PREFIXES = {
+    "of one token": ([(1, 1), (5, 1)], 4, 2, 64, 16, HALF, 1),
+    "small batch": ([(1, 1), (37, 1), (300, 1)], 8, 2, 128, 16, HALF, 1000),
+    "own contexts empty": ([(0, 1), (0, 1), (0, 2)], 8, 2, 128, 16, HALF, 130),
+    "batch of a few hundred rows": ([(1 + 13 * i % 90, 1) for i in range(70)], 8, 1, 128, 16, BF16, 2100),
+    "drafts and requests without tokens": ([(30, 3), (8, 0), (200, 5), (2, 2)], 8, 4, 128, 24, HALF, 777),
+    "prompts": ([(150, 150), (64, 30)], 4, 1, 128, 16, HALF, 500),
+    "dim 80": ([(20, 1), (90, 2)], 4, 1, 80, 16, BF16, 333),
+    "dim 256": ([(20, 1), (90, 2), (400, 40)], 8, 2, 256, 16, HALF, 333),
+    "dim 64, sevens": ([(20, 1)] * 9, 7, 1, 64, 7, HALF, 900),
+    "long own contexts": ([(3000, 1), (20, 1)], 4, 2, 128, 16, HALF, 200),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(PREFIXES))
+def test_shared_prefix(name):
+    requests, heads, kv_heads, dim, block, dtype, prefix = PREFIXES[name]
+    s = Step(12, requests, heads, kv_heads, dim, block, dtype, prefix=prefix)
+    got = attend(s)
+    assert_attention(got, s, name)
+    assert torch.equal(got, attend(s))
+
+
+@pytest.mark.gpu
+def test_a_token_that_sees_nothing_gets_zeros():
+    # a context that is shorter than the step's tokens: the first of them stand before its beginning
+    for counts, heads in (((3, 2), 2), ((200, 1), 4)):
+        s = Step(13, [(2, counts[0]), (0, counts[1])], heads, 1, 64, 16)
+        got = attend(s)
+        assert_attention(got, s, "tokens before the context")
+        assert bool((got[:counts[0] - 2] == 0).all()) and bool((got[counts[0]:] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("stale", [-1, 1 << 30, -(1 << 31)])
+def test_table_entries_that_nobody_sees_may_hold_anything(stale):
+    s = Step(14, [(700, 1), (300, 40), (64, 64)], 4, 2, 64, 16, window=50, sinks=3, stale=stale)
+    assert_attention(attend(s), s, f"stale entries {stale}")
+
+
+@pytest.mark.gpu
+def test_values_that_are_large_where_masked():
+    # scores of opposite extremes, and the type's largest finite values in slots past the contexts
+    s = Step(15, [(77, 1), (130, 130)], 4, 2, 64, 16, q_scale=8.0)
+    s.k_cache.nan_to_num_(65504.0)
+    s.v_cache.nan_to_num_(65504.0)
+    want, size = s.expected()
+    got = attend(s)
+    # scores reach 64 here: the 32-bit part of the bound grows with them
+    assert bool(((got.double() - want).abs() <= 3 * 2.0 ** -11 * size + 2.0 ** -24).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hint", [0, 1, 300, 100000])
+def test_max_context_is_a_hint(hint):
+    for requests in ([(5000, 1), (40, 1)], [(3000, 60)]):
+        s = Step(16, requests, 8, 2, 128, 16)
+        assert_attention(attend(s, max_context=hint), s, f"max_context={hint}")
+
+
+@pytest.mark.gpu
+def test_scale():
+    s = Step(17, [(200, 1), (50, 50)], 4, 2, 64, 16)
+    assert_attention(attend(s, scale=0.03), s, "scale 0.03", scale=0.03)
+
+
+@pytest.mark.gpu
+def test_strided_inputs():
+    s = Step(18, [(200, 1), (50, 20)], 8, 2, 64, 16)
+    want = attend(s)
+    # columns of a fused product, rows apart; a table whose rows are apart; offsets that are not 16-byte aligned
+    wide = torch.randn(s.tokens, (8 + 4) * 64, device="cuda").half()
+    wide[:, :512] = s.q.reshape(s.tokens, 512)
+    tables = torch.zeros(2, s.tables.shape[1] + 5, dtype=torch.int32, device="cuda")
+    tables[:, :s.tables.shape[1]] = s.tables
+    odd = torch.randn(s.tokens, 8 * 64 + 3, device="cuda").half()
+    odd[:, 3:] = s.q.reshape(s.tokens, 512)
+    swapped = s.q.transpose(0, 1).contiguous().transpose(0, 1)
+    s.tables = tables[:, :s.tables.shape[1]]
+    for q in (wide[:, :512].view(s.tokens, 8, 64), odd[:, 3:].view(s.tokens, 8, 64), swapped):
+        s.q = q
+        assert torch.equal(attend(s), want)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """A cache of more than 2^32 elements whose used blocks lie at its ends."""
+    s = Step(19, [(40, 1), (30, 20)], 2, 1, 128, 16)
+    want = attend(s)
+    blocks = (1 << 32) // (16 * 128) + 4096
+    caches = []
+    for cache in (s.k_cache, s.v_cache):
+        big = torch.empty((blocks, 16, 1, 128), dtype=cache.dtype, device="cuda")
+        big[blocks - cache.shape[0]:] = cache
+        caches.append(big)
+    used = s.tables >= 0
+    s.tables = torch.where(used, s.tables + blocks - s.k_cache.shape[0], s.tables)
+    s.k_cache, s.v_cache = caches
+    assert torch.equal(attend(s), want)
+    slots = torch.tensor([blocks * 16 - 1, (blocks - 5) * 16 + 2], dtype=torch.int32, device="cuda")
+    k, v = torch.randn(2, 2, 1, 128, device="cuda").half()
+    attention.cache_write(k, v, s.k_cache, s.v_cache, slots)
+    assert torch.equal(s.k_cache[blocks - 1, 15], k[0]) and torch.equal(s.v_cache[blocks - 5, 2], v[1])
+
+
+@pytest.mark.gpu
+def test_on_another_stream():
+    s = Step(20, [(3000, 1), (50, 50)], 4, 2, 128, 16)
+    want = attend(s)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = [attend(s) for _ in range(3)]
+    side.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prefix", [0, 600])
+def test_captured_in_a_graph(prefix):
+    s = Step(21, [(3000, 1), (50, 1), (1, 1)], 4, 2, 128, 16, prefix=prefix)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = attend(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = attend(s)
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            side.synchronize()
+            assert torch.equal(got, want)
+            assert torch.equal(attend(s), want)     # eager work between the replays
+            side.synchronize()
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    s = Step(22, [(40, 1), (30, 20)], 4, 2, 64, 16)
+    args = dict(q=s.q, k_cache=s.k_cache, v_cache=s.v_cache, tables=s.tables, starts=s.starts, contexts=s.contexts)
+    call = lambda **more: attention.paged_attention(**{**args, **more})
+    call()
+    for more, text in (
+            (dict(q=s.q.bfloat16()), "the cache"), (dict(q=s.q[:, :3]), "multiple"), (dict(q=s.q[..., :32]), r"\[tokens, heads, 64\]"),
+            (dict(q=s.q.cpu()), "no CPU fallback"), (dict(v_cache=s.v_cache[:, :8]), "alike"),
+            (dict(v_cache=s.v_cache.contiguous().transpose(1, 2).contiguous().transpose(1, 2)), "strides"),
+            (dict(k_cache=s.k_cache.float(), v_cache=s.v_cache.float()), "float16 or bfloat16"),
+            (dict(tables=s.tables.long()), "int32"), (dict(tables=s.tables[:1]), r"\[2, width\]"),
+            (dict(tables=s.tables.t().contiguous().t()), "contiguous"), (dict(starts=s.starts[:2]), "vector of 3"),
+            (dict(contexts=s.contexts[::2]), "vector"), (dict(window=-1), "window"), (dict(sinks=-1), "sinks"),
+            (dict(max_context=-5), "max_context"), (dict(scale=float("inf")), "scale"),
+            (dict(q=s.q.clone().requires_grad_()), "no backward")):
+        with pytest.raises(RuntimeError, match=text):
+            call(**more)
+    for scale in (0.0, -1.0, float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            call(scale=scale)
+    narrow = s.k_cache[..., :60], s.v_cache[..., :60]
+    with pytest.raises(RuntimeError, match="multiple of 8"):
+        call(q=s.q[..., :60], k_cache=narrow[0], v_cache=narrow[1])
+    with pytest.raises(RuntimeError, match="prefix_blocks has 0"):
+        attention.shared_prefix_attention(s.q, s.k_cache, s.v_cache, s.prefix_blocks, 5, s.tables, s.starts, s.contexts)
+    assert attention.paged_attention(s.q[:0], s.k_cache, s.v_cache, s.tables[:0], s.starts[:1], s.contexts[:0]).shape == (0, 4, 64)
+
+
+def test_cpu_tensors_are_refused():
+    s = Step(23, [(10, 1)], 2, 1, 64, 16, device="cpu")
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        attend(s)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        attention.cache_write(s.k[0], s.v[0], s.k_cache, s.v_cache, torch.arange(10, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        attention.cache_tables(s.contexts, s.contexts, s.tables, s.contexts, 10, 16)
+
+
+def plain(**more):
+    """A call's description whose pointers are never followed: everything is checked before."""
+    a = _lib.Attention()
+    a.cache.k = a.cache.v = a.q = a.out = a.tables = a.starts = a.contexts = 0x1000
+    values = dict(type=0, blocks=100, block_size=16, heads=8, dim=128, block_stride=16384, slot_stride=1024, head_stride=128)
+    for k, v in {**values, **{k: v for k, v in more.items() if k in values or k in ("k", "v")}}.items():
+        setattr(a.cache, k, v)
+    values = {**dict(tokens=64, requests=64, heads=32, table_width=64, max_context=1000, q_token_stride=4096, q_head_stride=128,
+                     table_stride=64, scale=0.1), **more}
+    for k, v in values.items():
+        if k not in ("type", "blocks", "block_size", "dim", "block_stride", "slot_stride", "head_stride", "k", "v"):
+            setattr(a, {"q_heads": "heads"}.get(k, k), v)
+    a.cache.heads = 8
+    return a
+
+
+@pytest.mark.parametrize("more, status", [
+    (dict(type=2), _lib.ERR_BAD_ARG), (dict(blocks=0), _lib.ERR_BAD_ARG), (dict(block_size=0), _lib.ERR_BAD_ARG),
+    (dict(dim=100), _lib.ERR_BAD_ARG), (dict(dim=264), _lib.ERR_UNSUPPORTED), (dict(block_stride=16380), _lib.ERR_BAD_ARG),
+    (dict(blocks=1 << 27), _lib.ERR_UNSUPPORTED), (dict(blocks=1 << 22, block_stride=1 << 20), _lib.ERR_UNSUPPORTED),
+    (dict(k=0x1008), _lib.ERR_BAD_ARG), (dict(k=None), _lib.ERR_BAD_ARG), (dict(q=0x1004), _lib.ERR_BAD_ARG),
+    (dict(out=None), _lib.ERR_BAD_ARG), (dict(starts=None), _lib.ERR_BAD_ARG), (dict(tables=None), _lib.ERR_BAD_ARG),
+    (dict(heads=31), _lib.ERR_BAD_ARG), (dict(requests=0), _lib.ERR_BAD_ARG), (dict(tokens=-1), _lib.ERR_BAD_ARG),
+    (dict(window=-1), _lib.ERR_BAD_ARG), (dict(scale=0.0), _lib.ERR_BAD_ARG), (dict(scale=float("nan")), _lib.ERR_BAD_ARG),
+    (dict(prefix_length=5), _lib.ERR_BAD_ARG), (dict(prefix_length=5, prefix_blocks=0x1000, window=3), _lib.ERR_BAD_ARG),
+    (dict(table_stride=63), _lib.ERR_BAD_ARG), (dict(q_token_stride=4100), _lib.ERR_BAD_ARG),
+    (dict(tokens=1 << 28), _lib.ERR_UNSUPPORTED)])
+def test_the_entry_point_refuses(more, status):
+    a = plain(**more)
+    assert _lib.lib().gptq_hip_attend(ctypes.byref(a), None, 0, None) == status
+
+
+def test_workspace():
+    lib = _lib.lib()
+    a = plain(max_context=30000, table_width=4096, table_stride=4096)
+    need = lib.gptq_hip_attention_workspace_bytes(ctypes.byref(a))
+    assert need > 65536
+    for ws, size in ((None, need), (0x1000, need - 1), (0x1008, need)):
+        assert lib.gptq_hip_attend(ctypes.byref(a), ws, size, None) == _lib.ERR_WORKSPACE
+    assert lib.gptq_hip_attention_workspace_bytes(None) == 0
+    assert lib.gptq_hip_attention_workspace_bytes(ctypes.byref(plain(tokens=0))) == 0
+    # a workspace stays within half a GiB of parts whatever the batch
+    for tokens, requests, context in ((1, 1, 1 << 20), (256, 256, 1 << 20), (8192, 1, 1 << 17), (4096, 4096, 4096)):
+        a = plain(tokens=tokens, requests=requests, max_context=context, table_width=1 << 16, table_stride=1 << 16)
+        assert lib.gptq_hip_attention_workspace_bytes(ctypes.byref(a)) <= (1 << 29) + (1 << 20)
+    assert lib.gptq_hip_attend(None, None, 0, None) == _lib.ERR_BAD_ARG

@@ -250,7 +250,7 @@ __device__ void join_parts(const AttentionParams &p, const QueryTile &q, int h, 
 }
 
 // rows_of_a_wave = 16 * RT rows of a tile; dims: the compiled width (64, 128 or 256) that covers dim
-int launch_attention_stream(const AttentionParams &p, int type, int rt, void *stream);
+int launch_attention_few(const AttentionParams &p, int type, int rt, void *stream);
 int launch_attention_tile(const AttentionParams &p, int type, void *stream);
 constexpr int kTileRows = 128;
 

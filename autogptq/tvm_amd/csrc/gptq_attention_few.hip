@@ -22,7 +22,7 @@ namespace gptq {
 
 // DP: compiled width, dims past p.dim are zero; RT: 16-row operands a wave holds
 template <typename E, int DP, int RT>
-__global__ __launch_bounds__(256) void attention_stream_kernel(const AttentionParams p)
+__global__ __launch_bounds__(256) void attention_few_kernel(const AttentionParams p)
 {
     typedef typename Vec<E>::e8 e8;
     constexpr int R = 16 * RT;
@@ -278,26 +278,26 @@ __global__ __launch_bounds__(256) void attention_stream_kernel(const AttentionPa
 }
 
 template <typename E>
-static void launch_stream(const AttentionParams &p, int rt, hipStream_t stream)
+static void launch_few(const AttentionParams &p, int rt, hipStream_t stream)
 {
     const dim3 grid((unsigned)((long long)p.kv_heads * p.tiles * p.splits));
-#define GPTQ_STREAM(DP, RT) hipLaunchKernelGGL((attention_stream_kernel<E, DP, RT>), grid, dim3(256), 0, stream, p)
+#define GPTQ_FEW(DP, RT) hipLaunchKernelGGL((attention_few_kernel<E, DP, RT>), grid, dim3(256), 0, stream, p)
     if (p.dim <= 64) {
-        if (rt == 1) GPTQ_STREAM(64, 1);
-        else GPTQ_STREAM(64, 2);
+        if (rt == 1) GPTQ_FEW(64, 1);
+        else GPTQ_FEW(64, 2);
     } else if (p.dim <= 128) {
-        if (rt == 1) GPTQ_STREAM(128, 1);
-        else GPTQ_STREAM(128, 2);
+        if (rt == 1) GPTQ_FEW(128, 1);
+        else GPTQ_FEW(128, 2);
     } else {
-        GPTQ_STREAM(256, 1);
+        GPTQ_FEW(256, 1);
     }
-#undef GPTQ_STREAM
+#undef GPTQ_FEW
 }
 
-int launch_attention_stream(const AttentionParams &p, int type, int rt, void *stream)
+int launch_attention_few(const AttentionParams &p, int type, int rt, void *stream)
 {
-    if (type == GPTQ_HIP_TYPE_FP16) launch_stream<_Float16>(p, rt, (hipStream_t)stream);
-    else launch_stream<__bf16>(p, rt, (hipStream_t)stream);
+    if (type == GPTQ_HIP_TYPE_FP16) launch_few<_Float16>(p, rt, (hipStream_t)stream);
+    else launch_few<__bf16>(p, rt, (hipStream_t)stream);
     return hipGetLastError() == hipSuccess ? GPTQ_HIP_OK : GPTQ_HIP_ERR_LAUNCH;
 }
 

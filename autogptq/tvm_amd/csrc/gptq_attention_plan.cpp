@@ -29,14 +29,14 @@ constexpr size_t kMostParts = (size_t)1 << 29;           // bytes that the parts
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 struct Division {
-    int rt = 0;       // 16-row operands a wave of the stream kernel, 0: the tile kernel
+    int rt = 0;       // 16-row operands a wave of the few-rows kernel, 0: the tile kernel
     int tiles = 0, splits = 1, chunk = 1;
     int rows() const { return rt ? 16 * rt : kTileRows; }
     int unit() const { return rt ? 256 : 64; }
 };
 
-// Rows of one request and key/value head (on average) up to which the stream kernel takes them.
-int stream_operands(long long rows, int dim)
+// Rows of one request and key/value head (on average) up to which the few-rows kernel takes them.
+int few_operands(long long rows, int dim)
 {
     if (rows <= 16) return 1;
     if (rows <= 32 && dim <= 128) return 2;
@@ -67,14 +67,14 @@ int plan(const gptq_hip_attention &a, Plan &pl)
     long long shared_parts = 0;
     if (a.prefix_length > 0) {
         Division &d = pl.shared;
-        d.rt = stream_operands(T * group, a.cache.dim);
+        d.rt = few_operands(T * group, a.cache.dim);
         d.tiles = (int)ceil_div(T * group, d.rows());
         divide(d, d.tiles * H, a.prefix_length, room);
         shared_parts = d.splits;
         if (d.tiles * H * d.splits >= 1ll << 31) return GPTQ_HIP_ERR_UNSUPPORTED;
     }
     Division &d = pl.own;
-    d.rt = stream_operands(ceil_div(T * group, B), a.cache.dim);
+    d.rt = few_operands(ceil_div(T * group, B), a.cache.dim);
     d.tiles = (int)(T * group / d.rows() + B);
     long long keys = (long long)a.table_width * a.cache.block_size;
     if (a.max_context > 0) keys = std::min<long long>(keys, a.max_context);
@@ -143,7 +143,7 @@ extern "C" int gptq_hip_attend(const gptq_hip_attention *a, void *workspace, siz
     p.c = a->scale * 1.44269504088896340736f;
     auto launch = [&](const gptq::Division &d) {
         p.tiles = d.tiles, p.splits = d.splits, p.chunk = d.chunk;
-        return d.rt ? gptq::launch_attention_stream(p, c.type, d.rt, stream) : gptq::launch_attention_tile(p, c.type, stream);
+        return d.rt ? gptq::launch_attention_few(p, c.type, d.rt, stream) : gptq::launch_attention_tile(p, c.type, stream);
     };
     if (a->prefix_length > 0) {
         p.shared = 1, p.prefix = a->prefix_length;

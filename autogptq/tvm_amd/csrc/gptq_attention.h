@@ -2,15 +2,15 @@
 //
 // Rows.  The query heads that share a key/value head are rows of one matrix: token t of a request and head g of the group
 // are row t * group + g, and a workgroup takes a tile of R consecutive rows of one request and one key/value head, so that
-// every key and value is loaded once for the whole group.  Request b of B owns the tiles from
-//   first_tile(b) = floor(starts[b] * group / R) + b:
-// the floors of two neighbours lie at least floor(rows / R) apart, and the + b adds the tile of a remainder.  The bound
-// floor(tokens * group / R) + B on the number of tiles, and the request of a tile, follow without any sum over requests;
-// tiles past a request's rows leave at once.
+// every key and value is loaded once for the whole group.
 //
 // Keys.  A tile sees the keys [0, ns) (sinks that its window has left behind) and [lo, hi) of its request.  The two are
 // walked as one list of n_seen keys; what single rows of the tile do not see in it is masked.  Nothing outside of the list
-// is read: block table entries there may hold anything.
+// is read: block table entries there may hold anything.  A short shared prefix may stand in front of the list, looked up in
+// a table of its own.
+//
+// Parts.  The keys of a tile may be divided among workgroups.  Each leaves m, l and o of its part in the workspace, and the
+// one that comes last joins them.
 //
 // Statistics.  Scores are kept in units of log2(e): p = 2^(c q.k - m) with c = scale * log2(e), m the running maximum, l
 // the sum of p and o the sum of p v, all in 32 bits.  p is rounded to the cache's type for the matrix instruction (the
@@ -24,109 +24,112 @@
 
 namespace gptq {
 
-constexpr int kMostKeys = 1 << 30;   // of a request: sums of positions and widths stay within 32 bits
+constexpr int kTileRows = 128;       // of a tile at most
+constexpr int kMostKeys = 1 << 29;   // of a request, a prefix, a window: sums of positions and widths stay within 32 bits
 
 struct AttentionParams {
     const void *q, *k, *v;
     void *out;
     const int32_t *tables, *starts, *contexts;
-    int *counters;     // one per (tile, key/value head): zero between calls
-    float *stats;      // [slot][row of tokens * heads][2]: m and l of a part
-    float *parts;      // [slot][row][dim]: o of a part
+    const int32_t *prefix_blocks;
+    int *counters;     // zero between calls
+    float *stats, *parts;        // m and l, and o, of the parts of a shared prefix: [part][row of tokens * heads][2 or dim]
+    float *own_stats, *own_parts;   // of a tile's own parts: as those, or (few-rows kernel) [place][row of the tile][2 or dim]
     int tokens, requests, heads, kv_heads, group, dim;
     int blocks, block_size, table_width;
     int window, sinks;
-    int shared;        // 1: every token sees the first `prefix` keys of the one table row, and the parts stay parts
+    int shared;        // 1: the launch computes the parts of a shared prefix of `prefix` keys
     int prefix;
+    int front;         // keys of a prefix that stands in front of every list
     int tiles, splits, chunk;   // tiles (bound), parts of a tile at most, keys of a part
-    int first_slot;    // parts of the shared prefix that stand before a tile's own
-    long long q_token, q_head, block_stride, slot_stride, head_stride, table_stride;   // in elements
+    int prefix_parts;  // parts of a shared prefix to be joined with a tile's own
+    int team, most_units;       // few-rows kernel: workgroups of a key/value head, units of a tile at most
+    long long q_token, q_head, head_stride, table_stride;   // in elements
+    uint32_t block_step, slot_step;   // of a cache, in units of 16 bytes
     float c;
+    uint32_t group_magic;    // x / group = x * magic >> 16 for x < group + kTileRows; 0: groups that are divided by
+    int block_shift;         // log2(block_size), or -1
 };
+
+// x / group for the rows of a tile, counted from its first token's
+__device__ __forceinline__ int tokens_of(const AttentionParams &p, int x)
+{
+    return p.group_magic ? (int)((uint32_t)x * p.group_magic >> 16) : x / p.group;
+}
 
 // A query tile: rows [row0, row0 + rows) of the request with the tokens [start, start + count), whose last one is at
 // position context - 1.
 struct QueryTile {
     int b, start, count, row0, rows;
     int position;      // of the request's first new token
-    int ns, lo, seen;  // the list of keys: [0, ns) and [lo, lo + seen - ns)
+    int front;         // the list of keys: [0, front) of a prefix, then [0, ns) and [lo, lo + seen - ns - front)
+    int ns, lo, seen;
     int t0, t1;        // first and last token of the tile
+    int g0;            // rows of the first token that belong to the tile before
 };
 
-template <int R>
-__device__ __forceinline__ bool find_tile(const AttentionParams &p, int tile, QueryTile &q)
+// keys of a request that a table can name
+__device__ __forceinline__ int held_keys(const AttentionParams &p)
 {
-    const int lane = threadIdx.x & 63;
-    int context;
-    if (p.shared) {
-        q.b = 0, q.start = 0, q.count = p.tokens, q.row0 = tile * R;
-        context = p.prefix;
-    } else {
-        int before = 0;
-        if (p.requests > 1) {
-            for (int b0 = 0; b0 < p.requests; b0 += 64) {
-                const int b = b0 + lane;
-                const bool there = b < p.requests;
-                const int s = there ? min(max(p.starts[b], 0), p.tokens) : 0;
-                before += __popcll(__ballot(there && (int)((uint32_t)s * (uint32_t)p.group / R) + b <= tile));
-            }
-            before = max(before, 1) - 1;
-        }
-        q.b = __builtin_amdgcn_readfirstlane(before);
-        // (what the tensors say is cut to what the other arguments allow: wrong lengths give wrong sums, not wrong addresses)
-        q.start = min(max(p.starts[q.b], 0), p.tokens);
-        q.count = min(max(p.starts[q.b + 1] - q.start, 0), p.tokens - q.start);
-        context = p.contexts[q.b];
-        q.row0 = (tile - ((int)((uint32_t)q.start * (uint32_t)p.group / R) + q.b)) * R;
-    }
-    const int all = q.count * p.group;
-    if (q.row0 < 0 || q.row0 >= all) return false;
-    q.rows = min(R, all - q.row0);
+    return (int)min((long long)p.table_width * p.block_size, (long long)kMostKeys);
+}
+
+// the rest of a tile whose request and rows are known
+template <bool SHARED>
+__device__ __forceinline__ void set_tile(const AttentionParams &p, QueryTile &q, int context)
+{
     q.t0 = q.row0 / p.group;
-    q.t1 = (q.row0 + q.rows - 1) / p.group;
-    if (p.shared) {
-        q.position = context, q.ns = 0, q.lo = 0, q.seen = context;
-        return true;
+    q.g0 = q.row0 - q.t0 * p.group;
+    q.t1 = q.t0 + tokens_of(p, q.g0 + q.rows - 1);
+    if (SHARED) {
+        q.position = context, q.ns = 0, q.lo = 0, q.seen = q.front = context;
+        return;
     }
     q.position = context - q.count;
-    const int held = (int)min((long long)p.table_width * p.block_size, (long long)kMostKeys);
-    const int hi = max(min(min(context, q.position + q.t1 + 1), held), 0);
+    const int hi = max(min(min(context, q.position + q.t1 + 1), held_keys(p)), 0);
     q.lo = p.window > 0 ? min(max(q.position + q.t0 - p.window + 1, 0), hi) : 0;
     q.ns = min(p.sinks, q.lo);
-    q.seen = q.ns + hi - q.lo;
-    return true;
+    q.front = p.front;
+    q.seen = q.front + q.ns + hi - q.lo;
 }
 
-// The keys of a part: [begin, end) of the list, and how many parts the tile has.  A list that is longer than the host
-// expected (splits * chunk) has longer parts.
-__device__ __forceinline__ int tile_parts(const AttentionParams &p, int seen, int unit, int &chunk)
+// position of entry i of the list; entries of the front have negative ones
+__device__ __forceinline__ int key_position(const QueryTile &q, int i)
 {
-    chunk = max(p.chunk, ((seen + p.splits - 1) / p.splits + unit - 1) / unit * unit);
-    return max(1, (seen + chunk - 1) / chunk);
+    const int own = i - q.front;
+    return own < q.ns ? own : own - q.ns + q.lo;
 }
 
-// position of entry i of the list
-__device__ __forceinline__ int key_position(const QueryTile &q, int i) { return i < q.ns ? i : i - q.ns + q.lo; }
-
-// Whether a row at position `pos` sees entry i of the list, whose part ends at `end`.  (Without branches: every entry of a
-// mixed tile is asked.)
-__device__ __forceinline__ bool sees(const AttentionParams &p, const QueryTile &q, int i, int end, int pos)
+// What a row at position `pos` sees of a part of the list that ends at `end`: the entries below `high` that are not below
+// `low`, and all below `free` (a prefix, sinks that the window has left behind, and what of the sinks it has not).
+struct Sight {
+    int low, high, free;
+    __device__ __forceinline__ bool sees(int i) const { return (i < high) & ((i >= low) | (i < free)); }
+};
+__device__ __forceinline__ Sight sight(const AttentionParams &p, const QueryTile &q, int end, int pos)
 {
-    const int at = key_position(q, i);
-    const int oldest = p.window > 0 ? pos - p.window : -1;      // the newest position that is no longer in the window
-    const bool seen = (at <= pos) & ((at > oldest) | (at < p.sinks));
-    return (i < end) & (seen | (p.shared != 0));
+    const int own = q.front + q.ns - q.lo;      // entry of position 0, were it in the window
+    return {p.window > 0 ? pos - p.window + 1 + own : -kMostKeys, min(max(pos + 1 + own, q.front), end), max(q.front + q.ns, p.sinks + own)};
 }
 
-// where the row of key position `at` stands in a cache, in units of 16 bytes (head 0).  A block that the cache does not
-// have counts as its first: the values are then undefined, the addresses are not.
-__device__ __forceinline__ uint32_t key_row(const AttentionParams &p, const int32_t *table, int at)
+// whether every row from the tile's token at position `first` to the one at `last` sees entries [i0, i1) of the list
+__device__ __forceinline__ bool all_see(const AttentionParams &p, const QueryTile &q, int i0, int i1, int first, int last)
 {
-    const uint32_t j = (uint32_t)at / (uint32_t)p.block_size;
-    const uint32_t slot = (uint32_t)at - j * (uint32_t)p.block_size;
-    uint32_t block = (uint32_t)table[j];
+    return i1 <= q.front || (key_position(q, i1 - 1) <= first &&
+                             (p.window <= 0 || (i0 >= q.front + q.ns && key_position(q, i0) > last - p.window)));
+}
+
+// Where the row of entry i stands in a cache, in units of 16 bytes (head 0).  A block that the cache does not have counts
+// as its first: the values are then undefined, the addresses are not.
+__device__ __forceinline__ uint32_t key_row(const AttentionParams &p, const QueryTile &q, const int32_t *table, int i)
+{
+    const bool front = i < q.front;
+    const uint32_t at = (uint32_t)(front ? i : key_position(q, i));
+    const uint32_t j = p.block_shift >= 0 ? at >> p.block_shift : at / (uint32_t)p.block_size;
+    const uint32_t slot = at - j * (uint32_t)p.block_size;
+    uint32_t block = (uint32_t)(front ? p.prefix_blocks : table)[j];
     if (block >= (uint32_t)p.blocks) block = 0;
-    return (uint32_t)(((unsigned long long)block * (unsigned long long)p.block_stride + slot * (unsigned long long)p.slot_stride) >> 3);
+    return block * p.block_step + slot * p.slot_step;   // (the host has seen to it that no row passes 2^32)
 }
 
 // fp16 or bf16 operands of the matrix instructions
@@ -181,11 +184,19 @@ __device__ __forceinline__ f2 load_stats(const float *src)
     return __builtin_bit_cast(f2, __hip_atomic_load((const unsigned long long *)src, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
-// row r of a tile -> row of the part arrays and of the output: token * heads + head
+// row r of a tile: its token (in the request) and query head
+__device__ __forceinline__ void token_head(const AttentionParams &p, const QueryTile &q, int h, int r, int &t, int &head)
+{
+    const int x = q.g0 + r, dt = tokens_of(p, x);
+    t = q.t0 + dt;
+    head = h * p.group + x - dt * p.group;
+}
+// ... and its row in the part arrays and the output: token * heads + head
 __device__ __forceinline__ long long out_row(const AttentionParams &p, const QueryTile &q, int h, int r)
 {
-    const int row = q.row0 + r, t = row / p.group, g = row - t * p.group;
-    return (long long)(q.start + t) * p.heads + h * p.group + g;
+    int t, head;
+    token_head(p, q, h, r, t, head);
+    return (long long)(q.start + t) * p.heads + head;
 }
 
 // 4 results of a row as 4 values of the output's type, 8 bytes
@@ -199,59 +210,86 @@ __device__ __forceinline__ void store_row4(void *out, long long at, f4 o)
 __device__ __forceinline__ bool last_part(const AttentionParams &p, int counter, int parts, int *flag)
 {
     if (parts > 1) return arrive_last(p.counters + counter, parts, flag);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the caller's barrier follows)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what this thread stored is there for the others
+    __syncthreads();
     return true;
 }
 
-// The last workgroup of a tile joins its parts, in their order: m = max m_i, l = sum l_i 2^(m_i - m), o likewise.
-// `weights`: LDS for rows * slots floats (at most kJoinWeights; longer lists go through it in rounds of rows).
-constexpr int kJoinWeights = 4096;
-template <typename E, int THREADS>
-__device__ void join_parts(const AttentionParams &p, const QueryTile &q, int h, int slots, float *weights)
+// Four values of a row with the row's statistics, and parts that join them: m = max m_i, l = sum l_i 2^(m_i - m), o likewise.
+struct Sum {
+    float m, l;
+    f4 o;
+    __device__ __forceinline__ void add(float mi, float li, f4 oi)
+    {
+        const float up = fmaxf(m, mi), to = reference(up), f = __builtin_amdgcn_exp2f(m - to), w = __builtin_amdgcn_exp2f(mi - to);
+        m = up;
+        l = f * l + w * li;
+        o = f * o + w * oi;
+    }
+    __device__ __forceinline__ f4 result() const { return o * (l > 0.0f ? 1.0f / l : 0.0f); }
+};
+// The parts first, first + step, ... < count.  `stat` and `part` give the address of a part's statistics and of its four
+// values; eight parts are asked for at a time.  Coherent: parts of other workgroups of this launch, past the caches.
+template <bool COHERENT, typename Stat, typename Part>
+__device__ __forceinline__ void add_parts(Sum &x, int first, int step, int count, Stat stat, Part part)
+{
+    for (int s0 = first; s0 < count; s0 += 8 * step) {
+        f2 ml[8];
+        f4 o[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const int s = min(s0 + u * step, count - 1);
+            ml[u] = COHERENT ? load_stats(stat(s)) : *(const f2 *)stat(s);
+            o[u] = COHERENT ? load_partial(part(s)) : *(const f4 *)part(s);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; u++)
+            if (s0 + u * step < count) x.add(ml[u][0], ml[u][1], o[u]);
+    }
+}
+// The parts of a shared prefix, which the launch before left.
+__device__ __forceinline__ void add_prefix(const AttentionParams &p, Sum &x, long long at, int d)
 {
     const long long all = (long long)p.tokens * p.heads;
-    const int quads = p.dim / 4;
-    const int round = max(1, min(q.rows, kJoinWeights / slots));
-    for (int r0 = 0; r0 < q.rows; r0 += round) {
-        const int rows = min(round, q.rows - r0);
+    add_parts<false>(x, 0, 1, p.prefix_parts, [&](int s) { return p.stats + 2 * (s * all + at); },
+                     [&](int s) { return p.parts + (s * all + at) * p.dim + d; });
+}
+
+// Joins the `parts` parts of a tile, in their order, behind those of a shared prefix.  place(part, row of the tile) is a row of
+// own_stats and own_parts.  Where a tile has few rows several threads share a value's parts.  `lds`: THREADS Sums.
+template <typename E, int THREADS, typename Place>
+__device__ void join_parts(const AttentionParams &p, const QueryTile &q, int h, int parts, void *lds, Place place)
+{
+    Sum *half_way = (Sum *)lds;
+    const int quads = p.dim / 4, items = q.rows * quads;
+    int teams = 1;
+    while (8 * teams < parts && 2 * teams * items <= THREADS) teams *= 2;
+    const int team = teams > 1 ? threadIdx.x / items : 0;
+    for (int i = threadIdx.x - team * items; i < items && team < teams; i += teams > 1 ? items : THREADS) {
+        const int r = i / quads, d = (i - r * quads) * 4;
+        const long long at = out_row(p, q, h, r);
+        Sum x = {kNone, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+        if (team == 0) add_prefix(p, x, at, d);
+        add_parts<true>(x, team, teams, parts, [&](int s) { return p.own_stats + 2 * place(s, r); },
+                        [&](int s) { return p.own_parts + place(s, r) * p.dim + d; });
+        if (teams > 1) half_way[threadIdx.x] = x;
+        else store_row4<E>(p.out, at * p.dim + d, x.result());
+    }
+    if (teams > 1) {
         __syncthreads();
-        // 16 lanes a row
-        for (int r = threadIdx.x / 16; r < rows; r += THREADS / 16) {
-            const long long at = out_row(p, q, h, r0 + r);
-            float m = kNone, l = 0.0f;
-            for (int s = threadIdx.x % 16; s < slots; s += 16) m = fmaxf(m, load_stats(p.stats + 2 * (s * all + at))[0]);
-            for (int d = 8; d >= 1; d /= 2) m = fmaxf(m, __shfl_xor(m, d, 16));
-            const float ref = reference(m);
-            for (int s = threadIdx.x % 16; s < slots; s += 16) {
-                const f2 ml = load_stats(p.stats + 2 * (s * all + at));
-                const float w = __builtin_amdgcn_exp2f(ml[0] - ref);
-                weights[r * slots + s] = w;
-                l += w * ml[1];
+        if ((int)threadIdx.x < items) {
+            Sum x = half_way[threadIdx.x];
+            for (int t = 1; t < teams; t++) {
+                const Sum y = half_way[t * items + threadIdx.x];
+                x.add(y.m, y.l, y.o);
             }
-            for (int d = 8; d >= 1; d /= 2) l += __shfl_xor(l, d, 16);
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            for (int s = threadIdx.x % 16; s < slots; s += 16) weights[r * slots + s] *= inv;
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < rows * quads; i += THREADS) {
-            const int r = i / quads, d = (i - r * quads) * 4;
-            const long long at = out_row(p, q, h, r0 + r);
-            f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-            for (int s = 0; s < slots; s++) {
-                const float w = weights[r * slots + s];
-                const f4 x = load_partial(p.parts + (s * all + at) * p.dim + d);
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[e] += w * x[e];
-            }
-            store_row4<E>(p.out, at * p.dim + d, o);
+            const int r = threadIdx.x / quads, d = (threadIdx.x - r * quads) * 4;
+            store_row4<E>(p.out, out_row(p, q, h, r) * p.dim + d, x.result());
         }
     }
 }
 
-// rows_of_a_wave = 16 * RT rows of a tile; dims: the compiled width (64, 128 or 256) that covers dim
 int launch_attention_few(const AttentionParams &p, int type, int rt, void *stream);
 int launch_attention_tile(const AttentionParams &p, int type, void *stream);
-constexpr int kTileRows = 128;
 
 }  // namespace gptq

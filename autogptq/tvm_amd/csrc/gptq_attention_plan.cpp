@@ -28,11 +28,13 @@ constexpr size_t kMostParts = (size_t)1 << 29;           // bytes that the parts
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
+// How a launch is divided among workgroups.
 struct Division {
-    int rt = 0;       // 16-row operands a wave of the few-rows kernel, 0: the tile kernel
-    int tiles = 0, splits = 1, chunk = 1;
+    int rt = 0;        // 16-row operands a wave of the few-rows kernel, 0: the tile kernel
+    int tiles = 0;     // of rows: all there can be
+    int splits = 1, chunk = 1;          // parts of a tile at most, keys of a part
+    int team = 1, most_units = 1;       // few-rows kernel on own contexts: see there
     int rows() const { return rt ? 16 * rt : kTileRows; }
-    int unit() const { return rt ? 256 : 64; }
 };
 
 // Rows of one request and key/value head (on average) up to which the few-rows kernel takes them.
@@ -42,49 +44,70 @@ int few_operands(long long rows, int dim)
     if (rows <= 32 && dim <= 128) return 2;
     return 0;
 }
+// workgroups of the few-rows kernel that a CU holds (registers)
+int few_resident(int rt, int dim) { return dim > 128 ? 1 : (rt == 1 ? 3 : 2) + (dim <= 64); }
 
-// How a call whose tiles see up to `keys` keys is divided: `busy` workgroups would run without a division.
+// Parts of tiles that see `keys` keys: enough that `busy` workgroups fill the chip twice over (the two that a CU holds), none
+// of fewer than 256 keys.  (723 tokens of 7 heads behind contexts of up to 9001, dim 80: 256 workgroups 107 us, 512 87, 1024
+// 90; 512 rows behind a prefix of 16384: 91, 94, 121.)
 void divide(Division &d, long long busy, long long keys, long long most_parts)
 {
-    const long long want = d.rt ? 1024 : 512;
-    long long s = std::min(ceil_div(want, busy), ceil_div(keys, 256));
-    if (d.rt) s = std::max(s, ceil_div(keys, 4096));     // requests of different lengths end together
-    s = std::max(1ll, std::min(s, most_parts));
-    d.chunk = (int)(ceil_div(ceil_div(std::max(keys, 1ll), s), d.unit()) * d.unit());
+    const long long unit = d.rt ? 256 : 64;
+    const long long s = std::max(1ll, std::min({ceil_div(512, busy), ceil_div(keys, 256), most_parts}));
+    d.chunk = (int)(ceil_div(ceil_div(std::max(keys, 1ll), s), unit) * unit);
     d.splits = (int)std::max(1ll, ceil_div(keys, d.chunk));
 }
 
+constexpr long long kMostPrefixParts = 1024;
+
 struct Plan {
     Division own, shared;
-    size_t slots = 0, rows = 0, bytes = 0;
+    bool prefix = false;             // a launch of its own for the shared prefix
+    size_t prefix_rows = 0, own_rows = 0, bytes = 0;     // rows of the parts in the workspace
 };
 
 int plan(const gptq_hip_attention &a, Plan &pl)
 {
     const long long group = a.heads / a.cache.heads, T = a.tokens, B = a.requests, H = a.cache.heads;
-    const size_t part = (size_t)T * a.heads * (a.cache.dim * 4 + 8);
-    const long long room = std::max<long long>(1, (long long)(kMostParts / part));
-    long long shared_parts = 0;
-    if (a.prefix_length > 0) {
-        Division &d = pl.shared;
-        d.rt = few_operands(T * group, a.cache.dim);
-        d.tiles = (int)ceil_div(T * group, d.rows());
-        divide(d, d.tiles * H, a.prefix_length, room);
-        shared_parts = d.splits;
-        if (d.tiles * H * d.splits >= 1ll << 31) return GPTQ_HIP_ERR_UNSUPPORTED;
-    }
+    const long long all = T * a.heads, row = a.cache.dim * 4 + 8;
+    const long long room = std::max(1ll, (long long)(kMostParts / (size_t)(all * row)));
     Division &d = pl.own;
     d.rt = few_operands(ceil_div(T * group, B), a.cache.dim);
     d.tiles = (int)(T * group / d.rows() + B);
+    if (d.tiles * H >= 1ll << 24) return GPTQ_HIP_ERR_UNSUPPORTED;
     long long keys = (long long)a.table_width * a.cache.block_size;
     if (a.max_context > 0) keys = std::min<long long>(keys, a.max_context);
     if (a.window > 0) keys = std::min<long long>(keys, (long long)a.window + a.sinks + d.rows() / group + 1);
-    const bool counted = d.tiles * H <= (long long)(kAttentionCounters / 4);
-    divide(d, std::max(B, ceil_div(T * group, d.rows())) * H, keys, counted ? room : 1);
-    if ((long long)d.tiles * H * d.splits >= 1ll << 31) return GPTQ_HIP_ERR_UNSUPPORTED;
-    pl.rows = (size_t)T * a.heads;
-    pl.slots = d.splits > 1 || shared_parts ? (size_t)(shared_parts + d.splits) : 0;
-    pl.bytes = pl.slots ? kAttentionCounters + (pl.slots * pl.rows * 8 + 255) / 256 * 256 + pl.slots * pl.rows * a.cache.dim * 4 : 0;
+    // A short prefix stands in front of every request's keys instead of taking a launch of its own: 8 requests behind 1000 keys
+    // 16 us against 23, 16 behind 2000 24 / 26, 8 behind 8000 (262 MB re-read) 28 / 33, 64 behind 2000 (524 MB) 54 / 32 (32
+    // heads in groups of 4, dim 128).
+    const bool alone = B == 1 && T * group <= d.rows();      // no other reader
+    pl.prefix = a.prefix_length > 0 &&
+                !(d.rt && (alone || (long long)d.tiles * a.prefix_length * H * a.cache.dim * 4 <= 256ll << 20));
+    if (pl.prefix) {
+        Division &s = pl.shared;
+        s.rt = few_operands(T * group, a.cache.dim);
+        s.tiles = (int)ceil_div(T * group, s.rows());
+        divide(s, s.tiles * H, a.prefix_length, std::min(room, kMostPrefixParts));
+        pl.prefix_rows = (size_t)(s.splits * all);
+    } else {
+        keys += a.prefix_length;
+    }
+    if (d.rt) {
+        const long long most = B * (T * group / d.rows() + 1);    // tiles, whatever the lengths on the GPU say
+        if (most > 1ll << 30) return GPTQ_HIP_ERR_UNSUPPORTED;
+        d.most_units = (int)std::min((1ll << 30) / most, 1ll << 20);
+        const long long units = (d.tiles + 0ll) * std::max(1ll, ceil_div(keys, 256));
+        d.team = (int)std::max(1ll, std::min(256ll * few_resident(d.rt, a.cache.dim) / H, units));
+        if (d.team * H > (long long)(kAttentionCounters / 4)) return GPTQ_HIP_ERR_UNSUPPORTED;
+        pl.own_rows = (size_t)(2 * d.team * H * d.rows());
+    } else {
+        divide(d, std::max(B, ceil_div(T * group, d.rows())) * H, keys,
+               d.tiles * H <= (long long)(kAttentionCounters / 4) ? room : 1);
+        if (d.splits > 1 || pl.prefix) pl.own_rows = (size_t)(d.splits * all);
+    }
+    const size_t rows = pl.prefix_rows + pl.own_rows;
+    pl.bytes = rows ? kAttentionCounters + (rows * 8 + 255) / 256 * 256 + rows * a.cache.dim * 4 : 0;
     return GPTQ_HIP_OK;
 }
 
@@ -132,26 +155,32 @@ extern "C" int gptq_hip_attend(const gptq_hip_attention *a, void *workspace, siz
     const gptq_hip_cache &c = a->cache;
     p.q = a->q, p.k = c.k, p.v = c.v, p.out = a->out;
     if (pl.bytes) {
+        const size_t rows = pl.prefix_rows + pl.own_rows;
         p.counters = (int *)workspace;
         p.stats = (float *)((char *)workspace + gptq::kAttentionCounters);
-        p.parts = (float *)((char *)p.stats + (pl.slots * pl.rows * 8 + 255) / 256 * 256);
+        p.parts = (float *)((char *)p.stats + (rows * 8 + 255) / 256 * 256);
+        p.own_stats = p.stats + 2 * pl.prefix_rows;
+        p.own_parts = p.parts + pl.prefix_rows * c.dim;
     }
     p.tokens = a->tokens, p.requests = a->requests, p.heads = a->heads, p.kv_heads = c.heads, p.group = a->heads / c.heads;
     p.dim = c.dim, p.blocks = c.blocks, p.block_size = c.block_size;
     p.q_token = a->q_token_stride, p.q_head = a->q_head_stride;
-    p.block_stride = c.block_stride, p.slot_stride = c.slot_stride, p.head_stride = c.head_stride;
+    p.head_stride = c.head_stride, p.block_step = (uint32_t)(c.block_stride / 8), p.slot_step = (uint32_t)(c.slot_stride / 8);
     p.c = a->scale * 1.44269504088896340736f;
+    if ((long long)p.group * (p.group + gptq::kTileRows) < 65536) p.group_magic = 65535u / (uint32_t)p.group + 1u;
+    p.block_shift = c.block_size & (c.block_size - 1) ? -1 : __builtin_ctz((unsigned)c.block_size);
     auto launch = [&](const gptq::Division &d) {
-        p.tiles = d.tiles, p.splits = d.splits, p.chunk = d.chunk;
+        p.tiles = d.tiles, p.splits = d.splits, p.chunk = d.chunk, p.team = d.team, p.most_units = d.most_units;
         return d.rt ? gptq::launch_attention_few(p, c.type, d.rt, stream) : gptq::launch_attention_tile(p, c.type, stream);
     };
-    if (a->prefix_length > 0) {
+    p.prefix_blocks = a->prefix_blocks;
+    if (pl.prefix) {
         p.shared = 1, p.prefix = a->prefix_length;
-        p.tables = a->prefix_blocks;
-        p.table_width = (int)gptq::ceil_div(a->prefix_length, c.block_size);
         rc = launch(pl.shared);
         if (rc != GPTQ_HIP_OK) return rc;
-        p.shared = 0, p.first_slot = pl.shared.splits;
+        p.shared = 0, p.prefix_parts = pl.shared.splits;
+    } else {
+        p.front = a->prefix_length;
     }
     p.tables = a->tables, p.table_width = a->table_width, p.table_stride = a->table_stride;
     p.starts = a->starts, p.contexts = a->contexts;

@@ -4,18 +4,65 @@
 // wave, and walks the tile's keys KT at a time; keys and values go through LDS, so that a row from the cache is read once
 // for 128 rows.
 //
-//   staging   direct requests from the cache into LDS (16 bytes a lane, no registers), one tile of keys ahead, two buffers
-//             and one barrier a tile.  The rows' places come from a list in LDS that the first KT threads keep two tiles
-//             ahead of the requests and whose block table entries they ask for three tiles ahead.
-//   LDS       rows as they lie in the cache; the 16-byte chunks of row r stand at chunk ^ r (keys) and chunk ^ 2 r (values),
-//             which spreads the lanes of a read over all banks.  The swizzle is in the requests' source addresses.
 //   S^T = K Q^T    32 x 32 results: a lane holds 16 keys of one row for each 32 keys, the maximum and the sum of a row are
 //             the lane's own and one exchange with lane ^ 32.
 //   O^T += V^T P^T  the sum over keys runs in the order in which the lane already holds p (keys 4 h + 8 x + y of 16, h =
 //             lane / 32); the operand of V in the same order comes from LDS through the transposing read.
+//   order     the products of S run one tile of keys ahead of the softmax and the products with V, so that a wave has matrix
+//             instructions to issue between its exponentials.
+//   staging   direct requests from the cache into LDS (16 bytes a lane, no registers), two buffers for keys and two for
+//             values, one barrier a tile: while tile n is summed, the keys of n + 2 and the values of n + 1 arrive.  The
+//             rows' places come from a ring of lists in LDS, filled every four tiles by all waves at once, a tile each (one
+//             wave doing it for every tile held the others up at every barrier).
+//   LDS       rows as they lie in the cache; the 16-byte chunks of row r stand at chunk ^ r (keys) and chunk ^ 2 r (values),
+//             which spreads the lanes of a read over all banks.  The swizzle is in the requests' source addresses.
+#include <type_traits>
+
 #include "gptq_attention.h"
 
 namespace gptq {
+
+// The tile of a workgroup.  Request b owns the tiles from first_tile(b) = floor(starts[b] * group / R) + b: the floors of two
+// neighbours lie at least floor(rows / R) apart, and the + b adds the tile of a remainder.  So the bound
+// floor(tokens * group / R) + requests on the number of tiles, and the request of a tile, follow without any sum over
+// requests.  False for a tile past its request's rows.
+template <int R>
+__device__ __forceinline__ bool find_tile(const AttentionParams &p, int tile, QueryTile &q)
+{
+    const int lane = threadIdx.x & 63;
+    int context = p.prefix;
+    if (p.shared) {
+        q.b = 0, q.start = 0, q.count = p.tokens, q.row0 = tile * R;
+    } else {
+        // what the tensors say is cut to what the other arguments allow: wrong lengths give wrong sums, not wrong addresses
+        int before = 0;
+        for (int b0 = 0; b0 < p.requests; b0 += 64) {
+            const int b = b0 + lane;
+            const bool there = b < p.requests;
+            const int s = there ? min(max(p.starts[b], 0), p.tokens) : 0;
+            before += __popcll(__ballot(there && (int)((uint32_t)s * (uint32_t)p.group / R) + b <= tile));
+        }
+        q.b = __builtin_amdgcn_readfirstlane(max(before, 1) - 1);
+        q.start = min(max(p.starts[q.b], 0), p.tokens);
+        q.count = min(max(p.starts[q.b + 1] - q.start, 0), p.tokens - q.start);
+        context = p.contexts[q.b];
+        q.row0 = (tile - ((int)((uint32_t)q.start * (uint32_t)p.group / R) + q.b)) * R;
+    }
+    const int all = q.count * p.group;
+    if (q.row0 < 0 || q.row0 >= all) return false;
+    q.rows = min(R, all - q.row0);
+    if (p.shared) set_tile<true>(p, q, context);
+    else set_tile<false>(p, q, context);
+    return true;
+}
+
+// The keys of a part, and how many parts the tile has.  A list that is longer than the host expected (splits * chunk) has
+// longer parts.
+__device__ __forceinline__ int tile_parts(const AttentionParams &p, int seen, int unit, int &chunk)
+{
+    chunk = max(p.chunk, ((seen + p.splits - 1) / p.splits + unit - 1) / unit * unit);
+    return max(1, (seen + chunk - 1) / chunk);
+}
 
 // 16 bytes of `src` to LDS at lds + 16 * lane.  Inline assembly, so that the compiler does not wait for every outstanding
 // request before each read of LDS; the kernel waits for them at its barrier.
@@ -30,11 +77,12 @@ template <typename E>
 __device__ __forceinline__ u2 read_turned(uint32_t at)
 {
     typedef short s4 __attribute__((ext_vector_type(4)));
-    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at));
+    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(uintptr_t)at));
 }
-__device__ __forceinline__ u4 read16(uint32_t at) { return *(const __attribute__((address_space(3))) u4 *)at; }
+__device__ __forceinline__ u4 read16(uint32_t at) { return *(const __attribute__((address_space(3))) u4 *)(uintptr_t)at; }
 
-template <typename E, int DP, int KT>
+// DP: row of LDS (a power of two), DC: dims that are computed, the multiple of 16 that covers p.dim
+template <typename E, int DP, int DC, int KT>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(const AttentionParams p)
 {
     typedef typename Vec<E>::e8 e8;
@@ -42,63 +90,68 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
     constexpr int RP = 256 / CH;            // rows that the workgroup requests at a time
     constexpr int PASSES = KT / RP;
     constexpr int TILE = KT * DP * 2;       // bytes of a tile of keys or values
-    constexpr int KA = KT / 32, DT = DP / 32;
+    constexpr int KA = KT / 32, SX = DC / 16, DT = (DC + 31) / 32, PX = KT / 16;
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
-    uint32_t *list = (uint32_t *)(smem + 4 * TILE);     // [2][KT]
-    int *flag = (int *)(list + 2 * KT);
+    uint32_t *list = (uint32_t *)(smem + 4 * TILE);     // [8][KT]
+    int *flag = (int *)(list + 8 * KT);
 
     const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int h = blockIdx.x % p.kv_heads, rest = blockIdx.x / p.kv_heads;
     // the last rows of a request see the most keys: they come first
-    const int tile = p.tiles - 1 - rest % p.tiles, split = rest / p.tiles;
+    const int h = blockIdx.x % p.kv_heads, tile = p.tiles - 1 - blockIdx.x / p.kv_heads, split = blockIdx.y;
     QueryTile q;
     if (!find_tile<kTileRows>(p, tile, q)) return;
     int chunk;
     const int parts = tile_parts(p, q.seen, KT, chunk);
     if (split >= parts) return;
     const int begin = split * chunk, end = min(q.seen, begin + chunk);
-    const int32_t *table = p.tables + (p.shared ? 0 : (long long)q.b * p.table_stride);
+    const int32_t *table = p.tables + (long long)q.b * p.table_stride;
     const char *kbase = (const char *)p.k + (long long)h * p.head_stride * 2;
     const char *vbase = (const char *)p.v + (long long)h * p.head_stride * 2;
 
     const int r = 32 * wave + col;
-    const int qrow = q.row0 + min(r, q.rows - 1), qt = qrow / p.group, hg = h * p.group + qrow - qt * p.group;
+    int qt, hg;
+    token_head(p, q, h, min(r, q.rows - 1), qt, hg);
     const int pos = q.position + qt;
-    e8 qf[DP / 16];
+    e8 qf[SX];
     {
         const char *src = (const char *)p.q + ((long long)(q.start + qt) * p.q_token + (long long)hg * p.q_head) * 2;
 #pragma unroll
-        for (int s = 0; s < DP / 16; s++) {
-            const int d = 16 * s + 8 * hh;
-            u4 x = {0u, 0u, 0u, 0u};
-            if (d < p.dim) x = *(const u4 *)(src + d * 2);
-            qf[s] = __builtin_bit_cast(e8, x);
+        for (int x = 0; x < SX; x++) {
+            const int d = 16 * x + 8 * hh;
+            u4 y = {0u, 0u, 0u, 0u};
+            if (d < p.dim) y = *(const u4 *)(src + d * 2);
+            qf[x] = __builtin_bit_cast(e8, y);
         }
     }
     // positions of this wave's first and last row
     const bool works = 32 * wave < q.rows;
-    const int pos_first = q.position + (q.row0 + min(32 * wave, q.rows - 1)) / p.group;
-    const int pos_last = q.position + (q.row0 + min(32 * wave + 31, q.rows - 1)) / p.group;
+    const int pos_first = q.position + q.t0 + tokens_of(p, q.g0 + min(32 * wave, q.rows - 1));
+    const int pos_last = q.position + q.t0 + tokens_of(p, q.g0 + min(32 * wave + 31, q.rows - 1));
 
+    const Sight my = sight(p, q, end, pos);
     const int tiles = (end - begin + KT - 1) / KT;
+    // Rows of tile n for the requests: four tiles at a time, one a wave.  A thread's rows of a tile stand side by side.
     auto look_up = [&](int n) {
-        return key_row(p, table, key_position(q, min(begin + n * KT + (int)threadIdx.x, end - 1)));
+        return key_row(p, q, table, min(begin + min(n, tiles - 1) * KT + min(lane, KT - 1), end - 1));
     };
-    // this thread's chunk of the rows it requests (RP is a multiple of 8, CH at most 32: the swizzle may change with the pass)
+    auto enter = [&](int n, uint32_t row) {
+        if (lane < KT) list[(n & 7) * KT + lane % RP * PASSES + lane / RP] = row;
+    };
+    typedef uint32_t Rows __attribute__((ext_vector_type(PASSES)));
+    // this thread's chunk of the rows it requests
     const int myrow = threadIdx.x / CH, place = threadIdx.x % CH;
-    auto request = [&](int n) {
-        const uint32_t *rows = list + (n & 1) * KT;
-        const uint32_t kdst = lds + (n & 1) * TILE + wave * 1024, vdst = kdst + 2 * TILE;
+    auto rows_of = [&](int n) { return *(const Rows *)(list + (n & 7) * KT + myrow * PASSES); };
+    auto request = [&](const Rows &rows, const char *from, uint32_t to, int twist) {
 #pragma unroll
         for (int j = 0; j < PASSES; j++) {
-            const int row = j * RP + myrow;
-            const int kc = place ^ (row & (CH - 1)), vc = place ^ ((2 * row) & (CH - 1));
-            const unsigned long long at = (unsigned long long)rows[row] * 16;
-            if (p.dim == DP || kc * 8 < p.dim) request16(kbase + at + kc * 16, __builtin_amdgcn_readfirstlane(kdst + j * 4096));
-            if (p.dim == DP || vc * 8 < p.dim) request16(vbase + at + vc * 16, __builtin_amdgcn_readfirstlane(vdst + j * 4096));
+            const int c = place ^ ((twist * (j * RP + myrow)) & (CH - 1));
+            if (p.dim == DP || c * 8 < p.dim)
+                request16(from + (unsigned long long)rows[j] * 16 + c * 16, __builtin_amdgcn_readfirstlane(to + wave * 1024 + j * 4096));
         }
     };
+    auto request_keys = [&](const Rows &rows, int buf) { request(rows, kbase, lds + buf * TILE, 1); };
+    auto request_values = [&](const Rows &rows, int buf) { request(rows, vbase, lds + (2 + buf) * TILE, 2); };
     auto meet = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
     float m = kNone, l = 0.0f;
@@ -106,106 +159,140 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) o[dt] = (f16)(0.0f);
 
+    // Where this lane's operands stand in the first buffers.  The rest of an address is an immediate: 32 keys on, or 8 or 16
+    // values, leave the swizzle as it is.
+    uint32_t kat[SX], vat[2][DT];
+#pragma unroll
+    for (int x = 0; x < SX; x++) kat[x] = lds + col * (DP * 2) + (((2 * x + hh) ^ (col & (CH - 1))) * 16);
+#pragma unroll
+    for (int up = 0; up < 2; up++)
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) {
+            const int key = 8 * up + 4 * hh + (col & 15) / 4, c = 4 * dt + 2 * (col >> 4) + (col & 3) / 2;
+            vat[up][dt] = lds + 2 * TILE + key * (DP * 2) + ((c ^ ((2 * key) & (CH - 1))) * 16) + (col & 1) * 8;
+        }
+    static_assert(CH <= 32 && (CH <= 16 || KT == 32), "the swizzle repeats within the rows that an immediate steps over");
+
+    f16 s[KA];
+    // S^T for the keys in the buffer BUF
+    auto scores = [&](auto buf) {
+        constexpr int BUF = decltype(buf)::value * TILE;
+#pragma unroll
+        for (int a = 0; a < KA; a++) s[a] = (f16)(0.0f);
+        // (32 keys at a time: two sums in turn, or one after the other where that is all there are)
+#pragma unroll
+        for (int x0 = 0; x0 < SX; x0 += 4) {
+            u4 kf[4][KA];
+#pragma unroll
+            for (int x = x0; x < SX && x < x0 + 4; x++)
+#pragma unroll
+                for (int a = 0; a < KA; a++) kf[x - x0][a] = read16(kat[x] + (BUF + 32 * a * DP * 2));
+#pragma unroll
+            for (int x = x0; x < SX && x < x0 + 4; x++)
+#pragma unroll
+                for (int a = 0; a < KA; a++) s[a] = mfma32(__builtin_bit_cast(e8, kf[x - x0][a]), qf[x], s[a]);
+        }
+    };
+    // softmax of tile n, whose scores are in s, and its products with the values in the buffer BUF; then the next scores
+    auto sum = [&](int n, auto buf) {
+        constexpr int BUF = decltype(buf)::value * TILE;
+        u2 vf[PX][DT][2];
+        auto read_values = [&](int x) {
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int up = 0; up < 2; up++) vf[x][dt][up] = read_turned<E>(vat[up][dt] + (BUF + 16 * x * DP * 2));
+        };
+        read_values(0);
+        __builtin_amdgcn_sched_barrier(0);
+        const int v0 = begin + n * KT, v1 = min(v0 + KT, end);
+        if (v0 + KT > end || !all_see(p, q, v0, v1, pos_first, pos_last)) {
+#pragma unroll
+            for (int a = 0; a < KA; a++)
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (!my.sees(v0 + 4 * hh + 32 * a + 8 * (i / 4) + i % 4)) s[a][i] = kNone;
+        }
+        float top = kNone;
+#pragma unroll
+        for (int a = 0; a < KA; a++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, s[a][i]);
+        top = max_halves(top) * p.c;
+        if (__ballot(top > m + 8.0f)) {
+            const float up = fmaxf(m, top);
+            const float down = __builtin_amdgcn_exp2f(m - reference(up));
+            m = up;
+            l *= down;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) o[dt] *= down;
+        }
+        const float ref = reference(m);
+#pragma unroll
+        for (int x = 0; x < PX; x++) {
+            if (x + 1 < PX) read_values(x + 1);
+            f8 pr;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                pr[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x / 2][(x & 1) * 8 + j], p.c, -ref));
+                l += pr[j];
+            }
+            const e8 pe = __builtin_convertvector(pr, e8);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                const u4 y = {vf[x][dt][0][0], vf[x][dt][0][1], vf[x][dt][1][0], vf[x][dt][1][1]};
+                o[dt] = mfma32(__builtin_bit_cast(e8, y), pe, o[dt]);
+            }
+        }
+        scores(std::integral_constant<int, 1 - decltype(buf)::value>());
+    };
+
     if (tiles > 0) {
-        if (p.dim < DP) {   // the chunks that no request fills
-            for (int x = threadIdx.x; x < 4 * TILE / 16; x += 256) ((u4 *)smem)[x] = (u4){0u, 0u, 0u, 0u};
+        if (p.dim < DC) {   // the chunks of keys that no request fills (of values they only reach dims that are not stored)
+            for (int x = threadIdx.x; x < 2 * TILE / 16; x += 256) ((u4 *)smem)[x] = (u4){0u, 0u, 0u, 0u};
         }
-        uint32_t next = 0;
-        if (threadIdx.x < KT) {
-            list[threadIdx.x] = look_up(0);
-            list[KT + threadIdx.x] = look_up(min(1, tiles - 1));
-            next = look_up(min(2, tiles - 1));
-        }
+        enter(wave, look_up(wave));
+        uint32_t next = look_up(4 + wave);
         meet();
-        request(0);
+        Rows keys = rows_of(0);
+        request_keys(keys, 0);
+        request_values(keys, 0);
+        keys = rows_of(1);
+        if (1 < tiles) request_keys(keys, 1);
         meet();
-        for (int n = 0; n < tiles; n++) {
-            if (n + 1 < tiles) request(n + 1);
-            if (threadIdx.x < KT && n + 2 < tiles) {
-                list[(n & 1) * KT + threadIdx.x] = next;    // (of tile n + 2; tile n's places were read before the last barrier)
-                next = look_up(min(n + 3, tiles - 1));
+        if (works) scores(std::integral_constant<int, 0>());
+        meet();
+        // tile n: the keys of n + 2 go where those of n were, the values of n + 1 where those of n - 1 were
+        auto step = [&](int n, auto buf) {
+            constexpr int BUF = decltype(buf)::value;
+            if (n + 1 < tiles) request_values(keys, 1 - BUF);
+            if (n + 2 < tiles) {
+                keys = rows_of(n + 2);
+                request_keys(keys, BUF);
             }
-            const int v0 = begin + n * KT, v1 = min(v0 + KT, end);
-            // does this wave see any of it, does every row see all of it?
-            const int at0 = key_position(q, v0), at1 = key_position(q, v1 - 1);
-            bool any = works, clear = v0 + KT <= end;
-            if (!p.shared) {
-                any = any && at0 <= pos_last && (p.window <= 0 || v0 < q.ns || at1 > pos_first - p.window);
-                clear = clear && at1 <= pos_first && (p.window <= 0 || (v0 >= q.ns && at0 > pos_last - p.window));
+            if ((n & 3) == 0) {      // (the places of tile n + 4 are read two tiles from here at the earliest)
+                enter(n + 4 + wave, next);
+                next = look_up(n + 8 + wave);
             }
-            if (any) {
-                const uint32_t kb = lds + (n & 1) * TILE, vb = kb + 2 * TILE;
-                f16 s[KA];
-#pragma unroll
-                for (int a = 0; a < KA; a++) {
-                    s[a] = (f16)(0.0f);
-                    const int key = 32 * a + col;
-                    const uint32_t krow = kb + key * (DP * 2);
-#pragma unroll
-                    for (int x = 0; x < DP / 16; x++) {
-                        const u4 kf = read16(krow + (((2 * x + hh) ^ (key & (CH - 1))) * 16));
-                        s[a] = mfma32(__builtin_bit_cast(e8, kf), qf[x], s[a]);
-                    }
-                }
-                if (!clear) {
-#pragma unroll
-                    for (int a = 0; a < KA; a++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const bool seen = sees(p, q, v0 + 32 * a + 4 * hh + 8 * (i / 4) + i % 4, end, pos);
-                            s[a][i] = seen ? s[a][i] : kNone;
-                        }
-                }
-                float top = kNone;
-#pragma unroll
-                for (int a = 0; a < KA; a++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) top = fmaxf(top, s[a][i]);
-                top = max_halves(top) * p.c;
-                if (__ballot(top > m + 8.0f)) {
-                    const float up = fmaxf(m, top);
-                    const float down = __builtin_amdgcn_exp2f(m - reference(up));
-                    m = up;
-                    l *= down;
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++) o[dt] *= down;
-                }
-                const float ref = reference(m);
-                e8 pe[KT / 16];
-#pragma unroll
-                for (int x = 0; x < KT / 16; x++) {
-                    f8 pr;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        pr[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x / 2][(x & 1) * 8 + j], p.c, -ref));
-                        l += pr[j];
-                    }
-                    pe[x] = __builtin_convertvector(pr, e8);
-                }
-#pragma unroll
-                for (int x = 0; x < KT / 16; x++) {
-                    const int key = 16 * x + 4 * hh + (col & 15) / 4;
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++) {
-                        const int c16 = 4 * dt + 2 * (col >> 4) + (col & 3) / 2;
-                        const u2 lo = read_turned<E>(vb + key * (DP * 2) + ((c16 ^ ((2 * key) & (CH - 1))) * 16) + (col & 1) * 8);
-                        const u2 hi = read_turned<E>(vb + (key + 8) * (DP * 2) + ((c16 ^ ((2 * (key + 8)) & (CH - 1))) * 16) + (col & 1) * 8);
-                        o[dt] = mfma32(__builtin_bit_cast(e8, ((u4){lo[0], lo[1], hi[0], hi[1]})), pe[x], o[dt]);
-                    }
-                }
-            }
+            if (works) sum(n, buf);
             meet();
+        };
+        for (int n = 0; n < tiles; n += 2) {
+            step(n, std::integral_constant<int, 0>());
+            if (n + 1 < tiles) step(n + 1, std::integral_constant<int, 1>());
         }
     }
 
     l = add_halves(l);
-    const bool whole = parts == 1 && p.first_slot == 0 && !p.shared;
+    const bool whole = parts == 1 && p.prefix_parts == 0 && !p.shared;
+    const long long all = (long long)p.tokens * p.heads;
+    float *stats = p.shared ? p.stats : p.own_stats, *outs = p.shared ? p.parts : p.own_parts;
     if (r < q.rows) {
         const long long at = out_row(p, q, h, r);
-        const long long all = (long long)p.tokens * p.heads;
-        const long long slot = (long long)(p.first_slot + split) * all;
+        const long long slot = split * all;
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        if (!whole && hh == 0) store_stats(p.stats + 2 * (slot + at), m, l);
+        if (!whole && hh == 0) store_stats(stats + 2 * (slot + at), m, l);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -214,22 +301,26 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
                 if (d >= p.dim) continue;
                 const f4 y = {o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
                 if (whole) store_row4<E>(p.out, at * p.dim + d, y * inv);
-                else store_partial(p.parts + (slot + at) * p.dim + d, y);
+                else store_partial(outs + (slot + at) * p.dim + d, y);
             }
     }
     if (whole || p.shared) return;
     if (last_part(p, tile * p.kv_heads + h, parts, flag))
-        join_parts<E, 256>(p, q, h, p.first_slot + parts, (float *)smem);
+        join_parts<E, 256>(p, q, h, parts, (float *)smem, [&](int part, int r) { return part * all + out_row(p, q, h, r); });
 }
 
 template <typename E>
 static void launch_tile(const AttentionParams &p, hipStream_t stream)
 {
-    const dim3 grid((unsigned)((long long)p.kv_heads * p.tiles * p.splits));
-#define GPTQ_TILE(DP, KT) hipLaunchKernelGGL((attention_tile_kernel<E, DP, KT>), grid, dim3(256), 4 * KT * DP * 2 + 2 * KT * 4 + 16, stream, p)
-    if (p.dim <= 64) GPTQ_TILE(64, 64);
-    else if (p.dim <= 128) GPTQ_TILE(128, 64);
-    else GPTQ_TILE(256, 32);
+    const dim3 grid((unsigned)(p.kv_heads * p.tiles), (unsigned)p.splits);
+#define GPTQ_TILE(DP, DC, KT) \
+    hipLaunchKernelGGL((attention_tile_kernel<E, DP, DC, KT>), grid, dim3(256), 4 * KT * DP * 2 + 8 * KT * 4 + 16, stream, p)
+    if (p.dim <= 64) GPTQ_TILE(64, 64, 64);
+    else if (p.dim <= 80) GPTQ_TILE(128, 80, 64);
+    else if (p.dim <= 96) GPTQ_TILE(128, 96, 64);
+    else if (p.dim <= 128) GPTQ_TILE(128, 128, 64);
+    else if (p.dim <= 192) GPTQ_TILE(256, 192, 32);
+    else GPTQ_TILE(256, 256, 32);
 #undef GPTQ_TILE
 }
 

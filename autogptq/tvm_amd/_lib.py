@@ -101,7 +101,7 @@ class Route(ctypes.Structure):
 
 
 TYPE_FP16, TYPE_BF16 = 0, 1
-CACHE_MAX_REQUESTS = 16384
+CACHE_MAX_REQUESTS = 8192
 
 
 class Cache(ctypes.Structure):

@@ -38,15 +38,13 @@ def cache_tables(lengths: torch.Tensor, counts: torch.Tensor, tables: torch.Tens
     (int32, on the GPU).  The blocks these need come from the front of ``free_blocks``, requests in order, and are entered
     into ``tables`` [requests, width] in place.  ``tokens`` is the sum of the counts, which the caller knows without asking
     the GPU.  If ``taken`` exceeds ``free_blocks``, or a table its width, the tokens that found no place have slot -1."""
-    _need_native()
-    return CacheTables(*torch.ops.gptq_hip.cache_tables(lengths, counts, tables, free_blocks, tokens, block_size))
+    return CacheTables(*_call("cache_tables", lengths, counts, tables, free_blocks, tokens, block_size))
 
 
 def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor) -> None:
     """``k`` and ``v`` [tokens, kv_heads, dim] (columns of a fused product as they are) into ``slots`` of the cache; tokens
     with slot -1 are skipped."""
-    _need_native()
-    torch.ops.gptq_hip.cache_write(k, v, k_cache, v_cache, slots)
+    _call("cache_write", k, v, k_cache, v_cache, slots)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, tables: torch.Tensor, starts: torch.Tensor,
@@ -58,9 +56,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     sees may be given back: their table entries are not read.  A token that sees nothing gets zeros.  Query head n reads
     key/value head n // (heads / kv_heads).  ``max_context``: the longest context as the host knows it, by which the work is
     divided (0: the tables' width); results do not depend on it beyond the order of sums.  ``scale``: 1 / sqrt(dim) if None."""
-    _need_native()
-    return torch.ops.gptq_hip.paged_attention(q, k_cache, v_cache, tables, starts, contexts, max_context, window, sinks,
-                                              _scale(scale))
+    return _call("paged_attention", q, k_cache, v_cache, tables, starts, contexts, max_context, window, sinks, _scale(scale))
 
 
 def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_blocks: torch.Tensor,
@@ -69,9 +65,8 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     """``paged_attention`` where every request stands behind the same ``prefix_length`` tokens, whose blocks are
     ``prefix_blocks``: all tokens see all of them, and they are read once for the batch.  ``tables``, ``contexts`` and
     ``max_context`` count a request's own tokens only."""
-    _need_native()
-    return torch.ops.gptq_hip.shared_prefix_attention(q, k_cache, v_cache, prefix_blocks, prefix_length, tables, starts,
-                                                      contexts, max_context, _scale(scale))
+    return _call("shared_prefix_attention", q, k_cache, v_cache, prefix_blocks, prefix_length, tables, starts, contexts,
+                 max_context, _scale(scale))
 
 
 def _scale(scale: Optional[float]) -> float:
@@ -82,10 +77,16 @@ def _scale(scale: Optional[float]) -> float:
     return scale
 
 
-def _need_native():
+def _call(name: str, *args):
+    """The operator by its C function (csrc/python_call.cpp), or by torch.ops where that leaves it to the dispatcher."""
     if not ops.NATIVE_OPS:
         raise RuntimeError("the operator library is missing or stale: build it with `python -m autogptq.tvm_amd.build` "
                            "(there is no fallback path)")
+    if not torch.compiler.is_compiling():
+        result = getattr(ops.CALL, name)(*args)
+        if result is not NotImplemented:
+            return result
+    return getattr(torch.ops.gptq_hip, name)(*args)
 
 
 __all__ = ["CacheTables", "cache_tables", "cache_write", "paged_attention", "shared_prefix_attention"]

@@ -6,6 +6,7 @@
 
 #include <mutex>
 #include <optional>
+#include <tuple>
 
 #include "gptq_hip.h"
 
@@ -66,5 +67,15 @@ Tensor dispatch(const Bound &q, const Tensor &x);
 
 // the operators' checks of a layer's tensors (devices, dtypes, shapes), once, when they are bound
 void check_bound(const Bound &q);
+
+// the serving operators torch.ops.gptq_hip.* of binding_attention.cpp
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> cache_tables(const Tensor &lengths, const Tensor &counts, const Tensor &tables,
+                                                                const Tensor &free_blocks, int64_t tokens, int64_t block_size);
+void cache_write(const Tensor &k, const Tensor &v, const Tensor &k_cache, const Tensor &v_cache, const Tensor &slots);
+Tensor paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &tables, const Tensor &starts,
+                       const Tensor &contexts, int64_t max_context, int64_t window, int64_t sinks, double scale);
+Tensor shared_prefix_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &prefix_blocks,
+                               int64_t prefix_length, const Tensor &tables, const Tensor &starts, const Tensor &contexts,
+                               int64_t max_context, double scale);
 
 }  // namespace gptq_torch

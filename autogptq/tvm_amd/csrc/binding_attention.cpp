@@ -2,6 +2,7 @@
 // libgptq_hip.so as dispatcher-visible operators (see binding.cpp for the products).  They check devices, dtypes, shapes and
 // strides, allocate what they return, and launch on the current HIP stream of the tensors' device.
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
@@ -91,7 +92,14 @@ void raised(int rc, const char *what)
     TORCH_CHECK(rc == GPTQ_HIP_OK, what, " failed: ", gptq_hip_strerror(rc), " [status ", rc, "]");
 }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> cache_tables(const Tensor &lengths, const Tensor &counts, const Tensor &tables,
+Tensor fresh(at::IntArrayRef sizes, const Tensor &like)
+{
+    return at::detail::empty_cuda(sizes, like.scalar_type(), like.device(), std::nullopt);
+}
+
+}  // namespace
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gptq_torch::cache_tables(const Tensor &lengths, const Tensor &counts, const Tensor &tables,
                                                                 const Tensor &free_blocks, int64_t tokens, int64_t block_size)
 {
     need_ints(lengths, "lengths", -1, lengths);
@@ -104,19 +112,30 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> cache_tables(const Tensor &le
     TORCH_CHECK(B <= GPTQ_HIP_CACHE_MAX_REQUESTS, "at most ", GPTQ_HIP_CACHE_MAX_REQUESTS, " requests, got ", B);
     TORCH_CHECK(free_blocks.size(0) < (1LL << 31), "too many free blocks");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(lengths.device());
-    const auto ints = lengths.options();
-    Tensor starts = at::empty({B + 1}, ints), contexts = at::empty({B}, ints), slots = at::empty({tokens}, ints),
-           positions = at::empty({tokens}, ints), taken = at::empty({1}, ints);
+    // the five results are parts of one allocation (five would cost the host as much as the launch)
+    const int64_t sizes[5] = {B + 1, B, tokens, tokens, 1};
+    int64_t all = 0;
+    for (int64_t n : sizes) all += (n + 3) / 4 * 4;
+    const Tensor memory = fresh({all}, lengths);
+    Tensor out[5];
+    int64_t at = 0;
+    for (int i = 0; i < 5; i++) {
+        out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(memory.storage()), memory.key_set(), memory.dtype());
+        out[i].unsafeGetTensorImpl()->set_storage_offset(at);
+        out[i].unsafeGetTensorImpl()->set_sizes_contiguous({sizes[i]});
+        at += (sizes[i] + 3) / 4 * 4;
+    }
+    const Tensor &starts = out[0], &contexts = out[1], &slots = out[2], &positions = out[3], &taken = out[4];
     raised(gptq_hip_cache_tables((const int32_t *)lengths.data_ptr(), (const int32_t *)counts.data_ptr(), (int32_t *)tables.data_ptr(),
                                  row_stride(tables), (int)tables.size(1), (const int32_t *)free_blocks.data_ptr(),
                                  (int)free_blocks.size(0), (int)B, (int)tokens, (int)block_size, (int32_t *)starts.data_ptr(),
                                  (int32_t *)contexts.data_ptr(), (int32_t *)slots.data_ptr(), (int32_t *)positions.data_ptr(),
                                  (int32_t *)taken.data_ptr(), current_stream(lengths)),
            "gptq_hip_cache_tables");
-    return {starts, contexts, slots, positions, taken};
+    return {out[0], out[1], out[2], out[3], out[4]};
 }
 
-void cache_write(const Tensor &k, const Tensor &v, const Tensor &k_cache, const Tensor &v_cache, const Tensor &slots)
+void gptq_torch::cache_write(const Tensor &k, const Tensor &v, const Tensor &k_cache, const Tensor &v_cache, const Tensor &slots)
 {
     on_gpu(k_cache, "k_cache", k_cache);
     const gptq_hip_cache c = describe(k_cache, v_cache);
@@ -139,7 +158,7 @@ void cache_write(const Tensor &k, const Tensor &v, const Tensor &k_cache, const 
            "gptq_hip_cache_write");
 }
 
-Tensor attend(const char *what, const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &prefix_blocks,
+static Tensor attend(const char *what, const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &prefix_blocks,
               int64_t prefix_length, const Tensor &tables, const Tensor &starts, const Tensor &contexts, int64_t max_context,
               int64_t window, int64_t sinks, double scale)
 {
@@ -169,7 +188,7 @@ Tensor attend(const char *what, const Tensor &q, const Tensor &k_cache, const Te
                     prefix_blocks.size(0));
         a.prefix_blocks = (const int32_t *)prefix_blocks.data_ptr();
     }
-    Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+    Tensor out = fresh(q.sizes(), q);
     if (q.size(0) == 0) return out;
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
     const Tensor qs = loadable(q);
@@ -185,13 +204,13 @@ Tensor attend(const char *what, const Tensor &q, const Tensor &k_cache, const Te
     return out;
 }
 
-Tensor paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &tables, const Tensor &starts,
+Tensor gptq_torch::paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &tables, const Tensor &starts,
                        const Tensor &contexts, int64_t max_context, int64_t window, int64_t sinks, double scale)
 {
     return attend("gptq_hip_attend", q, k_cache, v_cache, Tensor(), 0, tables, starts, contexts, max_context, window, sinks, scale);
 }
 
-Tensor shared_prefix_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &prefix_blocks,
+Tensor gptq_torch::shared_prefix_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &prefix_blocks,
                                int64_t prefix_length, const Tensor &tables, const Tensor &starts, const Tensor &contexts,
                                int64_t max_context, double scale)
 {
@@ -199,7 +218,7 @@ Tensor shared_prefix_attention(const Tensor &q, const Tensor &k_cache, const Ten
                   max_context, 0, 0, scale);
 }
 
-}  // namespace
+using namespace gptq_torch;
 
 TORCH_LIBRARY_FRAGMENT(gptq_hip, m)
 {

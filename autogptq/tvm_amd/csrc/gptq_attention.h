@@ -184,6 +184,21 @@ __device__ __forceinline__ f2 load_stats(const float *src)
     return __builtin_bit_cast(f2, __hip_atomic_load((const unsigned long long *)src, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
+// Four values of a part, and its statistics.  Parts of a shared prefix are read by the next launch and need no way past the
+// caches.
+template <bool COHERENT>
+__device__ __forceinline__ void put_part(float *to, f4 x)
+{
+    if constexpr (COHERENT) store_partial(to, x);
+    else *(f4 *)to = x;
+}
+template <bool COHERENT>
+__device__ __forceinline__ void put_stats(float *to, float m, float l)
+{
+    if constexpr (COHERENT) store_stats(to, m, l);
+    else *(f2 *)to = (f2){m, l};
+}
+
 // row r of a tile: its token (in the request) and query head
 __device__ __forceinline__ void token_head(const AttentionParams &p, const QueryTile &q, int h, int r, int &t, int &head)
 {

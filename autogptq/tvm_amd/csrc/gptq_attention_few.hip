@@ -365,8 +365,8 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                     store_row4<E>(p.out, at_row * p.dim + d, x.result());
                 } else {
                     const long long to = SHARED ? blockIdx.y * all + at_row : mine + row;
-                    store_partial((SHARED ? p.parts : p.own_parts) + to * p.dim + d, total);
-                    if (d == 0) store_stats((SHARED ? p.stats : p.own_stats) + 2 * to, top, sum);
+                    put_part<!SHARED>((SHARED ? p.parts : p.own_parts) + to * p.dim + d, total);
+                    if (d == 0) put_stats<!SHARED>((SHARED ? p.stats : p.own_stats) + 2 * to, top, sum);
                 }
             }
         }

@@ -47,16 +47,19 @@ int few_operands(long long rows, int dim)
 // workgroups of the few-rows kernel that a CU holds (registers)
 int few_resident(int rt, int dim) { return dim > 128 ? 1 : (rt == 1 ? 3 : 2) + (dim <= 64); }
 
-// Parts of tiles that see `keys` keys: enough that `busy` workgroups fill the chip twice over (the two that a CU holds), none
-// of fewer than 256 keys.  (723 tokens of 7 heads behind contexts of up to 9001, dim 80: 256 workgroups 107 us, 512 87, 1024
-// 90; 512 rows behind a prefix of 16384: 91, 94, 121.)
-void divide(Division &d, long long busy, long long keys, long long most_parts)
+// Parts of tiles that see `keys` keys: enough that `busy` workgroups become `want`, none of fewer than 256 keys.
+void divide(Division &d, long long want, long long busy, long long keys, long long most_parts)
 {
     const long long unit = d.rt ? 256 : 64;
-    const long long s = std::max(1ll, std::min({ceil_div(512, busy), ceil_div(keys, 256), most_parts}));
+    const long long s = std::max(1ll, std::min({ceil_div(want, busy), ceil_div(keys, 256), most_parts}));
     d.chunk = (int)(ceil_div(ceil_div(std::max(keys, 1ll), s), unit) * unit);
     d.splits = (int)std::max(1ll, ceil_div(keys, d.chunk));
 }
+// Own contexts on the tile kernel: the two workgroups that a CU holds, since they differ in length (723 tokens of 7 heads behind
+// contexts of up to 9001, dim 80: 256 workgroups 107 us, 512 87, 1024 90).  A shared prefix: parts of one length, which the
+// next launch reads again, so one a CU (512 rows behind 16384 keys: 256 workgroups 80 us, 512 84, 1024 111); rows that fit the
+// few-rows kernel two.
+constexpr long long kOwnWorkgroups = 512, kPrefixWorkgroups = 256;
 
 constexpr long long kMostPrefixParts = 1024;
 
@@ -78,9 +81,10 @@ int plan(const gptq_hip_attention &a, Plan &pl)
     long long keys = (long long)a.table_width * a.cache.block_size;
     if (a.max_context > 0) keys = std::min<long long>(keys, a.max_context);
     if (a.window > 0) keys = std::min<long long>(keys, (long long)a.window + a.sinks + d.rows() / group + 1);
-    // A short prefix stands in front of every request's keys instead of taking a launch of its own: 8 requests behind 1000 keys
-    // 16 us against 23, 16 behind 2000 24 / 26, 8 behind 8000 (262 MB re-read) 28 / 33, 64 behind 2000 (524 MB) 54 / 32 (32
-    // heads in groups of 4, dim 128).
+    // A short prefix stands in front of every request's keys instead of taking a launch of its own, which costs 4 us and less
+    // as the tiles read it again (32 heads in groups of 4, dim 128): 8 requests behind 1000 keys 11.3 us against 15.4, 16
+    // behind 1000 14.1 / 17.5, 64 behind 250 17.1 / 22.0, 8 behind 4000 17.2 / 17.8, 16 behind 2000 21.5 / 18.0, 32 behind 1000
+    // 23.8 / 18.9.
     const bool alone = B == 1 && T * group <= d.rows();      // no other reader
     pl.prefix = a.prefix_length > 0 &&
                 !(d.rt && (alone || (long long)d.tiles * a.prefix_length * H * a.cache.dim * 4 <= 256ll << 20));
@@ -88,7 +92,7 @@ int plan(const gptq_hip_attention &a, Plan &pl)
         Division &s = pl.shared;
         s.rt = few_operands(T * group, a.cache.dim);
         s.tiles = (int)ceil_div(T * group, s.rows());
-        divide(s, s.tiles * H, a.prefix_length, std::min(room, kMostPrefixParts));
+        divide(s, s.rt ? 2 * kPrefixWorkgroups : kPrefixWorkgroups, s.tiles * H, a.prefix_length, std::min(room, kMostPrefixParts));
         pl.prefix_rows = (size_t)(s.splits * all);
     } else {
         keys += a.prefix_length;
@@ -102,7 +106,7 @@ int plan(const gptq_hip_attention &a, Plan &pl)
         if (d.team * H > (long long)(kAttentionCounters / 4)) return GPTQ_HIP_ERR_UNSUPPORTED;
         pl.own_rows = (size_t)(2 * d.team * H * d.rows());
     } else {
-        divide(d, std::max(B, ceil_div(T * group, d.rows())) * H, keys,
+        divide(d, kOwnWorkgroups, std::max(B, ceil_div(T * group, d.rows())) * H, keys,
                d.tiles * H <= (long long)(kAttentionCounters / 4) ? room : 1);
         if (d.splits > 1 || pl.prefix) pl.own_rows = (size_t)(d.splits * all);
     }

@@ -292,7 +292,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
         const long long at = out_row(p, q, h, r);
         const long long slot = split * all;
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        if (!whole && hh == 0) store_stats(stats + 2 * (slot + at), m, l);
+        if (!whole && hh == 0) p.shared ? put_stats<false>(stats + 2 * (slot + at), m, l) : put_stats<true>(stats + 2 * (slot + at), m, l);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -301,7 +301,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
                 if (d >= p.dim) continue;
                 const f4 y = {o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
                 if (whole) store_row4<E>(p.out, at * p.dim + d, y * inv);
-                else store_partial(outs + (slot + at) * p.dim + d, y);
+                else if (p.shared) put_part<false>(outs + (slot + at) * p.dim + d, y);
+                else put_part<true>(outs + (slot + at) * p.dim + d, y);
             }
     }
     if (whole || p.shared) return;

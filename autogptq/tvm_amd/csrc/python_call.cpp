@@ -23,6 +23,8 @@
 
 #include <new>
 
+#include <tuple>
+
 #include "binding.h"
 
 namespace {
@@ -274,7 +276,117 @@ PyObject *install(PyObject *, PyObject *cls)
     END_HANDLE_TH_ERRORS
 }
 
-PyMethodDef functions[] = {{"aside", aside, METH_VARARGS, "aside(fn, *args): fn(*args), hidden from tracing and dispatch modes."},
+// ---- the serving operators
+// The same functions as torch.ops.gptq_hip.*, called with plain tensors and without the dispatcher, whose handling of ten
+// arguments costs as much as the shorter of these calls run (cache_tables for 64 requests 9.5 us a call through it, 5.5 so).
+// They return NotImplemented where something else wants to see the operator: a tensor subclass, a dispatch mode, a tracer.
+struct Arguments {
+    PyObject *const *args;
+    bool plain = true;
+    Arguments(PyObject *const *a, Py_ssize_t n, Py_ssize_t expected) : args(a)
+    {
+        TORCH_CHECK_TYPE(n == expected, expected, " arguments are expected, got ", n);
+        plain = !c10::impl::TorchDispatchModeTLS::any_modes_set() && !torch::jit::tracer::isTracing();
+    }
+    // (a reference to the caller's tensor, which its arguments keep alive)
+    const Tensor &tensor(int i)
+    {
+        TORCH_CHECK_TYPE(THPVariable_Check(args[i]), "argument ", i, " must be a tensor");
+        plain = plain && THPVariable_CheckExact(args[i]);
+        return THPVariable_Unpack(args[i]);
+    }
+    int64_t integer(int i) const
+    {
+        const long long x = PyLong_AsLongLong(args[i]);
+        if (x == -1 && PyErr_Occurred()) throw python_error();
+        return x;
+    }
+    double real(int i) const
+    {
+        const double x = PyFloat_AsDouble(args[i]);
+        if (x == -1.0 && PyErr_Occurred()) throw python_error();
+        return x;
+    }
+};
+
+PyObject *call_cache_tables(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    Arguments a(args, n, 6);
+    const Tensor &lengths = a.tensor(0), &counts = a.tensor(1), &tables = a.tensor(2), &free_blocks = a.tensor(3);
+    const int64_t tokens = a.integer(4), block_size = a.integer(5);
+    if (!a.plain) Py_RETURN_NOTIMPLEMENTED;
+    Tensor out[5];
+    {
+        const WithoutInterpreter free;
+        std::tie(out[0], out[1], out[2], out[3], out[4]) = cache_tables(lengths, counts, tables, free_blocks, tokens, block_size);
+    }
+    THPObjectPtr result(PyTuple_New(5));
+    if (!result) return nullptr;
+    for (int i = 0; i < 5; i++) {
+        PyObject *t = THPVariable_Wrap(std::move(out[i]));
+        if (!t) return nullptr;
+        PyTuple_SET_ITEM(result.get(), i, t);
+    }
+    return result.release();
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *call_cache_write(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    Arguments a(args, n, 5);
+    const Tensor &k = a.tensor(0), &v = a.tensor(1), &k_cache = a.tensor(2), &v_cache = a.tensor(3), &slots = a.tensor(4);
+    if (!a.plain) Py_RETURN_NOTIMPLEMENTED;
+    {
+        const WithoutInterpreter free;
+        cache_write(k, v, k_cache, v_cache, slots);
+        // (what the dispatcher does for arguments that are written)
+        for (const Tensor *t : {&k_cache, &v_cache})
+            if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    }
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *call_paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    Arguments a(args, n, 10);
+    const Tensor &q = a.tensor(0), &k = a.tensor(1), &v = a.tensor(2), &tables = a.tensor(3), &starts = a.tensor(4), &contexts = a.tensor(5);
+    const int64_t most = a.integer(6), window = a.integer(7), sinks = a.integer(8);
+    const double scale = a.real(9);
+    if (!a.plain) Py_RETURN_NOTIMPLEMENTED;
+    Tensor out;
+    {
+        const WithoutInterpreter free;
+        out = paged_attention(q, k, v, tables, starts, contexts, most, window, sinks, scale);
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *call_shared_prefix_attention(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    Arguments a(args, n, 10);
+    const Tensor &q = a.tensor(0), &k = a.tensor(1), &v = a.tensor(2), &blocks = a.tensor(3), &tables = a.tensor(5), &starts = a.tensor(6),
+                 &contexts = a.tensor(7);
+    const int64_t length = a.integer(4), most = a.integer(8);
+    const double scale = a.real(9);
+    if (!a.plain) Py_RETURN_NOTIMPLEMENTED;
+    Tensor out;
+    {
+        const WithoutInterpreter free;
+        out = shared_prefix_attention(q, k, v, blocks, length, tables, starts, contexts, most, scale);
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+#define GPTQ_FAST(NAME) {#NAME, (PyCFunction)(void (*)(void))call_##NAME, METH_FASTCALL, "torch.ops.gptq_hip." #NAME " on plain tensors, else NotImplemented."}
+PyMethodDef functions[] = {GPTQ_FAST(cache_tables), GPTQ_FAST(cache_write), GPTQ_FAST(paged_attention), GPTQ_FAST(shared_prefix_attention),
+                           {"aside", aside, METH_VARARGS, "aside(fn, *args): fn(*args), hidden from tracing and dispatch modes."},
                            {"install", install, METH_O, "Makes the call in C the one of a QuantLinear class."}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "gptq_hip_call", "the QuantLinear call in C", -1, functions};
 

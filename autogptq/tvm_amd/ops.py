@@ -394,6 +394,11 @@ def _meta_dequant(qweight, qzeros, scales, g_idx, bits, group_size):
     return scales.new_empty((qweight.shape[0] * 32 // bits, qweight.shape[1]), dtype=torch.float16)
 
 
+def _meta_cache_tables(lengths, counts, tables, free_blocks, tokens, block_size):
+    B = lengths.shape[0]
+    return tuple(lengths.new_empty(n) for n in (B + 1, B, tokens, tokens, 1))
+
+
 # The module call in C (csrc/python_call.cpp, an extension module in the operator library): BoundCall and install();
 # None without the built library.
 CALL = None
@@ -457,6 +462,11 @@ def _register_torch_ops():
     meta.impl("gemm_sorted", _meta_gemm_sorted)
     meta.impl("gemm_tiled", _meta_gemm_tiled)
     meta.impl("dequant", _meta_dequant)
+    if native:      # (the operators of attention.py have no Python form)
+        meta.impl("cache_tables", _meta_cache_tables)
+        meta.impl("cache_write", lambda k, v, k_cache, v_cache, slots: None)
+        meta.impl("paged_attention", lambda q, *args: q.new_empty(q.shape))
+        meta.impl("shared_prefix_attention", lambda q, *args: q.new_empty(q.shape))
     keep.append(meta)
     return keep
 

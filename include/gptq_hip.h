@@ -376,13 +376,13 @@ typedef struct gptq_hip_cache {
  *   tables int32 [requests, table_width], rows table_stride apart: read, and new entries written
  *   starts int32 [requests + 1]        out: new tokens before each request, and all of them
  *   contexts int32 [requests]          out: lengths + counts
- *   slots, positions int32 [tokens]    out: cache slot and position of every new token; tokens = the room in the two (a caller
+ *   slots, positions int32 [tokens]    out, 16-byte aligned: cache slot and position of every new token; tokens = the room in the two (a caller
  *                                      who knows the lengths knows the sum); entries past the last new token are -1
  *   taken int32 [1]                    out: blocks needed.  More than free_count: the tokens without a block got slot -1
  * Tokens that lie past a table's width get slot -1 too.  Up to GPTQ_HIP_CACHE_MAX_REQUESTS requests
  * (GPTQ_HIP_ERR_UNSUPPORTED beyond).  One launch; the same inputs give the same results however often it runs.
  */
-#define GPTQ_HIP_CACHE_MAX_REQUESTS 16384
+#define GPTQ_HIP_CACHE_MAX_REQUESTS 8192
 int gptq_hip_cache_tables(const int32_t *lengths, const int32_t *counts, int32_t *tables, long long table_stride,
                           int table_width, const int32_t *free_blocks, int free_count, int requests, int tokens,
                           int block_size, int32_t *starts, int32_t *contexts, int32_t *slots, int32_t *positions,

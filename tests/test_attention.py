@@ -294,3 +294,28 @@ def test_workspace():
         a = plain(tokens=tokens, requests=requests, max_context=context, table_width=1 << 16, table_stride=1 << 16)
         assert lib.gptq_hip_attention_workspace_bytes(ctypes.byref(a)) <= (1 << 29) + (1 << 20)
     assert lib.gptq_hip_attend(None, None, 0, None) == _lib.ERR_BAD_ARG
+
+
+@pytest.mark.gpu
+def test_through_the_dispatcher():
+    """torch.ops.gptq_hip.* and the call in C are the same; tensor subclasses, modes and fake tensors reach the operator."""
+    s = Step(24, [(40, 1), (30, 20)], 4, 2, 64, 16)
+    want = attend(s)
+    args = (s.q, s.k_cache, s.v_cache, s.tables, s.starts, s.contexts, 40, 0, 0, 0.0)
+    assert torch.equal(torch.ops.gptq_hip.paged_attention(*args), want)
+
+    class Sub(torch.Tensor):
+        pass
+    s.q = s.q.as_subclass(Sub)
+    assert torch.equal(attend(s).as_subclass(torch.Tensor), want)
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode() as mode:
+        fake = [mode.from_tensor(t.as_subclass(torch.Tensor)) if isinstance(t, torch.Tensor) else t for t in args]
+        out = torch.ops.gptq_hip.paged_attention(*fake)
+        assert out.shape == want.shape and out.dtype == want.dtype
+    k, v = torch.randn(2, 3, 2, 64, device="cuda").half()
+    before = s.k_cache._version, s.v_cache._version
+    attention.cache_write(k, v, s.k_cache, s.v_cache, torch.arange(3, dtype=torch.int32, device="cuda"))
+    assert s.k_cache._version > before[0] and s.v_cache._version > before[1]
+    with pytest.raises(TypeError):
+        attention.paged_attention(s.q, None, s.v_cache, s.tables, s.starts, s.contexts)

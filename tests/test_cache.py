@@ -56,7 +56,7 @@ CASES = [  # B, longest, new tokens at most, block, tokens beyond the sum, free 
     (1, 0, 1, 16, 0, None, 2), (1, 37, 0, 16, 0, None, 2), (5, 40, 1, 16, 0, None, 2), (64, 4096, 1, 16, 0, None, 2),
     (7, 100, 33, 1, 0, None, 2), (300, 900, 70, 24, 0, None, 2), (3, 10, 5000, 64, 0, None, 2), (1000, 50, 3, 7, 0, None, 2),
     (6, 50, 40, 16, 9, None, 2), (6, 50, 40, 16, -5, None, 2), (6, 50, 40, 16, 0, 3, 2), (6, 50, 40, 16, 0, 0, 2),
-    (6, 50, 40, 16, 0, None, -2), (0, 1, 1, 16, 4, None, 2), (16384, 3, 1, 16, 0, None, 2),
+    (6, 50, 40, 16, 0, None, -2), (0, 1, 1, 16, 4, None, 2), (8192, 3, 1, 16, 0, None, 2),
 ]
 
 
@@ -143,9 +143,9 @@ def test_refusals_on_the_gpu():
                        ((ints, ints, tables, ints, 3, 0), "block_size"), ((ints, ints, tables.cpu(), ints, 3, 16), "no CPU fallback")):
         with pytest.raises(RuntimeError, match=text):
             attention.cache_tables(*args)
-    many = torch.zeros(16385, dtype=torch.int32, device="cuda")
-    with pytest.raises(RuntimeError, match="at most 16384"):
-        attention.cache_tables(many, many, torch.zeros(16385, 1, dtype=torch.int32, device="cuda"), ints, 0, 16)
+    many = torch.zeros(8193, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="at most 8192"):
+        attention.cache_tables(many, many, torch.zeros(8193, 1, dtype=torch.int32, device="cuda"), ints, 0, 16)
 
 
 def test_the_entry_points_refuse():
@@ -155,7 +155,7 @@ def test_the_entry_points_refuse():
     for more, status in ((dict(lengths=None), _lib.ERR_BAD_ARG), (dict(stride=3), _lib.ERR_BAD_ARG), (dict(width=-1), _lib.ERR_BAD_ARG),
                          (dict(free=None), _lib.ERR_BAD_ARG), (dict(B=-1), _lib.ERR_BAD_ARG), (dict(T=-1), _lib.ERR_BAD_ARG),
                          (dict(block=0), _lib.ERR_BAD_ARG), (dict(starts=None), _lib.ERR_BAD_ARG), (dict(slots=None), _lib.ERR_BAD_ARG),
-                         (dict(B=16385), _lib.ERR_UNSUPPORTED)):
+                         (dict(B=8193), _lib.ERR_UNSUPPORTED)):
         assert tables(**more) == status, more
     cache = _lib.Cache(k=p, v=p, type=0, blocks=4, block_size=16, heads=2, dim=64, block_stride=2048, slot_stride=128, head_stride=64)
     write = lambda c=cache, k=p, strides=(128, 64, 128, 64), slots=p, T=3: \

@@ -1,0 +1,98 @@
+"""``PagedCache``: the host's bookkeeping, and a small decoder served from it."""
+import os
+import sys
+
+import pytest
+import torch
+
+from autogptq.tvm_amd import PagedCache
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.gpu
+def test_a_decoder_is_served_from_it():
+    sys.path.insert(0, os.path.join(ROOT, "examples"))
+    try:
+        import serve_paged
+    finally:
+        sys.path.pop(0)
+    # (half-precision rounding through two layers of products and normalisations; the example asserts 2e-2 at every step)
+    assert serve_paged.main(verbose=False) < 2e-2
+
+
+def cache(**more):
+    return PagedCache(**{**dict(layers=1, blocks=12, block_size=4, kv_heads=1, dim=8, max_requests=3, max_context=24), **more})
+
+
+@pytest.mark.gpu
+def test_blocks_are_dealt_out_and_come_back():
+    c = cache()
+    s = c.step([0, 2], [5, 3])
+    assert c.free_blocks == 9 and (c.length(0), c.length(1), c.length(2)) == (5, 0, 3)
+    assert s.positions.tolist() == [0, 1, 2, 3, 4, 0, 1, 2] and s.contexts.tolist() == [5, 3] and s.max_context == 5
+    s = c.step([2, 0, 1], [2, 0, 1])        # another order, and a request that gets nothing
+    assert c.free_blocks == 7 and s.contexts.tolist() == [5, 5, 1] and s.starts.tolist() == [0, 2, 2, 3]
+    used = [e for e in c.tables.flatten().tolist() if e >= 0]
+    assert len(used) == len(set(used)) == 5
+    assert s.slots.tolist()[:2] == [int(c.tables[2, 0]) * 4 + 3, int(c.tables[2, 1]) * 4]
+    c.free(0)
+    c.free(1)
+    assert c.free_blocks == 10 and c.length(0) == 0
+    c.step([0], [24])
+    with pytest.raises(RuntimeError, match="does not fit"):
+        c.step([0], [1])
+    c.step([1], [12])
+    before = c.tables.clone()
+    with pytest.raises(RuntimeError, match="2 blocks are needed and 1 are free"):
+        c.step([2], [9])
+    assert torch.equal(c.tables, before) and c.length(2) == 5
+    c.free(0), c.free(1), c.free(2)
+    assert sorted(c._free.tolist()) == list(range(12))
+
+
+@pytest.mark.gpu
+def test_trim_gives_back_what_the_window_has_left():
+    c = cache()
+    c.step([1], [20])
+    assert c.trim(1, window=6, sinks=1) == 2            # tokens up to 14 are unseen from token 20 on: blocks 1 and 2
+    assert c.tables[1].tolist()[1:3] == [-1, -1] and c.free_blocks == 9
+    assert c.trim(1, window=6, sinks=1) == 0
+    c.step([1], [4])
+    assert c.trim(1, window=6, sinks=1) == 1 and c.free_blocks == 9
+    c.free(1)
+    assert sorted(c._free.tolist()) == list(range(12))
+
+
+@pytest.mark.gpu
+def test_shared_prefixes():
+    c = cache()
+    c.step([0], [6])
+    c.share(0, 1)
+    s = c.step([1], [3])
+    assert s.prefix[1] == 6 and s.prefix[0].tolist() == c.tables[0, :2].tolist() and s.positions.tolist() == [6, 7, 8]
+    with pytest.raises(ValueError, match="one prefix"):
+        c.step([1, 2], [1, 1])
+    with pytest.raises(ValueError, match="has tokens"):
+        c.share(0, 1)
+    with pytest.raises(ValueError, match="behind a prefix itself"):
+        c.share(1, 2)
+    c.share(0, 2)
+    assert c.step([1, 2], [1, 2]).prefix[1] == 6
+    q = torch.zeros(3, 1, 8, dtype=torch.float16, device="cuda")
+    with pytest.raises(NotImplementedError):
+        c.attend(0, q, c.step([1, 2], [1, 2]), window=4)
+
+
+def test_refusals():
+    c = cache(device="cpu")
+    with pytest.raises(ValueError, match="distinct"):
+        c.step([1, 1], [1, 1])
+    with pytest.raises(ValueError, match="at least 0"):
+        c.step([1], [-1])
+    with pytest.raises(RuntimeError, match="does not fit"):
+        c.step([1], [25])
+    with pytest.raises(ValueError, match="window"):
+        c.trim(0, 0)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        c.step([1], [3])

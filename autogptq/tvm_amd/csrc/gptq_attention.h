@@ -271,12 +271,48 @@ __device__ __forceinline__ void add_prefix(const AttentionParams &p, Sum &x, lon
 }
 
 // Joins the `parts` parts of a tile, in their order, behind those of a shared prefix.  place(part, row of the tile) is a row of
-// own_stats and own_parts.  Where a tile has few rows several threads share a value's parts.  `lds`: THREADS Sums.
-template <typename E, int THREADS, typename Place>
+// own_stats and own_parts.  Where a tile has few rows several threads share a value's parts; where it has many a thread takes
+// two values' at a time, four parts each.  `lds`: THREADS Sums; ITEMS: the most quads of values that a tile of the kernel has.
+template <typename E, int THREADS, int ITEMS, typename Place>
 __device__ void join_parts(const AttentionParams &p, const QueryTile &q, int h, int parts, void *lds, Place place)
 {
-    Sum *half_way = (Sum *)lds;
     const int quads = p.dim / 4, items = q.rows * quads;
+    if (ITEMS > 2 * THREADS && items >= 2 * THREADS) {
+        for (int i = threadIdx.x; i < items; i += 2 * THREADS) {
+            Sum x[2];
+            int r[2], d[2];
+            long long at[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int item = min(i + u * THREADS, items - 1);       // (the last one twice, if there is no other)
+                r[u] = item / quads, d[u] = (item - r[u] * quads) * 4, at[u] = out_row(p, q, h, r[u]);
+                x[u] = {kNone, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+                add_prefix(p, x[u], at[u], d[u]);
+            }
+            for (int s0 = 0; s0 < parts; s0 += 4) {
+                f2 ml[2][4];
+                f4 o[2][4];
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        if (s0 + s >= parts) continue;
+                        const long long from = place(s0 + s, r[u]);
+                        ml[u][s] = load_stats(p.own_stats + 2 * from);
+                        o[u][s] = load_partial(p.own_parts + from * p.dim + d[u]);
+                    }
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+                        if (s0 + s < parts) x[u].add(ml[u][s][0], ml[u][s][1], o[u][s]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++) store_row4<E>(p.out, at[u] * p.dim + d[u], x[u].result());
+        }
+        return;
+    }
+    Sum *half_way = (Sum *)lds;
     int teams = 1;
     while (8 * teams < parts && 2 * teams * items <= THREADS) teams *= 2;
     const int team = teams > 1 ? threadIdx.x / items : 0;

@@ -371,7 +371,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
             }
         }
         if (parts > 1 && arrive_last(p.counters + first * p.kv_heads + h, parts, &flag))
-            join_parts<E, 64 * NW>(p, q, h, parts, join, [&](int part, int r) {
+            join_parts<E, 64 * NW, 16 * RT * DP / 4>(p, q, h, parts, join, [&](int part, int r) {
                 return (long long)((2 * (first + part) + (part == 0)) * p.kv_heads + h) * R + r;
             });
         if (at >= stop) break;

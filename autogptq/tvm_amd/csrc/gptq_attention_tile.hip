@@ -171,7 +171,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
             const int key = 8 * up + 4 * hh + (col & 15) / 4, c = 4 * dt + 2 * (col >> 4) + (col & 3) / 2;
             vat[up][dt] = lds + 2 * TILE + key * (DP * 2) + ((c ^ ((2 * key) & (CH - 1))) * 16) + (col & 1) * 8;
         }
-    static_assert(CH <= 32 && (CH <= 16 || KT == 32), "the swizzle repeats within the rows that an immediate steps over");
+    static_assert(CH <= 32, "the swizzle repeats every 32 rows, of keys, and every 16, of values");
 
     f16 s[KA];
     // S^T for the keys in the buffer BUF
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
     }
     if (whole || p.shared) return;
     if (last_part(p, tile * p.kv_heads + h, parts, flag))
-        join_parts<E, 256>(p, q, h, parts, (float *)smem, [&](int part, int r) { return part * all + out_row(p, q, h, r); });
+        join_parts<E, 256, kTileRows * DP / 4>(p, q, h, parts, (float *)smem, [&](int part, int r) { return part * all + out_row(p, q, h, r); });
 }
 
 template <typename E>
@@ -320,8 +320,8 @@ static void launch_tile(const AttentionParams &p, hipStream_t stream)
     else if (p.dim <= 80) GPTQ_TILE(128, 80, 64);
     else if (p.dim <= 96) GPTQ_TILE(128, 96, 64);
     else if (p.dim <= 128) GPTQ_TILE(128, 128, 64);
-    else if (p.dim <= 192) GPTQ_TILE(256, 192, 32);
-    else GPTQ_TILE(256, 256, 32);
+    else if (p.dim <= 192) GPTQ_TILE(256, 192, 64);
+    else GPTQ_TILE(256, 256, 32);   // 64 would not stay in the registers
 #undef GPTQ_TILE
 }
 

@@ -9,8 +9,8 @@
 // is read: block table entries there may hold anything.  A short shared prefix may stand in front of the list, looked up in
 // a table of its own.
 //
-// Parts.  The keys of a tile may be divided among workgroups.  Each leaves m, l and o of its part in the workspace, and the
-// one that comes last joins them.
+// Parts.  The keys of a tile may be divided among workgroups.  Each leaves m, l and o of its part in the workspace.  Parts of few
+// rows are joined by the workgroup that comes last, those of up to 128 by a launch of their own.
 //
 // Statistics.  Scores are kept in units of log2(e): p = 2^(c q.k - m) with c = scale * log2(e), m the running maximum, l
 // the sum of p and o the sum of p v, all in 32 bits.  p is rounded to the cache's type for the matrix instruction (the
@@ -184,8 +184,7 @@ __device__ __forceinline__ f2 load_stats(const float *src)
     return __builtin_bit_cast(f2, __hip_atomic_load((const unsigned long long *)src, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
-// Four values of a part, and its statistics.  Parts of a shared prefix are read by the next launch and need no way past the
-// caches.
+// Four values of a part, and its statistics.  Parts that a later launch reads need no way past the caches.
 template <bool COHERENT>
 __device__ __forceinline__ void put_part(float *to, f4 x)
 {
@@ -221,15 +220,6 @@ __device__ __forceinline__ void store_row4(void *out, long long at, f4 o)
     *(typename Vec<E>::e4 *)((E *)out + at) = __builtin_convertvector(o, typename Vec<E>::e4);
 }
 
-// Whether this workgroup joins the parts of its tile: the one that is last, or the only one (then behind a shared prefix).
-__device__ __forceinline__ bool last_part(const AttentionParams &p, int counter, int parts, int *flag)
-{
-    if (parts > 1) return arrive_last(p.counters + counter, parts, flag);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what this thread stored is there for the others
-    __syncthreads();
-    return true;
-}
-
 // Four values of a row with the row's statistics, and parts that join them: m = max m_i, l = sum l_i 2^(m_i - m), o likewise.
 struct Sum {
     float m, l;
@@ -262,7 +252,7 @@ __device__ __forceinline__ void add_parts(Sum &x, int first, int step, int count
             if (s0 + u * step < count) x.add(ml[u][0], ml[u][1], o[u]);
     }
 }
-// The parts of a shared prefix, which the launch before left.
+// The parts of a shared prefix, which a launch before left.
 __device__ __forceinline__ void add_prefix(const AttentionParams &p, Sum &x, long long at, int d)
 {
     const long long all = (long long)p.tokens * p.heads;

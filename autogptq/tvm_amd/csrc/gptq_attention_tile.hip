@@ -1,7 +1,7 @@
 // Attention over a paged cache for many rows a request: prompts, pieces of prompts, a batch behind a shared prefix.
 //
 // What bounds it: the matrix instructions and the exponentials beside them.  A workgroup of four waves takes 128 rows, 32 a
-// wave, and walks the tile's keys KT at a time; keys and values go through LDS, so that a row from the cache is read once
+// wave, and walks the tile's keys 64 at a time; keys and values go through LDS, so that a row from the cache is read once
 // for 128 rows.
 //
 //   S^T = K Q^T    32 x 32 results: a lane holds 16 keys of one row for each 32 keys, the maximum and the sum of a row are
@@ -14,6 +14,10 @@
 //             values, one barrier a tile: while tile n is summed, the keys of n + 2 and the values of n + 1 arrive.  The
 //             rows' places come from a ring of lists in LDS, filled every four tiles by all waves at once, a tile each (one
 //             wave doing it for every tile held the others up at every barrier).
+//   parts     where a batch has fewer tiles than the card holds workgroups, each tile's keys are divided; a second launch joins
+//             the parts, 16 rows a workgroup.  (The last workgroup of a tile doing it, one for up to 128 rows: 16 pieces of
+//             20 tokens behind 2048 keys, dim 128, 73.6 us against 54.5; 5 of up to 333 behind up to 9001, dim 80, 77.7
+//             against 66.6.)
 //   LDS       rows as they lie in the cache; the 16-byte chunks of row r stand at chunk ^ r (keys) and chunk ^ 2 r (values),
 //             which spreads the lanes of a read over all banks.  The swizzle is in the requests' source addresses.
 #include <type_traits>
@@ -21,6 +25,9 @@
 #include "gptq_attention.h"
 
 namespace gptq {
+
+constexpr int kTileKeys = 64;   // keys of a step
+constexpr int kJoinRows = 16;
 
 // The tile of a workgroup.  Request b owns the tiles from first_tile(b) = floor(starts[b] * group / R) + b: the floors of two
 // neighbours lie at least floor(rows / R) apart, and the + b adds the tile of a remainder.  So the bound
@@ -82,10 +89,11 @@ __device__ __forceinline__ u2 read_turned(uint32_t at)
 __device__ __forceinline__ u4 read16(uint32_t at) { return *(const __attribute__((address_space(3))) u4 *)(uintptr_t)at; }
 
 // DP: row of LDS (a power of two), DC: dims that are computed, the multiple of 16 that covers p.dim
-template <typename E, int DP, int DC, int KT>
+template <typename E, int DP, int DC>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(const AttentionParams p)
 {
     typedef typename Vec<E>::e8 e8;
+    constexpr int KT = kTileKeys;
     constexpr int CH = DP / 8;              // 16-byte chunks of a row
     constexpr int RP = 256 / CH;            // rows that the workgroup requests at a time
     constexpr int PASSES = KT / RP;
@@ -93,7 +101,6 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
     constexpr int KA = KT / 32, SX = DC / 16, DT = (DC + 31) / 32, PX = KT / 16;
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
     uint32_t *list = (uint32_t *)(smem + 4 * TILE);     // [8][KT]
-    int *flag = (int *)(list + 8 * KT);
 
     const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -133,10 +140,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
     const int tiles = (end - begin + KT - 1) / KT;
     // Rows of tile n for the requests: four tiles at a time, one a wave.  A thread's rows of a tile stand side by side.
     auto look_up = [&](int n) {
-        return key_row(p, q, table, min(begin + min(n, tiles - 1) * KT + min(lane, KT - 1), end - 1));
+        return key_row(p, q, table, min(begin + min(n, tiles - 1) * KT + lane, end - 1));
     };
     auto enter = [&](int n, uint32_t row) {
-        if (lane < KT) list[(n & 7) * KT + lane % RP * PASSES + lane / RP] = row;
+        list[(n & 7) * KT + lane % RP * PASSES + lane / RP] = row;
     };
     typedef uint32_t Rows __attribute__((ext_vector_type(PASSES)));
     // this thread's chunk of the rows it requests
@@ -179,7 +186,6 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
         constexpr int BUF = decltype(buf)::value * TILE;
 #pragma unroll
         for (int a = 0; a < KA; a++) s[a] = (f16)(0.0f);
-        // (32 keys at a time: two sums in turn, or one after the other where that is all there are)
 #pragma unroll
         for (int x0 = 0; x0 < SX; x0 += 4) {
             u4 kf[4][KA];
@@ -203,7 +209,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
 #pragma unroll
                 for (int up = 0; up < 2; up++) vf[x][dt][up] = read_turned<E>(vat[up][dt] + (BUF + 16 * x * DP * 2));
         };
-        read_values(0);
+        // (a step of 16 keys ahead, but for the widest rows, which leave no registers for it)
+        constexpr bool EARLY = DT <= 6;
+        if (EARLY) read_values(0);
         __builtin_amdgcn_sched_barrier(0);
         const int v0 = begin + n * KT, v1 = min(v0 + KT, end);
         if (v0 + KT > end || !all_see(p, q, v0, v1, pos_first, pos_last)) {
@@ -230,7 +238,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
         const float ref = reference(m);
 #pragma unroll
         for (int x = 0; x < PX; x++) {
-            if (x + 1 < PX) read_values(x + 1);
+            if (!EARLY) read_values(x);
+            else if (x + 1 < PX) read_values(x + 1);
             f8 pr;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -292,7 +301,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
         const long long at = out_row(p, q, h, r);
         const long long slot = split * all;
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        if (!whole && hh == 0) p.shared ? put_stats<false>(stats + 2 * (slot + at), m, l) : put_stats<true>(stats + 2 * (slot + at), m, l);
+        if (!whole && hh == 0) put_stats<false>(stats + 2 * (slot + at), m, l);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -301,28 +310,49 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
                 if (d >= p.dim) continue;
                 const f4 y = {o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
                 if (whole) store_row4<E>(p.out, at * p.dim + d, y * inv);
-                else if (p.shared) put_part<false>(outs + (slot + at) * p.dim + d, y);
-                else put_part<true>(outs + (slot + at) * p.dim + d, y);
+                else put_part<false>(outs + (slot + at) * p.dim + d, y);
             }
     }
-    if (whole || p.shared) return;
-    if (last_part(p, tile * p.kv_heads + h, parts, flag))
-        join_parts<E, 256, kTileRows * DP / 4>(p, q, h, parts, (float *)smem, [&](int part, int r) { return part * all + out_row(p, q, h, r); });
+}
+
+// Joins the parts of tiles that are divided, or stand behind a shared prefix: kJoinRows rows of a tile a workgroup.
+template <typename E>
+__global__ __launch_bounds__(256) void attention_join_kernel(const AttentionParams p)
+{
+    const int h = blockIdx.x % p.kv_heads, tile = blockIdx.x / p.kv_heads, r0 = blockIdx.y * kJoinRows;
+    QueryTile q;
+    if (!find_tile<kTileRows>(p, tile, q) || r0 >= q.rows) return;
+    int chunk;
+    const int parts = tile_parts(p, q.seen, kTileKeys, chunk);
+    if (parts == 1 && p.prefix_parts == 0) return;
+    const long long all = (long long)p.tokens * p.heads;
+    const int quads = p.dim / 4;
+    for (int i = threadIdx.x; i < min(kJoinRows, q.rows - r0) * quads; i += 256) {
+        const int r = i / quads, d = (i - r * quads) * 4;
+        const long long at = out_row(p, q, h, r0 + r);
+        Sum x = {kNone, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+        add_prefix(p, x, at, d);
+        add_parts<false>(x, 0, 1, parts, [&](int s) { return p.own_stats + 2 * (s * all + at); },
+                         [&](int s) { return p.own_parts + (s * all + at) * p.dim + d; });
+        store_row4<E>(p.out, at * p.dim + d, x.result());
+    }
 }
 
 template <typename E>
 static void launch_tile(const AttentionParams &p, hipStream_t stream)
 {
     const dim3 grid((unsigned)(p.kv_heads * p.tiles), (unsigned)p.splits);
-#define GPTQ_TILE(DP, DC, KT) \
-    hipLaunchKernelGGL((attention_tile_kernel<E, DP, DC, KT>), grid, dim3(256), 4 * KT * DP * 2 + 8 * KT * 4 + 16, stream, p)
-    if (p.dim <= 64) GPTQ_TILE(64, 64, 64);
-    else if (p.dim <= 80) GPTQ_TILE(128, 80, 64);
-    else if (p.dim <= 96) GPTQ_TILE(128, 96, 64);
-    else if (p.dim <= 128) GPTQ_TILE(128, 128, 64);
-    else if (p.dim <= 192) GPTQ_TILE(256, 192, 64);
-    else GPTQ_TILE(256, 256, 32);   // 64 would not stay in the registers
+#define GPTQ_TILE(DP, DC) \
+    hipLaunchKernelGGL((attention_tile_kernel<E, DP, DC>), grid, dim3(256), 4 * kTileKeys * DP * 2 + 8 * kTileKeys * 4, stream, p)
+    if (p.dim <= 64) GPTQ_TILE(64, 64);
+    else if (p.dim <= 80) GPTQ_TILE(128, 80);
+    else if (p.dim <= 96) GPTQ_TILE(128, 96);
+    else if (p.dim <= 128) GPTQ_TILE(128, 128);
+    else if (p.dim <= 192) GPTQ_TILE(256, 192);
+    else GPTQ_TILE(256, 256);
 #undef GPTQ_TILE
+    if (!p.shared && (p.splits > 1 || p.prefix_parts > 0))
+        hipLaunchKernelGGL(attention_join_kernel<E>, dim3(grid.x, kTileRows / kJoinRows), dim3(256), 0, stream, p);
 }
 
 int launch_attention_tile(const AttentionParams &p, int type, void *stream)

@@ -43,11 +43,11 @@ __device__ __forceinline__ bool find_tile(const AttentionParams &p, int tile, Qu
     } else {
         // what the tensors say is cut to what the other arguments allow: wrong lengths give wrong sums, not wrong addresses
         int before = 0;
+#pragma unroll 4
         for (int b0 = 0; b0 < p.requests; b0 += 64) {
             const int b = b0 + lane;
-            const bool there = b < p.requests;
-            const int s = there ? min(max(p.starts[b], 0), p.tokens) : 0;
-            before += __popcll(__ballot(there && (int)((uint32_t)s * (uint32_t)p.group / R) + b <= tile));
+            const int s = min(max(p.starts[min(b, p.requests)], 0), p.tokens);
+            before += __popcll(__ballot(b < p.requests && (int)((uint32_t)s * (uint32_t)p.group / R) + b <= tile));
         }
         q.b = __builtin_amdgcn_readfirstlane(max(before, 1) - 1);
         q.start = min(max(p.starts[q.b], 0), p.tokens);

@@ -20,6 +20,11 @@
 //             against 66.6.)
 //   LDS       rows as they lie in the cache; the 16-byte chunks of row r stand at chunk ^ r (keys) and chunk ^ 2 r (values),
 //             which spreads the lanes of a read over all banks.  The swizzle is in the requests' source addresses.
+//
+// Measured (32 heads in groups of 4, dim 128): a prompt of 8192 tokens 587 us, 937 TFLOP/s; the matrix pipes are busy in half
+// of the cycles, at the 1.7 to 1.9 GHz that the card's power leaves.  Without the exponentials it takes 6 % less, without the
+// requests 18 %, without the reads of values 3 %.  Not better: 64 rows a wave (spills, 1537 us), eight waves a workgroup
+// (the same), a wave's priority raised around its products (fewer cycles, the same time).
 #include <type_traits>
 
 #include "gptq_attention.h"

@@ -139,7 +139,8 @@ __global__ __launch_bounds__(kTableThreads) void cache_tables_kernel(const Cache
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Write.  Bound by memory: every row is read and written once, 16 bytes a thread.  Tokens of a step that are no longer wanted
-// (slot -1) and slots outside of the cache are skipped.
+// (slot -1) and slots outside of the cache are skipped.  (8192 tokens of 8 heads of 128: 67 MB in 11.2 us, 6.0 TB/s; 64 tokens
+// 2.6 us, of which a launch is 2.4.)
 // ---------------------------------------------------------------------------------------------------------------------
 struct CacheWrite {
     const char *k, *v;

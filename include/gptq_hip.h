@@ -403,14 +403,18 @@ int gptq_hip_cache_write(const gptq_hip_cache *cache, const void *k, const void 
  * q [tokens, heads, dim] in the cache's type (16-byte aligned, strides in elements, multiples of 8), out [tokens, heads,
  * dim] contiguous, 16-byte aligned.  scale > 0.  Scores, softmax and sums are fp32; shares of the softmax are rounded to the cache's
  * type for the product with v, the result once.  Table entries of blocks that no token of a request sees are
- * not read (blocks that a window has left behind may be given back), nor are slots past a context.
+ * not read (blocks that a window has left behind may be given back), nor are slots past a context.  Keys and values of
+ * neighbouring tokens of a request are read together: one that a token does not see has the share 0 in it, so values
+ * must be finite up to the request's last token (0 times an infinity or a NaN is a NaN); keys may be anything.
  *   prefix_length > 0: every token sees prefix_length more keys before its own context, those of the blocks
- *     prefix_blocks int32 [ceil(prefix_length / block_size)], shared by all requests and read once for all of them;
+ *     prefix_blocks int32 [ceil(prefix_length / block_size)], shared by all requests and read once for all of them (again for
+ *     each where it is so short that this costs less than a launch);
  *     contexts count a request's own tokens only.  window must be 0.
  *   max_context: the longest context, as the host knows it: it sets how the work is divided, not what is computed (0: the
  *     tables' width)
  * workspace: gptq_hip_attention_workspace_bytes, zeroed once; every call leaves its counters at zero, so calls on one
- * stream may share it, but no other entry point may write to it.  One launch, two with a prefix.
+ * stream may share it, but no other entry point may write to it.  One to three launches: a longer prefix has one of its own, and so
+ * has the join of a few tiles of many tokens whose keys were divided.
  */
 typedef struct gptq_hip_attention {
     gptq_hip_cache cache;

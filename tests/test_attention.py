@@ -53,6 +53,13 @@ CASES = {
     "prompt, dim 136": ([(300, 150), (77, 77)], 4, 2, 136, 16, BF16, "head", 64, 1),
     "prompts of many heads": ([(70, 70), (9, 9)], 40, 8, 128, 64, HALF, "token", 0, 0),
     "a piece behind a long context": ([(5000, 40)], 4, 1, 128, 16, HALF, "token", 0, 0),
+    "prompt, dim 96": ([(300, 150), (77, 77)], 4, 2, 96, 16, HALF, "token", 0, 0),
+    "pieces behind long contexts, dim 64": ([(2500, 40), (700, 33)], 4, 1, 64, 16, BF16, "head", 0, 0),
+    "pieces behind long contexts, dim 80": ([(2500, 40), (30, 30), (1700, 21)], 7, 1, 80, 24, HALF, "token", 0, 0),
+    "pieces behind long contexts, dim 192": ([(2500, 40), (700, 33)], 4, 1, 192, 16, HALF, "token", 0, 0),
+    "pieces behind long contexts, dim 256": ([(2500, 40), (700, 33)], 4, 1, 256, 16, BF16, "token", 0, 0),
+    "a piece under a long window with sinks": ([(4000, 90)], 4, 1, 128, 16, HALF, "token", 1500, 3),
+    "pieces of more requests than a wave": ([(300 + 11 * i, 17 * (i % 3)) for i in range(70)], 4, 1, 64, 16, HALF, "token", 0, 0),
     "one prompt among single tokens": ([(700, 1), (400, 400), (90, 1), (1200, 1)], 4, 1, 128, 16, HALF, "token", 0, 0),
     "long": ([(9000, 1)], 8, 2, 128, 16, HALF, "token", 0, 0),
     "long and short": ([(6000, 1), (3, 1), (900, 1), (1, 1)], 4, 2, 64, 16, BF16, "token", 0, 0),
@@ -78,6 +85,7 @@ PREFIXES = {
     "batch of a few hundred rows": ([(1 + 13 * i % 90, 1) for i in range(70)], 8, 1, 128, 16, BF16, 2100),
     "drafts and requests without tokens": ([(30, 3), (8, 0), (200, 5), (2, 2)], 8, 4, 128, 24, HALF, 777),
     "prompts": ([(150, 150), (64, 30)], 4, 1, 128, 16, HALF, 500),
+    "prompts and long own contexts": ([(3000, 60), (64, 30)], 4, 1, 128, 16, HALF, 500),
     "dim 80": ([(20, 1), (90, 2)], 4, 1, 80, 16, BF16, 333),
     "dim 256": ([(20, 1), (90, 2), (400, 40)], 8, 2, 256, 16, HALF, 333),
     "dim 64, sevens": ([(20, 1)] * 9, 7, 1, 64, 7, HALF, 900),
@@ -122,6 +130,21 @@ def test_values_that_are_large_where_masked():
     got = attend(s)
     # scores reach 64 here: the 32-bit part of the bound grows with them
     assert bool(((got.double() - want).abs() <= 3 * 2.0 ** -11 * size + 2.0 ** -24).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_keys_that_are_not_finite_where_masked(value):
+    # the keys of each request's last token, which the tokens before it do not see
+    for requests, dim in (([(130, 130), (2000, 50)], 128), ([(70, 4), (5, 2)], 64), ([(200, 60)], 256)):
+        s = Step(16, requests, 4, 2, dim, 16)
+        want, size = s.expected()
+        others = torch.ones(s.tokens, dtype=torch.bool, device=s.q.device)
+        for b, (context, _) in enumerate(requests):
+            s.k_cache[int(s.tables[b, (context - 1) // 16]), (context - 1) % 16] = value
+            others[int(s.starts[b + 1]) - 1] = False
+        err = (attend(s).double() - want).abs()
+        assert bool((err <= 2.25 * 2.0 ** -11 * size + 2.0 ** -24)[others].all())
 
 
 @pytest.mark.gpu
@@ -190,9 +213,9 @@ def test_on_another_stream():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("prefix", [0, 600])
-def test_captured_in_a_graph(prefix):
-    s = Step(21, [(3000, 1), (50, 1), (1, 1)], 4, 2, 128, 16, prefix=prefix)
+@pytest.mark.parametrize("prefix, tokens", [(0, 1), (600, 1), (0, 50), (600, 50)])
+def test_captured_in_a_graph(prefix, tokens):
+    s = Step(21, [(3000, tokens), (50, tokens), (tokens, tokens)], 4, 2, 128, 16, prefix=prefix)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):

@@ -55,7 +55,7 @@ void divide(Division &d, long long want, long long busy, long long keys, long lo
     d.chunk = (int)(ceil_div(ceil_div(std::max(keys, 1ll), s), unit) * unit);
     d.splits = (int)std::max(1ll, ceil_div(keys, d.chunk));
 }
-// Own contexts on the tile kernel: two workgroups a CU, since they differ in length (32 heads in groups of 4; us with 256, 512 and
+// Own contexts on the tile kernel: two workgroups a CU (also where it holds three: 768 for dim 64 bring nothing), since they differ in length (32 heads in groups of 4; us with 256, 512 and
 // 1024 workgroups: 16 pieces of 20 tokens behind 2048 keys, dim 128: 51, 54, 62, dim 256: 136, 124, 140; 8 of 256 behind 4096: dim
 // 128: 182, 181, 216, dim 256: 462, 464, 542; 723 tokens of 7 heads behind up to 9001, dim 80: 107, 87, 90).  A shared prefix: parts of one length, which the
 // next launch reads again, so one a CU (512 rows behind 16384 keys: 256 workgroups 80 us, 512 84, 1024 111); rows that fit the

@@ -25,6 +25,7 @@
 // of the cycles, at the 1.7 to 1.9 GHz that the card's power leaves.  Without the exponentials it takes 6 % less, without the
 // requests 18 %, without the reads of values 3 %.  Not better: 64 rows a wave (spills, 1537 us), eight waves a workgroup
 // (the same), a wave's priority raised around its products (fewer cycles, the same time).
+#include <algorithm>
 #include <type_traits>
 
 #include "gptq_attention.h"
@@ -95,7 +96,7 @@ __device__ __forceinline__ u4 read16(uint32_t at) { return *(const __attribute__
 
 // DP: row of LDS (a power of two), DC: dims that are computed, the multiple of 16 that covers p.dim
 template <typename E, int DP, int DC>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(const AttentionParams p)
+__global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attention_tile_kernel(const AttentionParams p)
 {
     typedef typename Vec<E>::e8 e8;
     constexpr int KT = kTileKeys;
@@ -214,8 +215,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attention_tile_kernel(
 #pragma unroll
                 for (int up = 0; up < 2; up++) vf[x][dt][up] = read_turned<E>(vat[up][dt] + (BUF + 16 * x * DP * 2));
         };
-        // (a step of 16 keys ahead, but for the widest rows, which leave no registers for it)
-        constexpr bool EARLY = DT <= 6;
+        // (a step of 16 keys ahead, but for the widest rows, which leave no registers for it, and those of 64, where the registers
+        // let a third workgroup into a CU: a prompt of 4096 tokens 122 us, 106 so)
+        constexpr bool EARLY = DT > 2 && DT <= 6;
         if (EARLY) read_values(0);
         __builtin_amdgcn_sched_barrier(0);
         const int v0 = begin + n * KT, v1 = min(v0 + KT, end);
@@ -347,8 +349,11 @@ template <typename E>
 static void launch_tile(const AttentionParams &p, hipStream_t stream)
 {
     const dim3 grid((unsigned)(p.kv_heads * p.tiles), (unsigned)p.splits);
+    // A CU holds three workgroups of rows of 64.  A grid of about two a CU (and the tiles that requests leave empty) would stand three
+    // on some and one on others; LDS for two keeps it even (8 pieces of 256 tokens behind 4096 keys, 576 workgroups: 119 us, 101 so).
+    const int least = (long long)p.kv_heads * p.tiles * p.splits <= 640 ? 56 * 1024 : 0;
 #define GPTQ_TILE(DP, DC) \
-    hipLaunchKernelGGL((attention_tile_kernel<E, DP, DC>), grid, dim3(256), 4 * kTileKeys * DP * 2 + 8 * kTileKeys * 4, stream, p)
+    hipLaunchKernelGGL((attention_tile_kernel<E, DP, DC>), grid, dim3(256), std::max(4 * kTileKeys * DP * 2 + 8 * kTileKeys * 4, least), stream, p)
     if (p.dim <= 64) GPTQ_TILE(64, 64);
     else if (p.dim <= 80) GPTQ_TILE(128, 80);
     else if (p.dim <= 96) GPTQ_TILE(128, 96);

@@ -9,8 +9,9 @@ layers are replaced); here a serving step finds what stands between q/k/v and o 
                                as they come, with or without a sliding window and first tokens that stay visible (sinks)
 * ``shared_prefix_attention``  the same for requests behind one long prefix, which is read once for all of them
 
-All run on the current stream of the tensors' device, are safe to capture in a graph once they ran before (the workspace
-exists then), have no backward, and exist as ``torch.ops.gptq_hip.*`` too.  Caches are float16 or bfloat16
+All run on the current stream of the tensors' device, have no backward, and exist as ``torch.ops.gptq_hip.*`` too.  They can be
+captured by ``torch.cuda.graph``: a capture gets a workspace of its own from the graph's memory, whatever runs before or after it
+(the graph clears its counters, one small launch a replay); what the kernels need loaded, a call on any stream before it loads.  Caches are float16 or bfloat16
 [blocks, block_size, kv_heads, dim] in any order of memory whose last dimension is contiguous; dim is a multiple of 8 up to 256.
 """
 from __future__ import annotations

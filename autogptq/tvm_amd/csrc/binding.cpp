@@ -13,9 +13,11 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/custom_class.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <atomic>
 #include <map>
 #include <mutex>
@@ -36,8 +38,19 @@ void raise(int rc, const char *what, int64_t M, int64_t K, int64_t N, int64_t bi
                 ") failed: ", gptq_hip_strerror(rc), " [status ", rc, "]");
 }
 
+unsigned long long capture_of(void *stream)
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) {
+        (void)hipGetLastError();     // (the default stream, while another thread captures: that stream itself is in no capture)
+        return 0;
+    }
+    return status == hipStreamCaptureStatusActive ? id + 1 : 0;
+}
+
 // One workspace per (device, stream) and kind (a replaced one stays valid for the work already queued on its stream: the
-// allocator gives its memory to that stream only).
+// allocator gives its memory to that stream only), and one for the capture that the stream is in.
 // kind 1: the decode plans of the tiled family with halved tiles, whose kernel keeps their bytes zero between launches
 // (the slots of the halves): nothing else may write there, so they do not share the workspace the other plans pack x
 // or partial sums into.
@@ -67,12 +80,20 @@ WorkspaceLease::WorkspaceLease(const Tensor &like, size_t nbytes, void *stream, 
         const std::lock_guard<std::mutex> lock(g_ws_mutex);
         l = {device, stream, &g_ws[{device, stream, kind}]};
     }
-    ws = l.ws;
-    held = std::unique_lock<std::mutex>(ws->busy);
-    if (!ws->bytes.defined() || (size_t)ws->bytes.numel() < nbytes) {
-        const int64_t n = (int64_t)std::max(nbytes, (size_t)1 << 20);
-        ws->bytes = at::zeros({n}, like.options().dtype(at::kByte));
+    Workspace &ws = *l.ws;
+    held = std::unique_lock<std::mutex>(ws.busy);
+    const unsigned long long capture = capture_of(stream);
+    if (ws.capture != capture) ws.captured = Tensor(), ws.capture = capture;
+    Tensor &own = capture ? ws.captured : ws.bytes;
+    if (!own.defined() || (size_t)own.numel() < nbytes) {
+        const Tensor larger = at::empty({(int64_t)(std::max(nbytes, (size_t)1 << 20) + 3) / 4 * 4}, like.options().dtype(at::kByte));
+        // kind 1 wants all of it zero, the others their counters at its head (which a replay clears each time)
+        const size_t clear = kind == 1 || !capture ? (size_t)larger.numel() : (size_t)1 << 16;
+        const int rc = gptq_hip_workspace_init(larger.data_ptr(), clear, stream);
+        TORCH_CHECK(rc == GPTQ_HIP_OK, "clearing a workspace failed: ", gptq_hip_strerror(rc), " [status ", rc, "]");
+        own = larger;
     }
+    bytes = &own;
 }
 
 int Bound::choose()

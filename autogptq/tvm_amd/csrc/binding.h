@@ -26,21 +26,31 @@ void raise(int rc, const char *what, int64_t M, int64_t K, int64_t N, int64_t bi
 constexpr int kAttentionWorkspace = 2;
 int workspace_kind(const gptq_hip_plan &plan);
 
+// 0, or a number of the graph capture that the stream is in (no two captures have the same)
+unsigned long long capture_of(void *stream);
+
 // The workspace of a stream for the launches of one call (none for nbytes = 0).  Held over all of them: a call is up to three
 // launches that hand x or partial sums on through the workspace, and those of another thread on the same stream must not
 // come between.
+//
+// Launches that are captured keep the address for as long as their graph lives, and replay on any stream beside anything, so
+// they never get the workspace of eager calls, which is replaced when a call needs more: each capture has one of its own, out of
+// the memory pool of its graph, cleared by a launch that is captured with them.  (One launch a capture, not a call.  A capture that
+// needs more on the way gets another: the pool hands the first one's memory to what the graph does later on the same stream.)
 struct Workspace {
     std::mutex busy;
-    Tensor bytes;
+    Tensor bytes;                      // of eager calls
+    Tensor captured;                   // of the capture `capture`; let go with the first call outside of it
+    unsigned long long capture = 0;
 };
 class WorkspaceLease {
 public:
     WorkspaceLease(const Tensor &like, size_t nbytes, void *stream, int kind = 0);
-    void *data() const { return ws ? ws->bytes.data_ptr() : nullptr; }
-    size_t size() const { return ws ? (size_t)ws->bytes.numel() : 0; }
+    void *data() const { return bytes ? bytes->data_ptr() : nullptr; }
+    size_t size() const { return bytes ? (size_t)bytes->numel() : 0; }
 
 private:
-    Workspace *ws = nullptr;
+    const Tensor *bytes = nullptr;
     std::unique_lock<std::mutex> held;
 };
 

@@ -342,3 +342,106 @@ def test_through_the_dispatcher():
     assert s.k_cache._version > before[0] and s.v_cache._version > before[1]
     with pytest.raises(TypeError):
         attention.paged_attention(s.q, None, s.v_cache, s.tables, s.starts, s.contexts)
+
+
+def captured(stream, call):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = call()
+    return graph, got
+
+
+def overwrite(n=256 << 20):
+    """Fills what the allocator can hand out, on the current stream, with bytes that are no zeros."""
+    junk = [torch.full((1 << k,), 0x7f, dtype=torch.uint8, device="cuda") for k in range(9, 28)]
+    junk += [torch.full((n // 16,), 0x7f, dtype=torch.uint8, device="cuda") for _ in range(16)]
+    return junk
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads, kv_heads", [(4, 2), (32, 8)])
+def test_a_captured_call_does_not_depend_on_later_calls(heads, kv_heads):
+    """Eager calls that need more workspace than a captured one come after it on its stream; what they leave behind is
+    overwritten."""
+    small = Step(31, [(2000, 1), (700, 1)], heads, kv_heads, 128, 16)
+    large = Step(32, [(6000, 500)], heads, kv_heads, 128, 16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want, other = attend(small), attend(large)
+        del other
+        torch.cuda.empty_cache()
+    # a stream whose workspace has the small call's size
+    stream = torch.cuda.Stream()
+    stream.wait_stream(side)
+    with torch.cuda.stream(stream):
+        attend(small)
+        graph, got = captured(stream, lambda: attend(small))
+        for _ in range(3):
+            attend(large)
+            junk = overwrite()
+            got.zero_()
+            graph.replay()
+            stream.synchronize()
+            assert torch.equal(got, want)
+            assert all(bool((j == 0x7f).all()) for j in junk), "a replay wrote into another tensor"
+            del junk
+
+
+@pytest.mark.gpu
+def test_captures_replay_in_any_order():
+    """Two captures on one stream that was not warmed up: the second is replayed first, and each with the other's parts in
+    between."""
+    steps = [Step(33, [(2000, 1), (700, 1)], 8, 2, 128, 16), Step(34, [(3000, 1), (90, 1), (1500, 2)], 8, 2, 128, 16),
+             Step(35, [(3000, 60)], 8, 2, 128, 16, prefix=0)]
+    want = [attend(s) for s in steps]
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    junk = overwrite()      # (what new pools get is not zero by chance)
+    del junk
+    torch.cuda.empty_cache()
+    made = [captured(stream, lambda s=s: attend(s)) for s in steps]
+    for order in ((1, 0, 2), (2, 1, 0), (0, 0, 1), (1, 2, 2)):
+        for i in order:
+            made[i][1].zero_()
+            made[i][0].replay()
+        torch.cuda.synchronize()
+        for i in set(order):
+            assert torch.equal(made[i][1], want[i]), (order, i)
+
+
+@pytest.mark.gpu
+def test_two_captures_replay_on_two_streams_at_once():
+    steps = [Step(36, [(4000, 1), (700, 1)], 8, 2, 128, 16), Step(37, [(3000, 1), (90, 1), (2500, 1)], 8, 2, 128, 16)]
+    want = [attend(s) for s in steps]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for s in steps:
+            attend(s)
+    made = [captured(stream, lambda s=s: attend(s)) for s in steps]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in made]
+    for _ in range(20):
+        for (graph, got), s in zip(made, streams):
+            with torch.cuda.stream(s):
+                got.zero_()
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, got), w in zip(made, want):
+            assert torch.equal(got, w)
+
+
+@pytest.mark.gpu
+def test_a_capture_that_grows_its_workspace():
+    steps = [Step(38, [(2000, 1)], 4, 2, 128, 16), Step(39, [(6000, 500)], 32, 8, 128, 16), Step(40, [(2500, 1), (40, 1)], 32, 8, 128, 16)]
+    want = [attend(s) for s in steps]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph, got = captured(stream, lambda: [attend(s) for s in steps])
+    for _ in range(3):
+        for g in got:
+            g.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))

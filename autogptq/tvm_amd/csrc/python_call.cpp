@@ -276,6 +276,16 @@ PyObject *install(PyObject *, PyObject *cls)
     END_HANDLE_TH_ERRORS
 }
 
+// capture(stream): 0, or a number of the graph capture that the stream (its handle) is in
+PyObject *capture(PyObject *, PyObject *arg)
+{
+    HANDLE_TH_ERRORS
+    const unsigned long long stream = PyLong_AsUnsignedLongLong(arg);
+    if (stream == (unsigned long long)-1 && PyErr_Occurred()) return nullptr;
+    return PyLong_FromUnsignedLongLong(capture_of((void *)(uintptr_t)stream));
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- the serving operators
 // The same functions as torch.ops.gptq_hip.*, called with plain tensors and without the dispatcher, whose handling of ten
 // arguments costs as much as the shorter of these calls run (cache_tables for 64 requests 9.5 us a call through it, 5.5 so).
@@ -386,6 +396,7 @@ PyObject *call_shared_prefix_attention(PyObject *, PyObject *const *args, Py_ssi
 
 #define GPTQ_FAST(NAME) {#NAME, (PyCFunction)(void (*)(void))call_##NAME, METH_FASTCALL, "torch.ops.gptq_hip." #NAME " on plain tensors, else NotImplemented."}
 PyMethodDef functions[] = {GPTQ_FAST(cache_tables), GPTQ_FAST(cache_write), GPTQ_FAST(paged_attention), GPTQ_FAST(shared_prefix_attention),
+                           {"capture", capture, METH_O, "capture(stream): 0, or a number of the graph capture that the stream is in."},
                            {"aside", aside, METH_VARARGS, "aside(fn, *args): fn(*args), hidden from tracing and dispatch modes."},
                            {"install", install, METH_O, "Makes the call in C the one of a QuantLinear class."}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "gptq_hip_call", "the QuantLinear call in C", -1, functions};

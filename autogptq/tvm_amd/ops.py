@@ -70,7 +70,16 @@ def check_shapes(qweight, qzeros, scales, g_idx, bias, bits: int, group_size: in
 class _Workspace:
     def __init__(self):
         self.busy = threading.Lock()
-        self.bytes = None
+        self.bytes = None       # of eager calls
+        self.captured = None    # of the capture `capture`
+        self.capture = 0
+
+
+def _capture(stream: int):
+    """0, or what tells the graph capture that the stream is in from every other (without the native library: from every other call)."""
+    if CALL is not None:
+        return CALL.capture(stream)
+    return object() if torch.cuda.is_current_stream_capturing() else 0
 
 
 _workspaces = {}
@@ -82,16 +91,27 @@ def _workspace(device: torch.device, nbytes: int, kind: int = 0):
     launches of one call: they hand x or partial sums on through it, and those of another thread on the same stream must
     not come between.  The kernels leave its counters at zero, so it is cleared only when it is (re)allocated.  kind 1: the
     decode plans of the tiled family with halved tiles, whose kernel keeps ALL their bytes zero between launches (the slots
-    through which the two halves of a tile meet); they do not share the workspace other plans pack x or partial sums into."""
+    through which the two halves of a tile meet); they do not share the workspace other plans pack x or partial sums into.
+    Captured launches keep the address while their graph lives: a capture has a workspace of its own, from the graph's pool, whose
+    counters (kind 1: all of it) the graph clears."""
     if not nbytes:
         yield None
         return
-    key = (device.index, _stream(device).value, kind)
-    ws = _workspaces.setdefault(key, _Workspace())
+    stream = _stream(device).value or 0
+    ws = _workspaces.setdefault((device.index, stream, kind), _Workspace())
     with ws.busy:
-        if ws.bytes is None or ws.bytes.numel() < nbytes:
-            ws.bytes = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        yield ws.bytes
+        capture = _capture(stream)
+        if ws.capture != capture:
+            ws.captured, ws.capture = None, capture
+        own = ws.captured if capture else ws.bytes
+        if own is None or own.numel() < nbytes:
+            own = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+            (own[:1 << 16] if capture and kind == 0 else own).zero_()
+            if capture:
+                ws.captured = own
+            else:
+                ws.bytes = own
+        yield own
 
 
 def gemm(x: torch.Tensor, qweight: torch.Tensor, qzeros: torch.Tensor, scales: torch.Tensor,

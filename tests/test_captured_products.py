@@ -70,3 +70,27 @@ def test_captures_replay_in_any_order():
         torch.cuda.synchronize()
         for i in set(order):
             assert torch.equal(made[i][1], want[i]), (order, i)
+
+
+def test_gradients_replay_after_calls_that_need_more():
+    """(The gradient's calls go through the front end in Python, which keeps workspaces of its own.)"""
+    K, N = 2176, 4096
+    q = make(13, K, N)
+    gen = torch.Generator().manual_seed(14)
+    gs = {M: torch.randn(M, N, generator=gen).half().cuda() for M in (20, 38, 70, 300, 1000)}
+    want = {M: q.grad_input(g) for M, g in gs.items()}
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    made = {M: capture(stream, lambda: q.grad_input(gs[M])) for M in (20, 38, 70)}
+    for order in ((38, 20, 70), (70, 38), (20, 70)):
+        with torch.cuda.stream(stream):
+            later = {n: q.grad_input(g) for n, g in gs.items()}
+            junk = overwrite()
+            for M in order:
+                made[M][1].zero_()
+                made[M][0].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(made[M][1], want[M]) for M in order), order
+        assert all(torch.equal(y, want[n]) for n, y in later.items())
+        assert all(bool((j == 0x7f).all()) for j in junk), "a replay wrote into another tensor"
+        del junk

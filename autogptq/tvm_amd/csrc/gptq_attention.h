@@ -12,11 +12,13 @@
 // Parts.  The keys of a tile may be divided among workgroups.  Each leaves m, l and o of its part in the workspace.  Parts of few
 // rows are joined by the workgroup that comes last, those of up to 128 by a launch of their own.
 //
-// Statistics.  Scores are kept in units of log2(e): p = 2^(c q.k - m) with c = scale * log2(e), m the running maximum, l
-// the sum of p and o the sum of p v, all in 32 bits.  p is rounded to the cache's type for the matrix instruction (the
-// largest p of a row is 1, so its error is at most the rounding of that type, relative to the largest share of a row).
-// m is raised, and o and l scaled down, only when a score passes it by 2^8: until then p is at most 2^8, far from the
-// largest fp16 and with the same relative rounding, and most tiles of keys need no pass over o.
+// Statistics.  Scores are kept in units of log2(e): p = 2^(c q.k - m) with c = scale * log2(e), m the row's reference, l the sum
+// of p and o the sum of p v, all in 32 bits.  m is set `lift` below the running maximum, and raised, with o and l scaled down,
+// only when a score passes it by `most`: most tiles of keys need no pass over o.  p is rounded to the cache's type for the matrix
+// instruction.  bf16 has the exponents of 32 bits: every p keeps the relative rounding of the type.  fp16 keeps it from 2^-14 up
+// and holds multiples of 2^-24 below, so its p are lifted to the upper end of the type: shares down to 2^-(14 + lift) of a row's
+// largest have the type's relative rounding, smaller ones an error of at most 2^-(25 + lift) of the largest.  (Parts that are
+// joined are of one type, hence of one lift, which o / l does not show.)
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -169,6 +171,18 @@ __device__ __forceinline__ float max_halves(float x) { const f2 r = swap_halves(
 __device__ __forceinline__ float add_halves(float x) { const f2 r = swap_halves(x); return r[0] + r[1]; }
 __device__ __forceinline__ float max_quarters(float x) { const f2 r = swap_quarters(max_halves(x)); return fmaxf(r[0], r[1]); }
 __device__ __forceinline__ float add_quarters(float x) { const f2 r = swap_quarters(add_halves(x)); return r[0] + r[1]; }
+
+// How far a score may pass a row's reference, and how far below the row's maximum the reference is set.  (fp16 holds 2^15.  A larger lift
+// keeps smaller shares whole and raises references more often: prompts of 4096 tokens, 16 heads of 256, take 215, 217, 219, 222 and 231 us
+// with 7, 9, 10, 11 and 13, and 243 with 15; 8192 of 32 heads of 128 600, 602, 602, 603, 615 and 626.)
+template <typename E>
+struct Shares {
+    static constexpr float most = 8.0f, lift = 0.0f;
+};
+template <>
+struct Shares<_Float16> {
+    static constexpr float most = 15.0f, lift = 9.0f;
+};
 
 constexpr float kNone = -__builtin_inff();
 // the reference of a row that has seen nothing yet (its p are 2^(-inf) = 0)

@@ -277,8 +277,8 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                         float top = fmaxf(fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), fmaxf(s[rt][0][2], s[rt][0][3])),
                                           fmaxf(fmaxf(s[rt][1][0], s[rt][1][1]), fmaxf(s[rt][1][2], s[rt][1][3])));
                         top = max_quarters(top);
-                        if (__ballot(top > m[rt] + 8.0f)) {
-                            const float up = fmaxf(m[rt], top);
+                        if (__ballot(top > m[rt] + Shares<E>::most)) {
+                            const float up = fmaxf(m[rt], top - Shares<E>::lift);
                             const float down = __builtin_amdgcn_exp2f(m[rt] - reference(up));
                             m[rt] = up;
                             l[rt] *= down;

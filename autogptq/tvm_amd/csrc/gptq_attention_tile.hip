@@ -234,8 +234,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
 #pragma unroll
             for (int i = 0; i < 16; i++) top = fmaxf(top, s[a][i]);
         top = max_halves(top) * p.c;
-        if (__ballot(top > m + 8.0f)) {
-            const float up = fmaxf(m, top);
+        if (__ballot(top > m + Shares<E>::most)) {
+            const float up = fmaxf(m, top - Shares<E>::lift);
             const float down = __builtin_amdgcn_exp2f(m - reference(up));
             m = up;
             l *= down;

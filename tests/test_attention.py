@@ -445,3 +445,36 @@ def test_a_capture_that_grows_its_workspace():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def one_high_key(s, gap, at):
+    """Key `at` of every request (of the prefix and its context together) lies `gap` octaves above all others and has no value: the
+    output is what the others' small shares make of it."""
+    gen = torch.Generator().manual_seed(41)
+    noise = lambda *shape: (torch.randn(*shape, generator=gen) * 0.25).to(s.dtype).to(s.q.device)
+    s.q = noise(*s.q.shape)
+    s.q[..., 0] = 4.0
+    front = noise(s.prefix, s.kv_heads, s.dim)
+    for b, (c, _) in enumerate(s.requests):
+        s.k[b] = torch.cat([front, noise(c, s.kv_heads, s.dim)])
+        s.k[b][..., 0] = 0.0
+        s.k[b][at] = 0.0
+        s.k[b][at, :, 0] = gap * 0.6931 * s.dim ** 0.5 / 4
+        s.v[b][at] = 0.0
+        p, blocks = s.prefix, -(-c // s.block_size)
+        s._fill(s.prefix_blocks, s.k[b][:p], s.v[b][:p], 0)
+        s._fill(s.tables[b, :blocks], s.k[b][p:], s.v[b][p:], 0)
+    return s
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [16.0, 22.3, 24.6])
+@pytest.mark.parametrize("requests, dim, dtype, prefix, at", [
+    ([(30000, 1)], 128, HALF, 0, 0), ([(9000, 1), (300, 1)], 64, HALF, 0, 3), ([(3000, 1), (500, 2)], 256, HALF, 0, 299),
+    ([(9000, 40)], 128, HALF, 0, 0), ([(2000, 90), (150, 60)], 64, HALF, 0, 5), ([(3000, 50)], 256, HALF, 0, 1000),
+    ([(400, 300)], 80, HALF, 0, 0), ([(20, 1), (900, 1)] * 3, 128, HALF, 9000, 0), ([(20, 1), (900, 1)], 128, HALF, 300, 250),
+    ([(300, 40)] * 3, 128, HALF, 3000, 2), ([(9000, 1)], 128, BF16, 0, 0), ([(9000, 40)], 128, BF16, 0, 0)])
+def test_shares_far_below_the_largest(requests, dim, dtype, prefix, at, gap):
+    """(One key holds nearly all of every row: what remains has shares of 2^-16 to 2^-25 of it, and makes the output.)"""
+    s = one_high_key(Step(40, requests, 4, 2, dim, 16, dtype, prefix=prefix), gap, at)
+    assert_attention(attend(s), s, f"{gap} octaves")

@@ -55,7 +55,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     last of them at position ``contexts[b] - 1`` (their keys are in the cache already); a token at position i sees the
     positions j <= i, under a ``window`` only j > i - window and the first ``sinks``.  Blocks that no token of a request
     sees may be given back: their table entries are not read, nor are slots past a context.  Values are finite up to a request's
-    last token (one that a token does not see may still count for it, with the share 0).  A token that sees nothing gets zeros.  Query head n reads
+    last token (one that a token does not see may still count for it, with the share 0).  A token that sees nothing gets zeros, and so do
+    tokens of no request (those from ``starts[-1]`` on: a step may be padded to a fixed size).  Query head n reads
     key/value head n // (heads / kv_heads).  ``max_context``: the longest context as the host knows it, by which the work is
     divided (0: the tables' width); results do not depend on it beyond the order of sums.  ``scale``: 1 / sqrt(dim) if None."""
     return _call("paged_attention", q, k_cache, v_cache, tables, starts, contexts, max_context, window, sinks, _scale(scale))

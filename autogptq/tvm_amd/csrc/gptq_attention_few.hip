@@ -91,6 +91,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
     Requests look = {};
     if (!SHARED) {
         look = look_at<R>(given, 0);
+        clear_rest(given, given.starts[0], given.starts[given.requests], blockIdx.x * (64ll * kFewWaves) + threadIdx.x, gridDim.x * (64ll * kFewWaves));
         upto = sum_upto(look.total);
         int total = __builtin_amdgcn_readlane(upto, 63);
         for (int b = 64; b < given.requests; b += 64) total += __builtin_amdgcn_readlane(sum_upto(look_at<R>(given, b).total), 63);

@@ -113,7 +113,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
     // the last rows of a request see the most keys: they come first
     const int h = blockIdx.x % p.kv_heads, tile = p.tiles - 1 - blockIdx.x / p.kv_heads, split = blockIdx.y;
     QueryTile q;
-    if (!find_tile<kTileRows>(p, tile, q)) return;
+    const int first_token = p.shared ? 0 : p.starts[0], end_token = p.shared ? p.tokens : p.starts[p.requests];
+    const bool found = find_tile<kTileRows>(p, tile, q);
+    if (!p.shared) clear_rest(p, first_token, end_token, (blockIdx.y * (long long)gridDim.x + blockIdx.x) * 256 + threadIdx.x, 256ll * gridDim.x * gridDim.y);
+    if (!found) return;
     int chunk;
     const int parts = tile_parts(p, q.seen, KT, chunk);
     if (split >= parts) return;

@@ -399,7 +399,8 @@ int gptq_hip_cache_write(const gptq_hip_cache *cache, const void *k, const void 
  * them: request b has the tokens starts[b] .. starts[b + 1] - 1, the last of them at position contexts[b] - 1, and the
  * query at position i sees the keys j <= i; with window > 0 only those with j > i - window or j < sinks (first tokens that
  * stay visible).  Query head n reads key/value head n / (heads / cache.heads).
- *   out[t, n] = sum_j softmax_j(scale q[t, n] . k[j]) v[j], zeros for a token that sees nothing
+ *   out[t, n] = sum_j softmax_j(scale q[t, n] . k[j]) v[j], zeros for a token that sees nothing, and for one of no request
+ *     (before starts[0] or from starts[requests] on: a step may be padded)
  * q [tokens, heads, dim] in the cache's type (16-byte aligned, strides in elements, multiples of 8), out [tokens, heads,
  * dim] contiguous, 16-byte aligned.  scale > 0.  Scores, softmax and sums are fp32; shares of the softmax are rounded to the cache's
  * type for the product with v, the result once.  Table entries of blocks that no token of a request sees are

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from autogptq.tvm_amd import _lib, attention
-from tests.attention_util import Step, assert_attention
+from tests.attention_util import ROUNDING, Step, assert_attention
 
 HALF, BF16 = torch.float16, torch.bfloat16
 
@@ -478,3 +478,22 @@ def test_shares_far_below_the_largest(requests, dim, dtype, prefix, at, gap):
     """(One key holds nearly all of every row: what remains has shares of 2^-16 to 2^-25 of it, and makes the output.)"""
     s = one_high_key(Step(40, requests, 4, 2, dim, 16, dtype, prefix=prefix), gap, at)
     assert_attention(attend(s), s, f"{gap} octaves")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("requests, heads, kv_heads, dim, prefix", [
+    ([(40, 1), (700, 1)], 8, 2, 128, 0), ([(5, 0), (0, 0)], 4, 2, 64, 0), ([(3, 1)], 7, 1, 72, 0), ([(40, 3), (7, 2)], 16, 2, 128, 0),
+    ([(300, 300)], 4, 2, 128, 0), ([(3000, 60), (64, 64)], 4, 1, 64, 0), ([(300, 150)], 4, 2, 256, 0),
+    ([(40, 1), (30, 1)], 8, 2, 128, 100), ([(40, 1), (30, 1)], 8, 2, 128, 9000), ([(300, 90)], 8, 1, 80, 3000)])
+@pytest.mark.parametrize("ahead, behind", [(0, 1), (0, 300), (3, 5)])
+def test_tokens_of_no_request_get_zeros(requests, heads, kv_heads, dim, prefix, ahead, behind):
+    s = Step(42, requests, heads, kv_heads, dim, 16, prefix=prefix)
+    want, size = s.expected()
+    n = s.tokens
+    s.q = torch.cat([torch.full((ahead, heads, dim), float("nan"), device="cuda").half(), s.q,
+                     torch.full((behind, heads, dim), float("nan"), device="cuda").half()])
+    s.starts += ahead
+    torch.full(s.q.shape, float("nan"), dtype=s.dtype, device="cuda")      # what the result's memory holds
+    got = attend(s)
+    assert bool((got[:ahead] == 0).all()) and bool((got[ahead + n:] == 0).all())
+    assert bool(((got[ahead:ahead + n].double() - want).abs() <= 2.25 * ROUNDING[s.dtype] * size + 2.0 ** -24).all())

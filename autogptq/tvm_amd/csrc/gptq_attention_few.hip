@@ -68,8 +68,9 @@ __device__ __forceinline__ int sum_upto(int x)
     return x;
 }
 
-// DP: compiled width, the dims past p.dim do not count; RT: 16-row operands a wave holds; SHARED: the parts of a shared prefix
-template <typename E, int DP, int RT, bool SHARED>
+// DP: compiled width, the dims past p.dim do not count; FULL: there are none; RT: 16-row operands a wave holds; SHARED: the parts of a
+// shared prefix
+template <typename E, int DP, bool FULL, int RT, bool SHARED>
 __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + (DP == 64)) void attention_few_kernel(const AttentionParams given)
 {
     typedef typename Vec<E>::e8 e8;
@@ -111,6 +112,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
         const int lane = thread & 63, i16 = lane & 15, g = lane >> 4;
         const int wave = __builtin_amdgcn_readfirstlane(thread >> 6);
         const AttentionParams &p = *(const AttentionParams *)((const __attribute__((address_space(4))) char *)__builtin_amdgcn_kernarg_segment_ptr() + first_argument);
+        const int dim = FULL ? DP : p.dim;
         const char *kbase = (const char *)p.k + (long long)h * p.head_stride * 2;
         const char *vbase = (const char *)p.v + (long long)h * p.head_stride * 2;
 
@@ -168,7 +170,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
             for (int s = 0; s < KS; s++) {
                 const int d = 32 * s + 8 * g;
                 u4 x = {0u, 0u, 0u, 0u};
-                if (d < p.dim) x = *(const u4 *)(src + d * 2);
+                if (d < dim) x = *(const u4 *)(src + d * 2);
                 qf[rt][s] = __builtin_bit_cast(e8, x);
             }
         }
@@ -184,8 +186,8 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                 for (int t = 0; t < VE; t++) o[rt][vh][t] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        // (Dims past p.dim: the last ones again.  Of keys they meet zeros of the query, of values they reach dims of o that are
-        // not stored.)
+        // (Dims past p.dim: the last ones again.  Of keys they are cleared before they meet the query's zeros, which an infinity would
+        // turn into a NaN; of values they reach dims of o that are not stored.)
         u4 kr[2][KS];
         uint32_t vr[8][VH][VW];
         auto load_keys = [&](const uint32_t *rows) {
@@ -194,7 +196,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                 const char *src = kbase + (unsigned long long)rows[16 * a + i16] * 16;
 #pragma unroll
                 for (int s = 0; s < KS; s++) {
-                    kr[a][s] = *(const u4 *)(src + min(32 * s + 8 * g, p.dim - 8) * 2);
+                    kr[a][s] = *(const u4 *)(src + min(32 * s + 8 * g, dim - 8) * 2);
                 }
             }
         };
@@ -204,7 +206,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                 const char *src = vbase + (unsigned long long)rows[16 * (j / 4) + 4 * g + j % 4] * 16;
 #pragma unroll
                 for (int vh = 0; vh < VH; vh++) {
-                    const char *from = src + min(128 * vh + VE * i16, p.dim - VE) * 2;
+                    const char *from = src + min(128 * vh + VE * i16, dim - VE) * 2;
                     if constexpr (VW == 4) {
                         const u4 x = *(const u4 *)from;
 #pragma unroll
@@ -243,6 +245,13 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                     // the rows of this wave's next block
                     const uint32_t *rows = half ? list[wave][turn ^ 1] : list[wave][turn] + 32;
                     const bool load = block + NW < blocks;
+                    if constexpr (!FULL) {
+#pragma unroll
+                        for (int a = 0; a < 2; a++)
+#pragma unroll
+                            for (int x = DP == 64 ? 0 : KS / 2; x < KS; x++)     // (wider kernels take dims above DP / 2)
+                                if (32 * x + 8 * g >= dim) kr[a][x] = (u4){0u, 0u, 0u, 0u};
+                    }
                     // S^T
                     f4 s[RT][2];
 #pragma unroll
@@ -344,7 +353,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
             __syncthreads();
             for (int x = threadIdx.x; x < 16 * (DP / 4); x += 64 * NW) {
                 const int r = x / (DP / 4), d = x % (DP / 4) * 4, row = 16 * rt + r;
-                if (row >= q.rows || d >= p.dim) continue;
+                if (row >= q.rows || d >= dim) continue;
                 float top = kNone, sum = 0.0f, ms[NW];
 #pragma unroll
                 for (int w = 0; w < NW; w++) {
@@ -366,10 +375,10 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                 if (whole) {
                     Sum x = {top, sum, total};
                     add_prefix(p, x, at_row, d);
-                    store_row4<E>(p.out, at_row * p.dim + d, x.result());
+                    store_row4<E>(p.out, at_row * dim + d, x.result());
                 } else {
                     const long long to = SHARED ? blockIdx.y * all + at_row : mine + row;
-                    put_part<!SHARED>((SHARED ? p.parts : p.own_parts) + to * p.dim + d, total);
+                    put_part<!SHARED>((SHARED ? p.parts : p.own_parts) + to * dim + d, total);
                     if (d == 0) put_stats<!SHARED>((SHARED ? p.stats : p.own_stats) + 2 * to, top, sum);
                 }
             }
@@ -389,13 +398,21 @@ template <typename E, bool SHARED>
 static void launch_few(const AttentionParams &p, int rt, hipStream_t stream)
 {
     const dim3 grid((unsigned)(p.kv_heads * (SHARED ? p.tiles : p.team)), SHARED ? (unsigned)p.splits : 1u);
-#define GPTQ_FEW(DP, RT) hipLaunchKernelGGL((attention_few_kernel<E, DP, RT, SHARED>), grid, dim3(64 * kFewWaves), 0, stream, p)
+#define GPTQ_FEW(DP, RT) \
+    if (p.dim == DP) hipLaunchKernelGGL((attention_few_kernel<E, DP, true, RT, SHARED>), grid, dim3(64 * kFewWaves), 0, stream, p); \
+    else hipLaunchKernelGGL((attention_few_kernel<E, DP, false, RT, SHARED>), grid, dim3(64 * kFewWaves), 0, stream, p)
     if (p.dim <= 64) {
-        if (rt == 1) GPTQ_FEW(64, 1);
-        else GPTQ_FEW(64, 2);
+        if (rt == 1) {
+            GPTQ_FEW(64, 1);
+        } else {
+            GPTQ_FEW(64, 2);
+        }
     } else if (p.dim <= 128) {
-        if (rt == 1) GPTQ_FEW(128, 1);
-        else GPTQ_FEW(128, 2);
+        if (rt == 1) {
+            GPTQ_FEW(128, 1);
+        } else {
+            GPTQ_FEW(128, 2);
+        }
     } else {
         GPTQ_FEW(256, 1);
     }

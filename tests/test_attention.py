@@ -497,3 +497,17 @@ def test_tokens_of_no_request_get_zeros(requests, heads, kv_heads, dim, prefix, 
     got = attend(s)
     assert bool((got[:ahead] == 0).all()) and bool((got[ahead + n:] == 0).all())
     assert bool(((got[ahead:ahead + n].double() - want).abs() <= 2.25 * ROUNDING[s.dtype] * size + 2.0 ** -24).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("requests", [[(300, 1), (70, 1)], [(130, 3), (40, 2)], [(300, 150)]])
+@pytest.mark.parametrize("dim", [8, 40, 64, 72, 96, 128, 200, 256])
+def test_a_key_that_is_minus_infinity_has_no_share(dim, requests):
+    """(In its last dimension, where the products of widths that are no power of two end.)"""
+    s = Step(43, requests, 4, 2, dim, 16)
+    s.q[..., -1] = s.q[..., -1].abs() + 0.125
+    for b in range(len(requests)):
+        for j in (5, 33):
+            s.k[b][j, :, -1] = -float("inf")
+            s.k_cache[int(s.tables[b, j // 16]), j % 16, :, -1] = -float("inf")
+    assert_attention(attend(s), s, "a key of minus infinity")

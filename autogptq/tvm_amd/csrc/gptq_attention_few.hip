@@ -76,6 +76,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
     typedef typename Vec<E>::e8 e8;
     constexpr int R = 16 * RT, NW = kFewWaves;
     constexpr int KS = DP / 32;                    // matrix instructions along dim for S
+    constexpr int FIRST = DP == 64 ? 0 : KS / 2;   // the first of them that may hold dims past p.dim (wider kernels take dims above DP / 2)
     constexpr int VE = DP >= 128 ? 8 : DP / 16;    // dims a lane loads of a value row at a time
     constexpr int VH = DP / 16 / VE;               // ... that many times
     constexpr int VW = VE / 2;                     // dwords of that
@@ -186,9 +187,15 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                 for (int t = 0; t < VE; t++) o[rt][vh][t] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        // (Dims past p.dim: the last ones again.  Of keys they are cleared before they meet the query's zeros, which an infinity would
-        // turn into a NaN; of values they reach dims of o that are not stored.)
+        // (Dims past p.dim: of keys their lanes load nothing and hold zeros, since an infinity times the query's zeros would be a NaN;
+        // of values they are the last ones again, and reach dims of o that are not stored.)
         u4 kr[2][KS];
+        if constexpr (!FULL) {
+#pragma unroll
+            for (int a = 0; a < 2; a++)
+#pragma unroll
+                for (int s = FIRST; s < KS; s++) kr[a][s] = (u4){0u, 0u, 0u, 0u};
+        }
         uint32_t vr[8][VH][VW];
         auto load_keys = [&](const uint32_t *rows) {
 #pragma unroll
@@ -196,7 +203,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                 const char *src = kbase + (unsigned long long)rows[16 * a + i16] * 16;
 #pragma unroll
                 for (int s = 0; s < KS; s++) {
-                    kr[a][s] = *(const u4 *)(src + min(32 * s + 8 * g, dim - 8) * 2);
+                    if (FULL || s < FIRST || 32 * s + 8 * g < dim) kr[a][s] = *(const u4 *)(src + (32 * s + 8 * g) * 2);
                 }
             }
         };
@@ -245,13 +252,6 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                     // the rows of this wave's next block
                     const uint32_t *rows = half ? list[wave][turn ^ 1] : list[wave][turn] + 32;
                     const bool load = block + NW < blocks;
-                    if constexpr (!FULL) {
-#pragma unroll
-                        for (int a = 0; a < 2; a++)
-#pragma unroll
-                            for (int x = DP == 64 ? 0 : KS / 2; x < KS; x++)     // (wider kernels take dims above DP / 2)
-                                if (32 * x + 8 * g >= dim) kr[a][x] = (u4){0u, 0u, 0u, 0u};
-                    }
                     // S^T
                     f4 s[RT][2];
 #pragma unroll

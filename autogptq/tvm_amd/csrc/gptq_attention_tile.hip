@@ -81,7 +81,7 @@ __device__ __forceinline__ int tile_parts(const AttentionParams &p, int seen, in
 // request before each read of LDS; the kernel waits for them at its barrier.
 __device__ __forceinline__ void request16(const char *src, uint32_t lds)
 {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "m0", "memory");
 }
 
 // a 4 x 16 block of 16-bit values of a row-major matrix, as 16 lanes hold its columns: lane x gets rows 0 .. 3 of column x,

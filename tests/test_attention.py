@@ -511,3 +511,19 @@ def test_a_key_that_is_minus_infinity_has_no_share(dim, requests):
             s.k[b][j, :, -1] = -float("inf")
             s.k_cache[int(s.tables[b, j // 16]), j % 16, :, -1] = -float("inf")
     assert_attention(attend(s), s, "a key of minus infinity")
+
+
+def test_assembly_declares_what_it_writes():
+    """Requests into LDS write m0: the compiler must know."""
+    import os
+    import re
+    csrc = os.path.dirname(_lib.LIB_PATH)
+    seen = 0
+    for name in os.listdir(csrc):
+        if name.startswith("gptq_attention"):
+            with open(os.path.join(csrc, name), encoding="utf-8") as f:
+                for statement in re.findall(r"asm volatile\(.*?\);", f.read(), re.S):
+                    if re.search(r"\bm0, ", statement):
+                        seen += 1
+                        assert '"m0"' in statement, (name, statement)
+    assert seen == 1

@@ -139,6 +139,8 @@ void gptq_torch::cache_write(const Tensor &k, const Tensor &v, const Tensor &k_c
 {
     on_gpu(k_cache, "k_cache", k_cache);
     const gptq_hip_cache c = describe(k_cache, v_cache);
+    no_grad(k_cache, "k_cache");
+    no_grad(v_cache, "v_cache");
     for (const Tensor *t : {&k, &v}) {
         const char *name = t == &k ? "k" : "v";
         on_gpu(*t, name, k_cache);
@@ -167,6 +169,8 @@ static Tensor attend(const char *what, const Tensor &q, const Tensor &k_cache, c
     a.cache = describe(k_cache, v_cache);
     on_gpu(q, "q", k_cache);
     no_grad(q, "q");
+    no_grad(k_cache, "k_cache");
+    no_grad(v_cache, "v_cache");
     TORCH_CHECK(q.scalar_type() == k_cache.scalar_type(), "q is ", q.scalar_type(), ", the cache ", k_cache.scalar_type());
     TORCH_CHECK(q.dim() == 3 && q.size(2) == a.cache.dim, "q must be [tokens, heads, ", a.cache.dim, "], got ", q.sizes());
     TORCH_CHECK(q.size(1) > 0 && q.size(1) % a.cache.heads == 0, "q has ", q.size(1), " heads, no multiple of the cache's ", a.cache.heads);

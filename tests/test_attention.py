@@ -527,3 +527,20 @@ def test_assembly_declares_what_it_writes():
                         seen += 1
                         assert '"m0"' in statement, (name, statement)
     assert seen == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["k_cache", "v_cache"])
+def test_caches_that_require_grad_are_refused(which):
+    s = Step(44, [(40, 1), (30, 20)], 4, 2, 64, 16, prefix=20)
+    setattr(s, which, getattr(s, which).clone().requires_grad_())
+    k, v = torch.randn(2, 3, 2, 64, device="cuda").half()
+    slots = torch.arange(3, dtype=torch.int32, device="cuda")
+    calls = (lambda: attend(s), lambda: attention.cache_write(k, v, s.k_cache, s.v_cache, slots),
+             lambda: attention.paged_attention(s.q, s.k_cache, s.v_cache, s.tables, s.starts, s.contexts),
+             lambda: torch.ops.gptq_hip.cache_write(k, v, s.k_cache, s.v_cache, slots))
+    for call in calls:
+        with pytest.raises(RuntimeError, match=f"{which} requires grad"):
+            call()
+        with torch.no_grad():
+            call()

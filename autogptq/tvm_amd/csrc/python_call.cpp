@@ -11,6 +11,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -289,21 +290,29 @@ PyObject *capture(PyObject *, PyObject *arg)
 // ---- the serving operators
 // The same functions as torch.ops.gptq_hip.*, called with plain tensors and without the dispatcher, whose handling of ten
 // arguments costs as much as the shorter of these calls run (cache_tables for 64 requests 9.5 us a call through it, 5.5 so).
-// They return NotImplemented where something else wants to see the operator: a tensor subclass, a dispatch mode, a tracer.
+// They return NotImplemented where something else has to see the operator: a tensor subclass, a mode (of dispatch or of torch
+// functions), a tracer, a function transform (torch.func) or its tensors, a tensor that is not on a GPU (meta tensors have a shape to give).
+constexpr c10::DispatchKeySet kHandled({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                        c10::DispatchKey::BatchedNestedTensor, c10::DispatchKey::Functionalize,
+                                        c10::DispatchKey::Conjugate, c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor});
 struct Arguments {
     PyObject *const *args;
     bool plain = true;
     Arguments(PyObject *const *a, Py_ssize_t n, Py_ssize_t expected) : args(a)
     {
         TORCH_CHECK_TYPE(n == expected, expected, " arguments are expected, got ", n);
-        plain = !c10::impl::TorchDispatchModeTLS::any_modes_set() && !torch::jit::tracer::isTracing();
+        plain = !c10::impl::TorchDispatchModeTLS::any_modes_set() && !torch::jit::tracer::isTracing() &&
+                !at::impl::torch_function_mode_enabled() &&
+                !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) &&
+                !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Functionalize);
     }
     // (a reference to the caller's tensor, which its arguments keep alive)
     const Tensor &tensor(int i)
     {
         TORCH_CHECK_TYPE(THPVariable_Check(args[i]), "argument ", i, " must be a tensor");
-        plain = plain && THPVariable_CheckExact(args[i]);
-        return THPVariable_Unpack(args[i]);
+        const Tensor &t = THPVariable_Unpack(args[i]);
+        plain = plain && THPVariable_CheckExact(args[i]) && t.is_cuda() && !t.key_set().has_any(kHandled);
+        return t;
     }
     int64_t integer(int i) const
     {

@@ -544,3 +544,42 @@ def test_caches_that_require_grad_are_refused(which):
             call()
         with torch.no_grad():
             call()
+
+
+def test_meta_tensors_have_a_shape():
+    s = Step(45, [(40, 1), (30, 20)], 4, 2, 64, 16, device="cpu")
+    meta = lambda t: t.to("meta")
+    out = attention.paged_attention(*map(meta, (s.q, s.k_cache, s.v_cache, s.tables, s.starts, s.contexts)))
+    assert out.device.type == "meta" and out.shape == s.q.shape and out.dtype == s.q.dtype
+    made = attention.cache_tables(meta(s.contexts), meta(s.contexts), meta(s.tables), meta(s.contexts), 21, 16)
+    assert [len(x) for x in made] == [3, 2, 21, 21, 1]
+    k = torch.zeros(3, 2, 64, dtype=HALF, device="meta")
+    assert attention.cache_write(k, k, meta(s.k_cache), meta(s.v_cache), meta(torch.arange(3, dtype=torch.int32))) is None
+
+
+@pytest.mark.gpu
+def test_function_modes_and_transforms_see_the_operators():
+    from torch.overrides import TorchFunctionMode
+
+    s = Step(46, [(40, 1), (30, 20)], 4, 2, 64, 16)
+    rest = (s.k_cache, s.v_cache, s.tables, s.starts, s.contexts)
+    want = attend(s)
+
+    class Mode(TorchFunctionMode):
+        seen = []
+
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            self.seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+    with Mode():
+        got = attend(s)
+        attention.cache_write(s.k_cache[0, :3], s.v_cache[0, :3], s.k_cache, s.v_cache, torch.full((3,), -1, dtype=torch.int32, device="cuda"))
+        attention.cache_tables(s.contexts, s.contexts, s.tables.clone(), s.contexts, 70, 16)
+    assert torch.equal(got, want)
+    for name in ("paged_attention", "cache_write", "cache_tables"):
+        assert any(name in f for f in Mode.seen), (name, Mode.seen)
+    qs = torch.stack([s.q, s.q * 0.5, s.q.flip(0)])
+    got = torch.func.vmap(lambda q: attention.paged_attention(q, *rest))(qs)
+    assert got.shape == qs.shape
+    for g, q in zip(got, qs):
+        assert torch.equal(g, attention.paged_attention(q, *rest))

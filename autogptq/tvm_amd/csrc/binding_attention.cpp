@@ -92,6 +92,12 @@ void raised(int rc, const char *what)
     TORCH_CHECK(rc == GPTQ_HIP_OK, what, " failed: ", gptq_hip_strerror(rc), " [status ", rc, "]");
 }
 
+// (the dispatcher counts the writes of torch's own operators only)
+void written(const Tensor &t)
+{
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor fresh(at::IntArrayRef sizes, const Tensor &like)
 {
     return at::detail::empty_cuda(sizes, like.scalar_type(), like.device(), std::nullopt);
@@ -132,6 +138,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gptq_torch::cache_tables(cons
                                  (int32_t *)contexts.data_ptr(), (int32_t *)slots.data_ptr(), (int32_t *)positions.data_ptr(),
                                  (int32_t *)taken.data_ptr(), current_stream(lengths)),
            "gptq_hip_cache_tables");
+    written(tables);
     return {out[0], out[1], out[2], out[3], out[4]};
 }
 
@@ -158,6 +165,8 @@ void gptq_torch::cache_write(const Tensor &k, const Tensor &v, const Tensor &k_c
     raised(gptq_hip_cache_write(&c, ks.data_ptr(), vs.data_ptr(), step(ks, 0), step(ks, 1), step(vs, 0), step(vs, 1),
                                 (const int32_t *)slots.data_ptr(), (int)k.size(0), current_stream(k_cache)),
            "gptq_hip_cache_write");
+    written(k_cache);
+    written(v_cache);
 }
 
 static Tensor attend(const char *what, const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &prefix_blocks,

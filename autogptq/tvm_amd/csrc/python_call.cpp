@@ -360,9 +360,6 @@ PyObject *call_cache_write(PyObject *, PyObject *const *args, Py_ssize_t n)
     {
         const WithoutInterpreter free;
         cache_write(k, v, k_cache, v_cache, slots);
-        // (what the dispatcher does for arguments that are written)
-        for (const Tensor *t : {&k_cache, &v_cache})
-            if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     }
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS

@@ -163,3 +163,22 @@ def test_the_entry_points_refuse():
     for more in (dict(c=None), dict(k=None), dict(k=0x1004), dict(strides=(128, 64, 130, 64)), dict(slots=None), dict(T=-1)):
         assert write(**more) == _lib.ERR_BAD_ARG, more
     assert write(T=0) == _lib.OK
+
+
+@pytest.mark.gpu
+def test_what_is_written_counts_as_written():
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    for call in (attention.cache_tables, torch.ops.gptq_hip.cache_tables):
+        tables = torch.full((2, 4), -1, dtype=torch.int32, device="cuda")
+        before = tables._version
+        call(ints(0, 3), ints(2, 2), tables, ints(5, 6, 7), 4, 2)
+        assert tables._version > before, call
+    with torch.inference_mode():
+        tables = torch.full((2, 4), -1, dtype=torch.int32, device="cuda")
+        attention.cache_tables(ints(0, 3), ints(2, 2), tables, ints(5, 6, 7), 4, 2)
+    for call in (attention.cache_write, torch.ops.gptq_hip.cache_write):
+        cache = torch.zeros(2, 4, 16, 2, 64, device="cuda", dtype=torch.float16)
+        k, v = torch.ones(2, 3, 2, 64, device="cuda", dtype=torch.float16)
+        before = cache._version
+        call(k, v, cache[0], cache[1], ints(0, 1, 2))
+        assert cache._version > before, call

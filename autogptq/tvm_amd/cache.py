@@ -40,6 +40,7 @@ class PagedCache:
         self._lengths = [0] * max_requests                  # the host's, and the same on the GPU
         self._on_gpu = torch.zeros(max_requests, dtype=torch.int32, device=device)
         self._prefixes: List[Optional[Tuple[torch.Tensor, int]]] = [None] * max_requests
+        self._source: List[Optional[int]] = [None] * max_requests       # whose prefix that is
         self._kept = [(0, 0)] * max_requests                # blocks [a, b) of a request that trim() has given back
         self._rows = ((), None)                             # the requests of the last step, as a tensor
 
@@ -56,21 +57,27 @@ class PagedCache:
 
     def share(self, source: int, request: int) -> None:
         """``request`` (without tokens so far) stands behind the tokens that ``source`` has now, whose blocks it reads and does
-        not own: ``source`` gets no more tokens and is not freed while others stand behind it."""
+        not own: ``source`` is neither trimmed nor freed while others stand behind it.  (What it gets later they do not see.)"""
         if self._lengths[request] or self._prefixes[request] is not None:
             raise ValueError(f"request {request} has tokens already")
         if self._prefixes[source] is not None or self._kept[source] != (0, 0):
             raise ValueError(f"request {source} stands behind a prefix itself, or was trimmed")
         n = self._lengths[source]
-        self._prefixes[request] = (self.tables[source, :self._blocks(n)], n) if n else None
+        if n:
+            self._prefixes[request], self._source[request] = (self.tables[source, :self._blocks(n)], n), source
+
+    def _alone(self, request: int) -> None:
+        behind = [r for r, s in enumerate(self._source) if s == request]
+        if behind:
+            raise ValueError(f"requests {behind} stand behind the tokens of request {request}")
 
     def step(self, requests: Sequence[int], counts: Sequence[int]) -> Step:
         """Makes room for ``counts[i]`` more tokens of ``requests[i]``.  Raises before anything is launched if there is none."""
         requests = tuple(requests)
         if len(set(requests)) != len(requests) or len(requests) != len(counts) or min(counts, default=0) < 0:
             raise ValueError("requests must be distinct, with a count of at least 0 each")
-        prefixes = {id(self._prefixes[r][0]) if self._prefixes[r] else 0: self._prefixes[r] for r in requests}
-        if len({(p[0].data_ptr(), p[1]) if p else None for p in prefixes.values()}) > 1:
+        prefixes = [self._prefixes[r] for r in requests]
+        if len({(self._source[r], p[1]) if p else None for r, p in zip(requests, prefixes)}) > 1:
             raise ValueError("the requests of a step must stand behind one prefix, or all behind none")
         after = [self._lengths[r] + n for r, n in zip(requests, counts)]
         if max(after, default=0) > self.tables.shape[1] * self.block_size:
@@ -92,7 +99,7 @@ class PagedCache:
         self._free = self._free[need:]
         for r, a in zip(requests, after):
             self._lengths[r] = a
-        prefix = next(iter(prefixes.values()), None)
+        prefix = prefixes[0] if prefixes else None
         return Step(tables, made.starts, made.contexts, made.slots, made.positions + prefix[1] if prefix else made.positions,
                     max(after, default=0), prefix)
 
@@ -117,6 +124,9 @@ class PagedCache:
         many.  From then on the request is attended to with this window and these sinks, or narrower ones."""
         if window < 1:
             raise ValueError("trim needs a window")
+        if self._prefixes[request] is not None:
+            raise NotImplementedError("a sliding window behind a shared prefix")
+        self._alone(request)
         first, last = self._blocks(sinks), max(0, self._lengths[request] + 1 - window) // self.block_size
         first = max(first, self._kept[request][1])
         if last <= first:
@@ -129,12 +139,14 @@ class PagedCache:
 
     def free(self, request: int) -> None:
         """Ends a request: its blocks are free again."""
+        self._alone(request)
         a, b = self._kept[request]
         n = self._blocks(self._lengths[request])
         self._free = torch.cat([self._free, self.tables[request, :a], self.tables[request, b:n]])
         self.tables[request] = -1
         self._on_gpu[request] = 0
-        self._lengths[request], self._prefixes[request], self._kept[request] = 0, None, (0, 0)
+        self._lengths[request], self._kept[request] = 0, (0, 0)
+        self._prefixes[request] = self._source[request] = None
 
 
 __all__ = ["PagedCache", "Step"]

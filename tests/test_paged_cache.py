@@ -96,3 +96,88 @@ def test_refusals():
         c.trim(0, 0)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         c.step([1], [3])
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """The bookkeeping without a GPU: cache_tables request by request, on CPU tensors."""
+    from autogptq.tvm_amd import attention
+
+    def cache_tables(lengths, counts, tables, free, tokens, block):
+        taken, slots, positions, starts = 0, [], [], [0]
+        for b, (held, n) in enumerate(zip(lengths.tolist(), counts.tolist())):
+            for p in range(held, held + n):
+                if p % block == 0:
+                    tables[b, p // block] = free[taken]
+                    taken += 1
+                slots.append(int(tables[b, p // block]) * block + p % block)
+                positions.append(p)
+            starts.append(starts[-1] + n)
+        ints = lambda x: torch.tensor(x, dtype=torch.int32)
+        return attention.CacheTables(ints(starts), lengths + counts, ints(slots), ints(positions), ints([taken]))
+    monkeypatch.setattr(attention, "cache_tables", cache_tables)
+    return lambda **more: cache(device="cpu", **more)
+
+
+def test_a_source_stays_while_others_stand_behind_it(host):
+    c = host(max_requests=4)
+    c.step([0], [6])
+    c.share(0, 1)
+    c.share(0, 2)
+    c.step([1], [3])
+    blocks = c.tables[0, :2].tolist()
+    for call in (lambda: c.free(0), lambda: c.trim(0, 1)):
+        with pytest.raises(ValueError, match=r"\[1, 2\] stand behind"):
+            call()
+    assert c.tables[0, :2].tolist() == blocks and c.length(0) == 6
+    c.free(1)
+    with pytest.raises(ValueError, match=r"\[2\] stand behind"):
+        c.free(0)
+    # a request that ended stands behind nobody, whatever it gets next
+    c.step([1], [4])
+    assert c.step([2], [1]).prefix[0].tolist() == blocks
+    c.free(2)
+    c.free(0)
+    c.free(1)
+    assert sorted(c._free.tolist()) == list(range(12))
+
+
+def test_a_source_may_go_on(host):
+    c = host()
+    c.step([0], [6])
+    c.share(0, 1)
+    blocks = c.tables[0, :2].tolist()
+    c.step([0], [7])
+    assert c.step([1], [2]).prefix[0].tolist() == blocks and c.step([1], [1]).prefix[1] == 6
+    c.share(0, 2)
+    with pytest.raises(ValueError, match="one prefix"):       # (13 tokens, not 6)
+        c.step([1, 2], [1, 1])
+    assert c.step([2], [1]).prefix[1] == 13
+
+
+def test_a_request_behind_a_prefix_is_not_trimmed(host):
+    c = host()
+    c.step([0], [6])
+    c.share(0, 1)
+    c.step([1], [12])
+    with pytest.raises(NotImplementedError):
+        c.trim(1, 4)
+    assert -1 not in c.tables[1, :3].tolist()
+
+
+@pytest.mark.gpu
+def test_a_source_that_goes_on_is_not_seen():
+    """(The prefix ends within a block, which the source fills up.)"""
+    c = cache(dim=64, blocks=40, max_context=80)
+    gen = torch.Generator().manual_seed(3)
+    draw = lambda n: torch.randn(2, n, 1, 64, generator=gen).half().cuda()
+    c.write(0, *draw(38), c.step([0], [38]))
+    c.share(0, 1)
+    s = c.step([1], [3])
+    k, v = draw(3)
+    c.write(0, k, v, s)
+    q = torch.randn(3, 1, 64, generator=gen).half().cuda()
+    want = c.attend(0, q, s)
+    k, v = draw(9)
+    c.write(0, torch.full_like(k, float("nan")), torch.full_like(v, float("nan")), c.step([0], [9]))
+    assert bool(want.isfinite().all()) and torch.equal(c.attend(0, q, s), want)

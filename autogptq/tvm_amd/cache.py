@@ -128,13 +128,15 @@ class PagedCache:
             raise NotImplementedError("a sliding window behind a shared prefix")
         self._alone(request)
         first, last = self._blocks(sinks), max(0, self._lengths[request] + 1 - window) // self.block_size
-        first = max(first, self._kept[request][1])
+        start, gone = self._kept[request]
+        if gone > 0 and first > start:
+            raise ValueError(f"request {request} has kept its first {start * self.block_size} tokens only: {sinks} sinks are too many")
+        first = max(first, gone)
         if last <= first:
             return 0
         self._free = torch.cat([self._free, self.tables[request, first:last]])
         self.tables[request, first:last] = -1
-        start = self._kept[request][0] if self._kept[request] != (0, 0) else first
-        self._kept[request] = (start, last)
+        self._kept[request] = (start if gone > 0 else first, last)
         return last - first
 
     def free(self, request: int) -> None:

@@ -181,3 +181,20 @@ def test_a_source_that_goes_on_is_not_seen():
     k, v = draw(9)
     c.write(0, torch.full_like(k, float("nan")), torch.full_like(v, float("nan")), c.step([0], [9]))
     assert bool(want.isfinite().all()) and torch.equal(c.attend(0, q, s), want)
+
+
+def test_a_second_trim_with_other_sinks_loses_no_blocks(host):
+    c = host(blocks=40, max_context=160)
+    c.step([0], [100])
+    assert c.trim(0, window=40, sinks=1) == 14                 # blocks 1 to 14
+    with pytest.raises(ValueError, match="60 sinks are too many"):
+        c.trim(0, window=8, sinks=60)
+    assert c.trim(0, window=8, sinks=4) == 8 and c.trim(0, window=200, sinks=0) == 0
+    c.step([0], [20])
+    assert c.trim(0, window=8, sinks=0) == 5
+    c.free(0)
+    assert sorted(c._free.tolist()) == list(range(40))
+    c.step([1], [100])
+    assert c.trim(1, window=40, sinks=8) == 13 and c.trim(1, window=8, sinks=1) == 8
+    c.free(1)
+    assert sorted(c._free.tolist()) == list(range(40))

@@ -22,6 +22,8 @@ class Step(NamedTuple):
     positions: torch.Tensor   # [tokens], for rotary embeddings and the like
     max_context: int
     prefix: Optional[Tuple[torch.Tensor, int]]     # blocks and length of a prefix that all of them share
+    window: int = 0           # the widest window, and the most sinks, under which the blocks that trim() has given back are not
+    sinks: int = 0            # seen (window 0: none are missing)
 
 
 class PagedCache:
@@ -80,6 +82,8 @@ class PagedCache:
         if len({(self._source[r], p[1]) if p else None for r, p in zip(requests, prefixes)}) > 1:
             raise ValueError("the requests of a step must stand behind one prefix, or all behind none")
         after = [self._lengths[r] + n for r, n in zip(requests, counts)]
+        gaps = [(self._lengths[r] + 1 - self._kept[r][1] * self.block_size, self._kept[r][0] * self.block_size)
+                for r, n in zip(requests, counts) if n and self._kept[r][1]]
         if max(after, default=0) > self.tables.shape[1] * self.block_size:
             raise RuntimeError(f"a request of {max(after)} tokens does not fit the tables")
         need = sum(self._blocks(a) - self._blocks(self._lengths[r]) for r, a in zip(requests, after))
@@ -101,7 +105,7 @@ class PagedCache:
             self._lengths[r] = a
         prefix = prefixes[0] if prefixes else None
         return Step(tables, made.starts, made.contexts, made.slots, made.positions + prefix[1] if prefix else made.positions,
-                    max(after, default=0), prefix)
+                    max(after, default=0), prefix, min((w for w, _ in gaps), default=0), min((k for _, k in gaps), default=0))
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, step: Step) -> None:
         """The step's keys and values [tokens, kv_heads, dim] of a layer."""
@@ -111,6 +115,9 @@ class PagedCache:
                scale: Optional[float] = None) -> torch.Tensor:
         """The attention of the step's queries [tokens, heads, dim] in a layer, after ``write``."""
         k, v = self.k[layer], self.v[layer]
+        if step.window and not (0 < window <= step.window and sinks <= step.sinks):
+            raise ValueError(f"what trim has left of these requests suffices for windows of at most {step.window} tokens and {step.sinks} "
+                             f"sinks, not for window={window}, sinks={sinks}")
         if step.prefix is None:
             return attention.paged_attention(q, k, v, step.tables, step.starts, step.contexts, max_context=step.max_context,
                                              window=window, sinks=sinks, scale=scale)
@@ -121,7 +128,8 @@ class PagedCache:
 
     def trim(self, request: int, window: int, sinks: int = 0) -> int:
         """Gives back the blocks that no later token of a request sees under a window (of at least 1) with sinks; returns how
-        many.  From then on the request is attended to with this window and these sinks, or narrower ones."""
+        many.  From then on the request is attended to with this window and these sinks, or narrower ones (what sees blocks that are
+        gone is refused)."""
         if window < 1:
             raise ValueError("trim needs a window")
         if self._prefixes[request] is not None:

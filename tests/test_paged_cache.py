@@ -198,3 +198,28 @@ def test_a_second_trim_with_other_sinks_loses_no_blocks(host):
     assert c.trim(1, window=40, sinks=8) == 13 and c.trim(1, window=8, sinks=1) == 8
     c.free(1)
     assert sorted(c._free.tolist()) == list(range(40))
+
+
+def test_blocks_that_were_given_back_are_not_read(host, monkeypatch):
+    from autogptq.tvm_amd import attention
+
+    seen = []
+    monkeypatch.setattr(attention, "paged_attention", lambda *args, window, sinks, **more: seen.append((window, sinks)))
+    c = host(blocks=40, max_context=160)
+    q = torch.zeros(1, 1, 8, dtype=torch.float16)
+    c.step([0], [100])
+    c.step([1], [30])
+    assert c.trim(0, window=10, sinks=5) == 20         # blocks 2 to 21: tokens 8 to 87
+    both = c.step([0, 1], [1, 1])                      # (the token at 100 sees from 88 on under a window of 13)
+    for window, sinks in ((0, 0), (14, 5), (10, 9), (0, 5)):
+        with pytest.raises(ValueError, match="at most 13 tokens and 8 sinks"):
+            c.attend(0, q, both, window=window, sinks=sinks)
+    assert not seen
+    for mask in ((13, 8), (10, 5), (1, 0)):
+        c.attend(0, q, both, window=mask[0], sinks=mask[1])
+    # requests with all of their blocks, or without tokens in the step, ask for nothing
+    c.attend(0, q, c.step([1], [1]))
+    c.attend(0, q, c.step([0, 1], [0, 1]))
+    assert seen == [(13, 8), (10, 5), (1, 0), (0, 0), (0, 0)]
+    c.free(0)
+    c.attend(0, q, c.step([0], [1]))

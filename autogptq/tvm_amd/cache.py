@@ -13,7 +13,8 @@ from . import attention
 
 
 class Step(NamedTuple):
-    """One step of some requests: what ``PagedCache.step`` returns and ``write`` and ``attend`` take, for every layer."""
+    """One step of some requests: what ``PagedCache.step`` returns and ``write`` and ``attend`` take, for every layer.  It stays as it is
+    whatever is trimmed or freed between two layers; blocks that were given back hold what they held until a later step's ``write``."""
 
     tables: torch.Tensor      # [requests, width]
     starts: torch.Tensor      # [requests + 1]
@@ -45,6 +46,7 @@ class PagedCache:
         self._source: List[Optional[int]] = [None] * max_requests       # whose prefix that is
         self._kept = [(0, 0)] * max_requests                # blocks [a, b) of a request that trim() has given back
         self._rows = ((), None)                             # the requests of the last step, as a tensor
+        self._handed_out = False                            # whether a Step holds self.tables itself, or a row as its prefix
 
     @property
     def free_blocks(self) -> int:
@@ -67,6 +69,7 @@ class PagedCache:
         n = self._lengths[source]
         if n:
             self._prefixes[request], self._source[request] = (self.tables[source, :self._blocks(n)], n), source
+            self._handed_out = True
 
     def _alone(self, request: int) -> None:
         behind = [r for r, s in enumerate(self._source) if s == request]
@@ -95,6 +98,7 @@ class PagedCache:
         rows = self._rows[1]
         every = requests == tuple(range(self.tables.shape[0]))
         tables = self.tables if every else self.tables[rows]
+        self._handed_out |= every
         made = attention.cache_tables(self._on_gpu[rows], torch.tensor(counts, dtype=torch.int32).to(device, non_blocking=True), tables,
                                       self._free, sum(counts), self.block_size)
         if not every:
@@ -126,6 +130,12 @@ class PagedCache:
         return attention.shared_prefix_attention(q, k, v, step.prefix[0], step.prefix[1], step.tables, step.starts, step.contexts,
                                                  max_context=step.max_context, scale=scale)
 
+    def _forget(self, request: int, first: int, last: Optional[int] = None) -> None:
+        """Takes entries out of a request's table.  (Steps keep theirs; the entries that later steps add lie past their contexts.)"""
+        if self._handed_out:
+            self.tables, self._handed_out = self.tables.clone(), False
+        self.tables[request, first:last] = -1
+
     def trim(self, request: int, window: int, sinks: int = 0) -> int:
         """Gives back the blocks that no later token of a request sees under a window (of at least 1) with sinks; returns how
         many.  From then on the request is attended to with this window and these sinks, or narrower ones (what sees blocks that are
@@ -143,7 +153,7 @@ class PagedCache:
         if last <= first:
             return 0
         self._free = torch.cat([self._free, self.tables[request, first:last]])
-        self.tables[request, first:last] = -1
+        self._forget(request, first, last)
         self._kept[request] = (start if gone > 0 else first, last)
         return last - first
 
@@ -153,7 +163,7 @@ class PagedCache:
         a, b = self._kept[request]
         n = self._blocks(self._lengths[request])
         self._free = torch.cat([self._free, self.tables[request, :a], self.tables[request, b:n]])
-        self.tables[request] = -1
+        self._forget(request, 0)
         self._on_gpu[request] = 0
         self._lengths[request], self._kept[request] = 0, (0, 0)
         self._prefixes[request] = self._source[request] = None

@@ -223,3 +223,53 @@ def test_blocks_that_were_given_back_are_not_read(host, monkeypatch):
     assert seen == [(13, 8), (10, 5), (1, 0), (0, 0), (0, 0)]
     c.free(0)
     c.attend(0, q, c.step([0], [1]))
+
+
+@pytest.mark.parametrize("requests", [[0, 1, 2], [2, 0], [0]])
+def test_a_step_keeps_its_tables(host, requests):
+    c = host(blocks=40, max_context=160)
+    c.step(requests, [30 + r for r in requests])
+    s = c.step(requests, [2] * len(requests))
+    before = s.tables.clone()
+    assert c.trim(0, window=4) > 0
+    assert torch.equal(s.tables, before)
+    c.free(requests[-1])
+    c.free(0)
+    c.step([0], [9])
+    assert torch.equal(s.tables, before)
+    # and the cache's own go on
+    s = c.step([0, 1, 2], [5, 5, 5])
+    assert s.tables[0, :4].tolist() == c.tables[0, :4].tolist() and -1 not in s.tables[0, :4].tolist()
+    used = [e for e in c.tables.flatten().tolist() if e >= 0]
+    assert sorted(used + c._free.tolist()) == list(range(40))
+
+
+def test_a_step_keeps_its_prefix(host):
+    c = host()
+    c.step([0], [6])
+    c.share(0, 1)
+    s = c.step([1], [2])
+    before = s.prefix[0].clone(), s.tables.clone()
+    c.free(1)
+    c.free(0)
+    c.step([0], [20])
+    assert torch.equal(s.prefix[0], before[0]) and torch.equal(s.tables, before[1])
+
+
+@pytest.mark.gpu
+def test_a_trim_between_two_layers():
+    c = cache(layers=2, dim=64, blocks=60, max_context=100, max_requests=1)
+    gen = torch.Generator().manual_seed(5)
+    draw = lambda *shape: torch.randn(*shape, 1, 64, generator=gen).half().cuda()
+    q = draw(40)
+    s = c.step([0], [80])
+    k, v = draw(2, 80)
+    for layer in (0, 1):
+        c.write(layer, k, v, s)
+    s = c.step([0], [20])
+    k, v = draw(2, 20)
+    c.write(0, k, v, s), c.write(1, k, v, s)
+    out = [c.attend(0, q[:20], s, window=16)]
+    assert c.trim(0, window=16) > 0
+    out.append(c.attend(1, q[:20], s, window=16))
+    assert torch.equal(out[0], out[1])

@@ -54,7 +54,13 @@ class PagedCache:
 
     def length(self, request: int) -> int:
         """Tokens of a request in the cache (its own: without those of a shared prefix)."""
+        self._known(request)
         return self._lengths[request]
+
+    def _known(self, *requests: int) -> None:
+        for r in requests:
+            if not 0 <= r < len(self._lengths):
+                raise IndexError(f"request {r} is not a number from 0 to {len(self._lengths) - 1}")
 
     def _blocks(self, tokens: int) -> int:
         return -(-tokens // self.block_size)
@@ -62,6 +68,7 @@ class PagedCache:
     def share(self, source: int, request: int) -> None:
         """``request`` (without tokens so far) stands behind the tokens that ``source`` has now, whose blocks it reads and does
         not own: ``source`` is neither trimmed nor freed while others stand behind it.  (What it gets later they do not see.)"""
+        self._known(source, request)
         if self._lengths[request] or self._prefixes[request] is not None:
             raise ValueError(f"request {request} has tokens already")
         if self._prefixes[source] is not None or self._kept[source] != (0, 0):
@@ -79,6 +86,7 @@ class PagedCache:
     def step(self, requests: Sequence[int], counts: Sequence[int]) -> Step:
         """Makes room for ``counts[i]`` more tokens of ``requests[i]``.  Raises before anything is launched if there is none."""
         requests = tuple(requests)
+        self._known(*requests)
         if len(set(requests)) != len(requests) or len(requests) != len(counts) or min(counts, default=0) < 0:
             raise ValueError("requests must be distinct, with a count of at least 0 each")
         prefixes = [self._prefixes[r] for r in requests]
@@ -140,6 +148,7 @@ class PagedCache:
         """Gives back the blocks that no later token of a request sees under a window (of at least 1) with sinks; returns how
         many.  From then on the request is attended to with this window and these sinks, or narrower ones (what sees blocks that are
         gone is refused)."""
+        self._known(request)
         if window < 1:
             raise ValueError("trim needs a window")
         if self._prefixes[request] is not None:
@@ -159,6 +168,7 @@ class PagedCache:
 
     def free(self, request: int) -> None:
         """Ends a request: its blocks are free again."""
+        self._known(request)
         self._alone(request)
         a, b = self._kept[request]
         n = self._blocks(self._lengths[request])

@@ -273,3 +273,14 @@ def test_a_trim_between_two_layers():
     assert c.trim(0, window=16) > 0
     out.append(c.attend(1, q[:20], s, window=16))
     assert torch.equal(out[0], out[1])
+
+
+def test_requests_that_do_not_exist(host):
+    """(A negative number would name a request by a second name, twice in one step.)"""
+    c = host()
+    c.step([2], [3])
+    for call in (lambda: c.step([-1, 2], [1, 1]), lambda: c.step([3], [1]), lambda: c.free(-1), lambda: c.trim(-1, 4), lambda: c.share(-1, 0),
+                 lambda: c.share(2, -3), lambda: c.length(-1)):
+        with pytest.raises(IndexError, match="0 to 2"):
+            call()
+    assert c.length(2) == 3 and c.free_blocks == 11

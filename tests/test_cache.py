@@ -182,3 +182,33 @@ def test_what_is_written_counts_as_written():
         before = cache._version
         call(k, v, cache[0], cache[1], ints(0, 1, 2))
         assert cache._version > before, call
+
+
+# above 32768 tokens a thread takes four neighbours: sums that leave a remainder, room beyond and below them, requests without tokens,
+# blocks of one and of no power of two, too few free blocks, too narrow tables
+LARGE = [  # as CASES, and every how many requests have none
+    (5, 300, 20000, 16, 0, None, 2, 0), (400, 900, 500, 24, 3, None, 2, 3), (400, 900, 500, 7, -2, None, 2, 2), (3000, 5, 30, 1, 1, None, 2, 5),
+    (9, 100, 15000, 64, -30001, None, 2, 0), (1, 7, 70001, 16, 2, None, 2, 0), (40, 50, 3000, 16, 50000, 1000, 2, 4),
+    (40, 50, 3000, 16, 0, None, -9, 4), (8192, 3, 12, 16, 0, None, 2, 7), (2, 0, 1, 16, 40001, None, 2, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", LARGE, ids=[str(c) for c in LARGE])
+def test_cache_tables_of_many_tokens(case):
+    B, longest, new, block, more, short, room, every = case
+    lengths, counts, tables, free = make(32, B, longest, new, block, short, room)
+    if every:
+        counts[::every] = 0
+    if B == 1:
+        counts[0] = new
+    tokens = int(counts.sum()) + more
+    assert tokens > 32768
+    dev = [t.to(torch.int32).cuda() for t in (lengths, counts, tables, free)]
+    for _ in range(2):
+        torch.full((tokens + 20000,), 77, dtype=torch.int32, device="cuda")      # what the results' memory holds
+        made = attention.cache_tables(*dev, tokens, block)
+    want = loops(lengths.tolist(), counts.tolist(), tables.tolist(), free.tolist(), tokens, block)
+    assert [x.tolist() for x in made] == [list(x) for x in want[1:]]
+    for got, row in zip(dev[2].tolist(), want[0]):
+        assert all(e is None or g == e for g, e in zip(got, row))

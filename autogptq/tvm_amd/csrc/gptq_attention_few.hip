@@ -2,8 +2,8 @@
 //
 // What bounds it: memory.  Every visible key and value is read once (4 dim bytes in all), for 4 dim flops a row, and a tile
 // has 16 RT rows.  So the kernel is a stream: four waves of a workgroup take every fourth block of 32 keys of the part and
-// load keys and values straight into the registers of the matrix instructions, without LDS and without a barrier, the next
-// 32 keys' loads in flight while the present ones are used.
+// load keys and values straight into the registers of the matrix instructions, past LDS and without a barrier, the next
+// 32 keys' loads in flight while the present ones are used.  (LDS holds the places of a wave's rows, and the waves' sums at the end.)
 //
 //   S^T[key, row] = K Q^T   keys are rows of the A operand: lane (i, g) = (lane % 16, lane / 16) loads 16 bytes of key i at
 //                           dims 32 s + 8 g; a result lane holds for its row i the keys 4 g .. 4 g + 3
@@ -16,13 +16,13 @@
 //
 // The division.  Two to four workgroups fill a CU's registers, so a grid with a workgroup for every part that
 // a request might have spends its time on those that find none (16 contexts of up to 32768 tokens: 146 us, with the
-// division below 75).  Instead a head has `team` workgroups, as many as run at once, and each takes the same number of units
+// division below 70).  Instead a head has `team` workgroups, as many as run at once, and each takes the same number of units
 // of up to 256 keys of the requests' tiles, one after the other, in the order of the requests: a workgroup ends one tile, takes
 // whole ones and begins another, and leaves at most two parts.  Every wave finds its place from the requests' lengths by
 // itself, 64 requests at a time.
 //
-// Measured (32 heads in groups of 4, dim 128): 16 contexts of 32768 364 us, 5.9 TB/s of keys and values; 64 of up to 32768 under a
-// window of 4096 72.8 us; one of 512 8.5 us, a chain of reads of about 1 us each (lengths, table, keys, values, parts).
+// Measured (32 heads in groups of 4, dim 128): 16 contexts of 32768 363 us, 5.9 TB/s of keys and values (a plain read of as much: 7.06);
+// 64 of up to 32768 under a window of 4096 72.5 us; one of 512 8.5 us, a chain of reads of about 1 us each (lengths, table, keys, values, parts).
 #include "gptq_attention.h"
 
 namespace gptq {

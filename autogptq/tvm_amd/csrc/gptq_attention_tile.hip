@@ -19,12 +19,13 @@
 //             20 tokens behind 2048 keys, dim 128, 73.6 us against 54.5; 5 of up to 333 behind up to 9001, dim 80, 77.7
 //             against 66.6.)
 //   LDS       rows as they lie in the cache; the 16-byte chunks of row r stand at chunk ^ r (keys) and chunk ^ 2 r (values),
-//             which spreads the lanes of a read over all banks.  The swizzle is in the requests' source addresses.
+//             without which all lanes of a read would stand on the same banks.  Some still do: a third of the cycles of LDS are
+//             conflicts.  The swizzle is in the requests' source addresses.
 //
-// Measured (32 heads in groups of 4, dim 128): a prompt of 8192 tokens 587 us, 937 TFLOP/s; the matrix pipes are busy in half
-// of the cycles, at the 1.7 to 1.9 GHz that the card's power leaves.  Without the exponentials it takes 6 % less, without the
-// requests 18 %, without the reads of values 3 %.  Not better: 64 rows a wave (spills, 1537 us), eight waves a workgroup
-// (the same), a wave's priority raised around its products (fewer cycles, the same time).
+// Measured (32 heads in groups of 4, dim 128): a prompt of 8192 tokens 587 to 613 us on different cards, 897 to 937 TFLOP/s; the matrix
+// pipes are busy in half of the cycles, at 1.8 GHz; a wave waits for data or the barrier 31 % of its time, and 31 % to issue.  Without
+// the exponentials it takes 6 % less, without the requests 18 %, without the reads of values 3 %.  Not better: 64 rows a wave (spills,
+// 1537 us), eight waves a workgroup (the same), a wave's priority raised around its products (fewer cycles, the same time).
 #include <algorithm>
 #include <type_traits>
 
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
                 for (int up = 0; up < 2; up++) vf[x][dt][up] = read_turned<E>(vat[up][dt] + (BUF + 16 * x * DP * 2));
         };
         // (a step of 16 keys ahead, but for the widest rows, which leave no registers for it, and those of 64, where the registers
-        // let a third workgroup into a CU: a prompt of 4096 tokens 122 us, 106 so)
+        // let a third workgroup into a CU: a prompt of 4096 tokens 106 us, 97 so)
         constexpr bool EARLY = DT > 2 && DT <= 6;
         if (EARLY) read_values(0);
         __builtin_amdgcn_sched_barrier(0);
@@ -353,7 +354,9 @@ static void launch_tile(const AttentionParams &p, hipStream_t stream)
 {
     const dim3 grid((unsigned)(p.kv_heads * p.tiles), (unsigned)p.splits);
     // A CU holds three workgroups of rows of 64.  A grid of about two a CU (and the tiles that requests leave empty) would stand three
-    // on some and one on others; LDS for two keeps it even (8 pieces of 256 tokens behind 4096 keys, 576 workgroups: 119 us, 101 so).
+    // on some and one on others; LDS for two keeps it even.  Behind 4096 keys, 32 heads in groups of 4, us with LDS for two and for three: 8
+    // pieces of 128 tokens (640 workgroups, two parts) 62 / 72, of 256 (576) 94 / 114, of 288 (640) 141 / 117, of 320 (704) 155 / 124; 16 of 64
+    // behind 1000 (768, two parts) 39 / 30.  With 8 heads: 8 of 256 (576, four parts) 52 / 43, of 512 (544, two parts) 61 / 71.
     const int least = (long long)p.kv_heads * p.tiles * p.splits <= 640 ? 56 * 1024 : 0;
 #define GPTQ_TILE(DP, DC) \
     hipLaunchKernelGGL((attention_tile_kernel<E, DP, DC>), grid, dim3(256), std::max(4 * kTileKeys * DP * 2 + 8 * kTileKeys * 4, least), stream, p)

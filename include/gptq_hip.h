@@ -414,7 +414,8 @@ int gptq_hip_cache_write(const gptq_hip_cache *cache, const void *k, const void 
  *   max_context: the longest context, as the host knows it: it sets how the work is divided, not what is computed (0: the
  *     tables' width)
  * workspace: gptq_hip_attention_workspace_bytes, zeroed once; every call leaves its counters at zero, so calls on one
- * stream may share it, but no other entry point may write to it.  One to three launches: a longer prefix has one of its own, and so
+ * stream may share it, but no other entry point may write to it.  (A captured call keeps its address: it belongs to that graph then.)
+ * One to three launches: a longer prefix has one of its own, and so
  * has the join of a few tiles of many tokens whose keys were divided.
  */
 typedef struct gptq_hip_attention {

@@ -353,11 +353,13 @@ template <typename E>
 static void launch_tile(const AttentionParams &p, hipStream_t stream)
 {
     const dim3 grid((unsigned)(p.kv_heads * p.tiles), (unsigned)p.splits);
-    // A CU holds three workgroups of rows of 64.  A grid of about two a CU (and the tiles that requests leave empty) would stand three
-    // on some and one on others; LDS for two keeps it even.  Behind 4096 keys, 32 heads in groups of 4, us with LDS for two and for three: 8
-    // pieces of 128 tokens (640 workgroups, two parts) 62 / 72, of 256 (576) 94 / 114, of 288 (640) 141 / 117, of 320 (704) 155 / 124; 16 of 64
-    // behind 1000 (768, two parts) 39 / 30.  With 8 heads: 8 of 256 (576, four parts) 52 / 43, of 512 (544, two parts) 61 / 71.
-    const int least = (long long)p.kv_heads * p.tiles * p.splits <= 640 ? 56 * 1024 : 0;
+    // A CU holds three workgroups of rows of 64.  Where those that have rows are two a CU at most (and not many others run beside them) three
+    // would stand on some and one on others; LDS for two keeps it even.  Behind 4096 keys, 32 heads in groups of 4, us with LDS for two and
+    // for three: 8 pieces of 128 tokens (512 with rows of 640, two parts) 62 / 72, of 256 (512 of 576) 94 / 114, of 288 (576 of 640) 141 / 117,
+    // of 320 (640 of 704) 155 / 124; 16 of 64 behind 1000 (512 of 768, two parts) 39 / 30.  With 8 heads: 8 of 512 (512 of 544, two
+    // parts) 61 / 71, of 288 (576 of 640) 54 / 45; on the wrong side 8 of 256 (512 of 576, four parts) 52 / 43.
+    const long long groups = (long long)p.kv_heads * p.splits, full = ((long long)p.tokens * p.group + kTileRows - 1) / kTileRows;
+    const int least = groups * full <= 512 && groups * p.tiles <= 640 ? 56 * 1024 : 0;
 #define GPTQ_TILE(DP, DC) \
     hipLaunchKernelGGL((attention_tile_kernel<E, DP, DC>), grid, dim3(256), std::max(4 * kTileKeys * DP * 2 + 8 * kTileKeys * 4, least), stream, p)
     if (p.dim <= 64) GPTQ_TILE(64, 64);

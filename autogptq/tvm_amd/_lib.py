@@ -51,6 +51,9 @@ ABI_SYMBOLS = (
     "gptq_hip_dequant",
     "gptq_hip_cache_tables",
     "gptq_hip_cache_write",
+    "gptq_hip_cache_read",
+    "gptq_hip_cache_write_mx",
+    "gptq_hip_cache_read_mx",
     "gptq_hip_attention_workspace_bytes",
     "gptq_hip_attend",
     "gptq_hip_probe",
@@ -110,6 +113,15 @@ class Cache(ctypes.Structure):
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + [
         (name, ctypes.c_int) for name in ("type", "blocks", "block_size", "heads", "dim")] + [
         (name, ctypes.c_longlong) for name in ("block_stride", "slot_stride", "head_stride")]
+
+
+class CacheMx(ctypes.Structure):
+    """Mirror of ``gptq_hip_cache_mx``."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("k", "v", "k_scales", "v_scales")] + [
+        (name, ctypes.c_int) for name in ("type", "blocks", "block_size", "heads", "dim")] + [
+        (name, ctypes.c_longlong) for name in ("block_stride", "slot_stride", "head_stride", "scale_block_stride", "scale_slot_stride",
+                                               "scale_head_stride")]
 
 
 class Attention(ctypes.Structure):
@@ -216,6 +228,12 @@ def lib() -> ctypes.CDLL:
     l.gptq_hip_cache_tables.argtypes = [vp, vp, vp, ll, i, vp, i, i, i, i, vp, vp, vp, vp, vp, vp]
     l.gptq_hip_cache_write.restype = i
     l.gptq_hip_cache_write.argtypes = [ctypes.POINTER(Cache), vp, vp, ll, ll, ll, ll, vp, i, vp]
+    l.gptq_hip_cache_read.restype = i
+    l.gptq_hip_cache_read.argtypes = [ctypes.POINTER(Cache), vp, i, vp, vp, vp]
+    l.gptq_hip_cache_write_mx.restype = i
+    l.gptq_hip_cache_write_mx.argtypes = [ctypes.POINTER(CacheMx), vp, vp, ll, ll, ll, ll, vp, i, vp]
+    l.gptq_hip_cache_read_mx.restype = i
+    l.gptq_hip_cache_read_mx.argtypes = [ctypes.POINTER(CacheMx), vp, i, vp, vp, vp]
     l.gptq_hip_attention_workspace_bytes.restype = sz
     l.gptq_hip_attention_workspace_bytes.argtypes = [ctypes.POINTER(Attention)]
     l.gptq_hip_attend.restype = i

@@ -5,8 +5,8 @@ import hashlib
 import os
 
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
-SOURCES = ["gptq_stream.hip", "gptq_grouped.hip", "gptq_dequant.hip", "gptq_static.hip", "gptq_probe.hip", "gptq_tiled.hip", "gptq_tiled_decode.hip", "gptq_tiled_decode16.hip", "gptq_panel.hip", "gptq_cache.hip", "gptq_attention_few.hip", "gptq_attention_tile.hip", "gptq_attention_plan.cpp", "gptq_dispatch.cpp", "gptq_capi.cpp"]
-HEADERS = ["gptq_unpack.h", "gptq_internal.h", "gptq_device.h", "gptq_tiled_common.h", "gptq_attention.h", os.path.join("..", "..", "..", "include", "gptq_hip.h"),
+SOURCES = ["gptq_stream.hip", "gptq_grouped.hip", "gptq_dequant.hip", "gptq_static.hip", "gptq_probe.hip", "gptq_tiled.hip", "gptq_tiled_decode.hip", "gptq_tiled_decode16.hip", "gptq_panel.hip", "gptq_cache.hip", "gptq_cache_mx.hip", "gptq_attention_few.hip", "gptq_attention_tile.hip", "gptq_attention_plan.cpp", "gptq_dispatch.cpp", "gptq_capi.cpp"]
+HEADERS = ["gptq_unpack.h", "gptq_internal.h", "gptq_device.h", "gptq_tiled_common.h", "gptq_attention.h", "gptq_mx.h", os.path.join("..", "..", "..", "include", "gptq_hip.h"),
            "binding.cpp", "binding.h", "binding_attention.cpp", "python_call.cpp"]   # (hashed with the rest: both libraries carry one build id)
 # Compiler options of single sources.  The decode kernels keep the four result registers of their small matrix
 # instructions in ordinary vector registers: left to itself the compiler puts them into accumulation registers

@@ -5,6 +5,7 @@ layers are replaced); here a serving step finds what stands between q/k/v and o 
 
 * ``cache_tables``             block tables, slot maps, query offsets and positions of a step, from the requests' lengths
 * ``cache_write``              the step's keys and values into their slots
+* ``cache_read``               the rows of slots back
 * ``paged_attention``          causal attention over the requests' blocks: prompts, pieces of prompts and single tokens, mixed
                                as they come, with or without a sliding window and first tokens that stay visible (sinks)
 * ``shared_prefix_attention``  the same for requests behind one long prefix, which is read once for all of them
@@ -13,14 +14,42 @@ All run on the current stream of the tensors' device, have no backward, and exis
 captured by ``torch.cuda.graph``: a capture gets a workspace of its own from the graph's memory, whatever runs before or after it
 (the graph clears its counters, one small launch a replay); what the kernels need loaded, a call on any stream before it loads.  Caches are float16 or bfloat16
 [blocks, block_size, kv_heads, dim] in any order of memory whose last dimension is contiguous; dim is a multiple of 8 up to 256.
+
+A cache may also be held in MXFP4, 4.25 bits a value: pass an ``Mxfp4`` (see there, and ``mxfp4_cache``) wherever a cache is asked for; the
+write quantises, the attention reads the codes.  The operators of these are ``torch.ops.gptq_hip.<name>_mx``, with codes and scales as
+two arguments each.
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
 from . import ops
+
+
+class Mxfp4(NamedTuple):
+    """Keys or values of a cache in MXFP4, the microscaling format with 4-bit floats.  A head's ``dim`` values of a token, padded to
+    a multiple of 32, are groups of 32 codes and a power of two 2^e each; a code is a sign and one of 0, 1/2, 1, 3/2, 2, 3, 4, 6.
+    A write takes the e that puts a group's largest magnitude into [3.5, 7) 2^e and the nearest codes, ties to the even one (a group of
+    float16 values has e within -23 .. 13, of bfloat16 -125 .. 125: what it stands for is a value of the type, and what lies beyond 6 2^e
+    becomes that).  A group with an infinity or a NaN stands for NaN.  A cache is read in the type it was written in."""
+
+    codes: torch.Tensor       # uint8 [blocks, block_size, kv_heads, 16 ceil(dim / 32)]: value 2 j in the low half of byte j
+    scales: torch.Tensor      # uint8 [blocks, block_size, kv_heads, 2 (dim up to 64), 4 (up to 128) or 8]: e + 127; 255: NaN
+
+
+Cache = Union[torch.Tensor, Mxfp4]
+
+
+def mxfp4_cache(blocks: int, block_size: int, kv_heads: int, dim: int, device="cuda:0") -> Tuple[Mxfp4, Mxfp4]:
+    """Keys and values of a cache in MXFP4, unwritten.  (A block's rows of a head lie together: whole lines for the kernels that read one
+    head.)"""
+    if dim < 8 or dim % 8 or dim > 256:
+        raise ValueError(f"dim must be a multiple of 8 up to 256, got {dim}")
+    codes, scales = (torch.empty((2, blocks, kv_heads, block_size, n), dtype=torch.uint8, device=device).transpose(2, 3)
+                     for n in (-(-dim // 32) * 16, 2 if dim <= 64 else 4 if dim <= 128 else 8))
+    return Mxfp4(codes[0], scales[0]), Mxfp4(codes[1], scales[1])
 
 
 class CacheTables(NamedTuple):
@@ -42,10 +71,25 @@ def cache_tables(lengths: torch.Tensor, counts: torch.Tensor, tables: torch.Tens
     return CacheTables(*_call("cache_tables", lengths, counts, tables, free_blocks, tokens, block_size))
 
 
-def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor) -> None:
+def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: Cache, v_cache: Cache, slots: torch.Tensor) -> None:
     """``k`` and ``v`` [tokens, kv_heads, dim] (columns of a fused product as they are) into ``slots`` of the cache; tokens
-    with slot -1 are skipped."""
-    _call("cache_write", k, v, k_cache, v_cache, slots)
+    with slot -1 are skipped.  Slots are distinct (one that is named twice is left with parts of both tokens)."""
+    if _packed(k_cache, v_cache):
+        _call("cache_write_mx", k, v, *k_cache, *v_cache, slots)
+    else:
+        _call("cache_write", k, v, k_cache, v_cache, slots)
+
+
+def cache_read(k_cache: Cache, v_cache: Cache, slots: torch.Tensor, dim: Optional[int] = None,
+               dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) [tokens, kv_heads, dim]: the rows of ``slots`` (int32), zeros for slots that the cache does not have (-1).  ``dim`` and
+    ``dtype`` say what an ``Mxfp4`` cache was written with (default: all of its groups, float16); other caches know both."""
+    if _packed(k_cache, v_cache):
+        dim = 2 * k_cache.codes.shape[-1] if dim is None else dim
+        return _call("cache_read_mx", *k_cache, *v_cache, slots, dim, dtype or torch.float16)
+    if dim not in (None, k_cache.shape[-1]) or dtype not in (None, k_cache.dtype):
+        raise ValueError(f"the cache holds rows of {k_cache.shape[-1]} in {k_cache.dtype}, not of {dim} in {dtype}")
+    return _call("cache_read", k_cache, v_cache, slots)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, tables: torch.Tensor, starts: torch.Tensor,
@@ -80,6 +124,13 @@ def _scale(scale: Optional[float]) -> float:
     return scale
 
 
+def _packed(k_cache: Cache, v_cache: Cache) -> bool:
+    packed = isinstance(k_cache, Mxfp4)
+    if packed != isinstance(v_cache, Mxfp4):
+        raise TypeError("k_cache and v_cache must both be tensors or both be Mxfp4")
+    return packed
+
+
 def _call(name: str, *args):
     """The operator by its C function (csrc/python_call.cpp), or by torch.ops where that leaves it to the dispatcher."""
     if not ops.NATIVE_OPS:
@@ -92,4 +143,4 @@ def _call(name: str, *args):
     return getattr(torch.ops.gptq_hip, name)(*args)
 
 
-__all__ = ["CacheTables", "cache_tables", "cache_write", "paged_attention", "shared_prefix_attention"]
+__all__ = ["CacheTables", "Mxfp4", "cache_read", "cache_tables", "cache_write", "mxfp4_cache", "paged_attention", "shared_prefix_attention"]

@@ -82,6 +82,11 @@ void check_bound(const Bound &q);
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> cache_tables(const Tensor &lengths, const Tensor &counts, const Tensor &tables,
                                                                 const Tensor &free_blocks, int64_t tokens, int64_t block_size);
 void cache_write(const Tensor &k, const Tensor &v, const Tensor &k_cache, const Tensor &v_cache, const Tensor &slots);
+std::tuple<Tensor, Tensor> cache_read(const Tensor &k_cache, const Tensor &v_cache, const Tensor &slots);
+void cache_write_mx(const Tensor &k, const Tensor &v, const Tensor &k_codes, const Tensor &k_scales, const Tensor &v_codes, const Tensor &v_scales,
+                    const Tensor &slots);
+std::tuple<Tensor, Tensor> cache_read_mx(const Tensor &k_codes, const Tensor &k_scales, const Tensor &v_codes, const Tensor &v_scales,
+                                         const Tensor &slots, int64_t dim, at::ScalarType dtype);
 Tensor paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &tables, const Tensor &starts,
                        const Tensor &contexts, int64_t max_context, int64_t window, int64_t sinks, double scale);
 Tensor shared_prefix_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &prefix_blocks,

@@ -1,4 +1,5 @@
-// torch.ops.gptq_hip.{cache_tables, cache_write, paged_attention, shared_prefix_attention}: the serving entry points of
+// torch.ops.gptq_hip.{cache_tables, cache_write, cache_read, paged_attention, shared_prefix_attention} and the same of a cache held in
+// MXFP4 (..._mx): the serving entry points of
 // libgptq_hip.so as dispatcher-visible operators (see binding.cpp for the products).  They check devices, dtypes, shapes and
 // strides, allocate what they return, and launch on the current HIP stream of the tensors' device.
 #include <ATen/ATen.h>
@@ -7,6 +8,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
 
+#include <array>
 #include <cmath>
 #include <tuple>
 
@@ -79,6 +81,42 @@ gptq_hip_cache describe(const Tensor &k, const Tensor &v)
     c.type = k.scalar_type() == at::kHalf ? GPTQ_HIP_TYPE_FP16 : GPTQ_HIP_TYPE_BF16;
     c.blocks = (int)k.size(0), c.block_size = (int)k.size(1), c.heads = (int)k.size(2), c.dim = (int)k.size(3);
     c.block_stride = block, c.slot_stride = slot, c.head_stride = head;
+    return c;
+}
+
+// bytes [blocks, block_size, heads, n] whose rows lie side by side; the steps of its first three dimensions
+std::array<int64_t, 3> rows_of(const Tensor &t, const char *name, int64_t n, int64_t unit)
+{
+    TORCH_CHECK(t.scalar_type() == at::kByte, name, " must be uint8, got ", t.scalar_type());
+    TORCH_CHECK(t.dim() == 4 && t.size(3) == n, name, " must be [blocks, block_size, heads, ", n, "], got ", t.sizes());
+    TORCH_CHECK(t.numel() > 0, "the cache is empty");
+    const std::array<int64_t, 3> steps = {step(t, 0), step(t, 1), step(t, 2)};
+    TORCH_CHECK(t.stride(3) == 1 && steps[0] % unit == 0 && steps[1] % unit == 0 && steps[2] % unit == 0 && (uintptr_t)t.data_ptr() % unit == 0,
+                "the rows of ", name, " must be contiguous and ", unit, "-byte aligned (strides ", t.strides(), ")");
+    return steps;
+}
+
+gptq_hip_cache_mx describe_mx(const Tensor &k, const Tensor &k_scales, const Tensor &v, const Tensor &v_scales, int64_t dim, at::ScalarType type)
+{
+    on_gpu(v, "v_codes", k);
+    on_gpu(k_scales, "k_scales", k);
+    on_gpu(v_scales, "v_scales", k);
+    TORCH_CHECK(type == at::kHalf || type == at::kBFloat16, "an MXFP4 cache holds float16 or bfloat16 values, not ", type);
+    TORCH_CHECK(dim >= 8 && dim % 8 == 0 && dim <= 256, "dim must be a multiple of 8 up to 256, got ", dim);
+    const int64_t row = (dim + 31) / 32 * 16, scales = dim <= 64 ? 2 : dim <= 128 ? 4 : 8;
+    const auto at = rows_of(k, "k_codes", row, 16), scale_at = rows_of(k_scales, "k_scales", scales, scales);
+    TORCH_CHECK(rows_of(v, "v_codes", row, 16) == at && rows_of(v_scales, "v_scales", scales, scales) == scale_at && v.sizes() == k.sizes() &&
+                    v_scales.sizes() == k_scales.sizes(), "keys and values must have the same shapes and strides");
+    for (int d = 0; d < 3; d++)
+        TORCH_CHECK(k.size(d) == k_scales.size(d), "codes and scales must be of the same rows, got ", k.sizes(), " and ", k_scales.sizes());
+    TORCH_CHECK(k.size(0) < (1LL << 31) && k.size(1) < (1LL << 31) && k.size(0) * k.size(1) < (1LL << 31) && k.size(2) < (1LL << 31),
+                "the cache has too many slots");
+    gptq_hip_cache_mx c;
+    c.k = k.data_ptr(), c.v = v.data_ptr(), c.k_scales = k_scales.data_ptr(), c.v_scales = v_scales.data_ptr();
+    c.type = type == at::kHalf ? GPTQ_HIP_TYPE_FP16 : GPTQ_HIP_TYPE_BF16;
+    c.blocks = (int)k.size(0), c.block_size = (int)k.size(1), c.heads = (int)k.size(2), c.dim = (int)dim;
+    c.block_stride = at[0], c.slot_stride = at[1], c.head_stride = at[2];
+    c.scale_block_stride = scale_at[0], c.scale_slot_stride = scale_at[1], c.scale_head_stride = scale_at[2];
     return c;
 }
 
@@ -169,6 +207,62 @@ void gptq_torch::cache_write(const Tensor &k, const Tensor &v, const Tensor &k_c
     written(v_cache);
 }
 
+void gptq_torch::cache_write_mx(const Tensor &k, const Tensor &v, const Tensor &k_codes, const Tensor &k_scales, const Tensor &v_codes,
+                                const Tensor &v_scales, const Tensor &slots)
+{
+    on_gpu(k_codes, "k_codes", k_codes);
+    TORCH_CHECK(k.dim() == 3, "k must be [tokens, heads, dim], got ", k.sizes());
+    const gptq_hip_cache_mx c = describe_mx(k_codes, k_scales, v_codes, v_scales, k.size(2), k.scalar_type());
+    for (const Tensor *t : {&k, &v}) {
+        const char *name = t == &k ? "k" : "v";
+        on_gpu(*t, name, k_codes);
+        no_grad(*t, name);
+        TORCH_CHECK(t->scalar_type() == k.scalar_type(), name, " is ", t->scalar_type(), ", k ", k.scalar_type());
+        TORCH_CHECK(t->dim() == 3 && t->size(1) == c.heads && t->size(2) == c.dim, name, " must be [tokens, ", c.heads, ", ", c.dim,
+                    "], got ", t->sizes());
+        TORCH_CHECK(t->size(0) < (1LL << 31), "too many tokens");
+    }
+    need_ints(slots, "slots", k.size(0), k_codes);
+    TORCH_CHECK(v.size(0) == k.size(0), "k has ", k.size(0), " tokens, v ", v.size(0));
+    if (k.size(0) == 0) return;
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(k_codes.device());
+    const Tensor ks = loadable(k), vs = loadable(v);
+    raised(gptq_hip_cache_write_mx(&c, ks.data_ptr(), vs.data_ptr(), step(ks, 0), step(ks, 1), step(vs, 0), step(vs, 1),
+                                   (const int32_t *)slots.data_ptr(), (int)k.size(0), current_stream(k_codes)),
+           "gptq_hip_cache_write_mx");
+    for (const Tensor *t : {&k_codes, &k_scales, &v_codes, &v_scales}) written(*t);
+}
+
+std::tuple<Tensor, Tensor> gptq_torch::cache_read(const Tensor &k_cache, const Tensor &v_cache, const Tensor &slots)
+{
+    on_gpu(k_cache, "k_cache", k_cache);
+    const gptq_hip_cache c = describe(k_cache, v_cache);
+    no_grad(k_cache, "k_cache");
+    no_grad(v_cache, "v_cache");
+    need_ints(slots, "slots", -1, k_cache);
+    TORCH_CHECK(slots.size(0) < (1LL << 31), "too many tokens");
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+    Tensor k = fresh({slots.size(0), c.heads, c.dim}, k_cache), v = fresh(k.sizes(), k_cache);
+    raised(gptq_hip_cache_read(&c, (const int32_t *)slots.data_ptr(), (int)slots.size(0), k.data_ptr(), v.data_ptr(), current_stream(k_cache)),
+           "gptq_hip_cache_read");
+    return {k, v};
+}
+
+std::tuple<Tensor, Tensor> gptq_torch::cache_read_mx(const Tensor &k_codes, const Tensor &k_scales, const Tensor &v_codes, const Tensor &v_scales,
+                                                     const Tensor &slots, int64_t dim, at::ScalarType dtype)
+{
+    on_gpu(k_codes, "k_codes", k_codes);
+    const gptq_hip_cache_mx c = describe_mx(k_codes, k_scales, v_codes, v_scales, dim, dtype);
+    need_ints(slots, "slots", -1, k_codes);
+    TORCH_CHECK(slots.size(0) < (1LL << 31), "too many tokens");
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(k_codes.device());
+    Tensor k = at::detail::empty_cuda({slots.size(0), c.heads, dim}, dtype, k_codes.device(), std::nullopt);
+    Tensor v = at::detail::empty_cuda(k.sizes(), dtype, k_codes.device(), std::nullopt);
+    raised(gptq_hip_cache_read_mx(&c, (const int32_t *)slots.data_ptr(), (int)slots.size(0), k.data_ptr(), v.data_ptr(), current_stream(k_codes)),
+           "gptq_hip_cache_read_mx");
+    return {k, v};
+}
+
 static Tensor attend(const char *what, const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &prefix_blocks,
               int64_t prefix_length, const Tensor &tables, const Tensor &starts, const Tensor &contexts, int64_t max_context,
               int64_t window, int64_t sinks, double scale)
@@ -238,6 +332,11 @@ TORCH_LIBRARY_FRAGMENT(gptq_hip, m)
     m.def("cache_tables(Tensor lengths, Tensor counts, Tensor(a!) tables, Tensor free_blocks, int tokens, int block_size) -> "
           "(Tensor, Tensor, Tensor, Tensor, Tensor)");
     m.def("cache_write(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots) -> ()");
+    m.def("cache_read(Tensor k_cache, Tensor v_cache, Tensor slots) -> (Tensor, Tensor)");
+    m.def("cache_write_mx(Tensor k, Tensor v, Tensor(a!) k_codes, Tensor(b!) k_scales, Tensor(c!) v_codes, Tensor(d!) v_scales, "
+          "Tensor slots) -> ()");
+    m.def("cache_read_mx(Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, Tensor slots, int dim, ScalarType dtype) -> "
+          "(Tensor, Tensor)");
     m.def("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor tables, Tensor starts, Tensor contexts, "
           "int max_context, int window, int sinks, float scale) -> Tensor");
     m.def("shared_prefix_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor prefix_blocks, int prefix_length, "
@@ -249,6 +348,9 @@ TORCH_LIBRARY_IMPL(gptq_hip, CUDA, m)
 {
     m.impl("cache_tables", &cache_tables);
     m.impl("cache_write", &cache_write);
+    m.impl("cache_read", &cache_read);
+    m.impl("cache_write_mx", &cache_write_mx);
+    m.impl("cache_read_mx", &cache_read_mx);
     m.impl("paged_attention", &paged_attention);
     m.impl("shared_prefix_attention", &shared_prefix_attention);
 }
@@ -257,6 +359,9 @@ TORCH_LIBRARY_IMPL(gptq_hip, CPU, m)
 {
     m.impl("cache_tables", &cache_tables);
     m.impl("cache_write", &cache_write);
+    m.impl("cache_read", &cache_read);
+    m.impl("cache_write_mx", &cache_write_mx);
+    m.impl("cache_read_mx", &cache_read_mx);
     m.impl("paged_attention", &paged_attention);
     m.impl("shared_prefix_attention", &shared_prefix_attention);
 }

@@ -1,8 +1,10 @@
 // The host side of the attention over a paged cache: argument checks, the choice between the two kernels, and how a call is
 // divided among workgroups.
 #include <algorithm>
+#include <array>
 
 #include "gptq_attention.h"
+#include "gptq_mx.h"
 
 namespace gptq {
 
@@ -18,6 +20,25 @@ int check_cache(const gptq_hip_cache *c)
     const unsigned __int128 rows = (unsigned __int128)(c->blocks - 1) * (unsigned long long)c->block_stride +
                                    (unsigned __int128)(c->block_size - 1) * (unsigned long long)c->slot_stride;
     if (rows / 8 >= 1ull << 32) return GPTQ_HIP_ERR_UNSUPPORTED;
+    return GPTQ_HIP_OK;
+}
+
+int check_cache_mx(const gptq_hip_cache_mx *c)
+{
+    if (!c || !c->k || !c->v || !c->k_scales || !c->v_scales || ((uintptr_t)c->k | (uintptr_t)c->v) % 16 != 0) return GPTQ_HIP_ERR_BAD_ARG;
+    if (c->type != GPTQ_HIP_TYPE_FP16 && c->type != GPTQ_HIP_TYPE_BF16) return GPTQ_HIP_ERR_BAD_ARG;
+    if (c->blocks < 1 || c->block_size < 1 || c->heads < 1 || c->dim < 8 || c->dim % 8 != 0) return GPTQ_HIP_ERR_BAD_ARG;
+    if (c->dim > 256 || (long long)c->blocks * c->block_size >= 1ll << 31) return GPTQ_HIP_ERR_UNSUPPORTED;
+    const long long scale = mx_scale_bytes(c->dim);
+    if (((uintptr_t)c->k_scales | (uintptr_t)c->v_scales) % scale != 0) return GPTQ_HIP_ERR_BAD_ARG;
+    for (const auto &[unit, block, slot, head] : {std::array{16ll, c->block_stride, c->slot_stride, c->head_stride},
+                                                  std::array{scale, c->scale_block_stride, c->scale_slot_stride, c->scale_head_stride}}) {
+        if (block < 0 || slot < 0 || head < 0 || (block | slot | head) % unit != 0) return GPTQ_HIP_ERR_BAD_ARG;
+        // the places of rows are 32-bit numbers of units
+        const unsigned __int128 rows = (unsigned __int128)(c->blocks - 1) * (unsigned long long)block +
+                                       (unsigned __int128)(c->block_size - 1) * (unsigned long long)slot;
+        if (rows / unit >= 1ull << 32) return GPTQ_HIP_ERR_UNSUPPORTED;
+    }
     return GPTQ_HIP_OK;
 }
 

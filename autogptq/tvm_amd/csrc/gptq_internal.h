@@ -358,5 +358,6 @@ int launch_tiled(const void *x, const void *qtile, const uint32_t *sz, const int
 
 // the cache's shape and strides are ones the cache kernels take (gptq_attention_plan.cpp)
 int check_cache(const gptq_hip_cache *cache);
+int check_cache_mx(const gptq_hip_cache_mx *cache);
 
 }  // namespace gptq

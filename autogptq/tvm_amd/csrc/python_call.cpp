@@ -17,6 +17,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -365,6 +366,65 @@ PyObject *call_cache_write(PyObject *, PyObject *const *args, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
+PyObject *call_cache_write_mx(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    Arguments a(args, n, 7);
+    const Tensor &k = a.tensor(0), &v = a.tensor(1), &kc = a.tensor(2), &ks = a.tensor(3), &vc = a.tensor(4), &vs = a.tensor(5), &slots = a.tensor(6);
+    if (!a.plain) Py_RETURN_NOTIMPLEMENTED;
+    {
+        const WithoutInterpreter free;
+        cache_write_mx(k, v, kc, ks, vc, vs, slots);
+    }
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *two_tensors(std::tuple<Tensor, Tensor> &&made)
+{
+    THPObjectPtr result(PyTuple_New(2));
+    if (!result) return nullptr;
+    for (int i = 0; i < 2; i++) {
+        PyObject *t = THPVariable_Wrap(std::move(i ? std::get<1>(made) : std::get<0>(made)));
+        if (!t) return nullptr;
+        PyTuple_SET_ITEM(result.get(), i, t);
+    }
+    return result.release();
+}
+
+PyObject *call_cache_read(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    Arguments a(args, n, 3);
+    const Tensor &k = a.tensor(0), &v = a.tensor(1), &slots = a.tensor(2);
+    if (!a.plain) Py_RETURN_NOTIMPLEMENTED;
+    std::tuple<Tensor, Tensor> out;
+    {
+        const WithoutInterpreter free;
+        out = cache_read(k, v, slots);
+    }
+    return two_tensors(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *call_cache_read_mx(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    Arguments a(args, n, 7);
+    const Tensor &kc = a.tensor(0), &ks = a.tensor(1), &vc = a.tensor(2), &vs = a.tensor(3), &slots = a.tensor(4);
+    const int64_t dim = a.integer(5);
+    TORCH_CHECK_TYPE(THPDtype_Check(args[6]), "argument 6 must be a dtype");
+    const at::ScalarType dtype = ((THPDtype *)args[6])->scalar_type;
+    if (!a.plain) Py_RETURN_NOTIMPLEMENTED;
+    std::tuple<Tensor, Tensor> out;
+    {
+        const WithoutInterpreter free;
+        out = cache_read_mx(kc, ks, vc, vs, slots, dim, dtype);
+    }
+    return two_tensors(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject *call_paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
@@ -401,7 +461,8 @@ PyObject *call_shared_prefix_attention(PyObject *, PyObject *const *args, Py_ssi
 }
 
 #define GPTQ_FAST(NAME) {#NAME, (PyCFunction)(void (*)(void))call_##NAME, METH_FASTCALL, "torch.ops.gptq_hip." #NAME " on plain tensors, else NotImplemented."}
-PyMethodDef functions[] = {GPTQ_FAST(cache_tables), GPTQ_FAST(cache_write), GPTQ_FAST(paged_attention), GPTQ_FAST(shared_prefix_attention),
+PyMethodDef functions[] = {GPTQ_FAST(cache_tables), GPTQ_FAST(cache_write), GPTQ_FAST(cache_read), GPTQ_FAST(cache_write_mx), GPTQ_FAST(cache_read_mx),
+                           GPTQ_FAST(paged_attention), GPTQ_FAST(shared_prefix_attention),
                            {"capture", capture, METH_O, "capture(stream): 0, or a number of the graph capture that the stream is in."},
                            {"aside", aside, METH_VARARGS, "aside(fn, *args): fn(*args), hidden from tracing and dispatch modes."},
                            {"install", install, METH_O, "Makes the call in C the one of a QuantLinear class."}, {nullptr, nullptr, 0, nullptr}};

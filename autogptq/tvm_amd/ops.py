@@ -419,6 +419,14 @@ def _meta_cache_tables(lengths, counts, tables, free_blocks, tokens, block_size)
     return tuple(lengths.new_empty(n) for n in (B + 1, B, tokens, tokens, 1))
 
 
+def _meta_rows(cache, slots):
+    return cache.new_empty((slots.shape[0], *cache.shape[2:]))
+
+
+def _meta_cache_read_mx(k_codes, k_scales, v_codes, v_scales, slots, dim, dtype):
+    return tuple(k_codes.new_empty((slots.shape[0], k_codes.shape[2], dim), dtype=dtype) for _ in range(2))
+
+
 # The module call in C (csrc/python_call.cpp, an extension module in the operator library): BoundCall and install();
 # None without the built library.
 CALL = None
@@ -485,6 +493,9 @@ def _register_torch_ops():
     if native:      # (the operators of attention.py have no Python form)
         meta.impl("cache_tables", _meta_cache_tables)
         meta.impl("cache_write", lambda k, v, k_cache, v_cache, slots: None)
+        meta.impl("cache_read", lambda k_cache, v_cache, slots: (_meta_rows(k_cache, slots), _meta_rows(v_cache, slots)))
+        meta.impl("cache_write_mx", lambda *args: None)
+        meta.impl("cache_read_mx", _meta_cache_read_mx)
         meta.impl("paged_attention", lambda q, *args: q.new_empty(q.shape))
         meta.impl("shared_prefix_attention", lambda q, *args: q.new_empty(q.shape))
     keep.append(meta)

@@ -394,6 +394,35 @@ int gptq_hip_cache_write(const gptq_hip_cache *cache, const void *k, const void 
                          long long k_head_stride, long long v_token_stride, long long v_head_stride,
                          const int32_t *slots, int tokens, void *stream);
 
+/* The rows of slots back, [tokens, heads, dim] in the cache's type, 16-byte aligned; zeros for slots below 0 or outside of the cache. */
+int gptq_hip_cache_read(const gptq_hip_cache *cache, const int32_t *slots, int tokens, void *k, void *v, void *stream);
+
+/*
+ * The same cache held in 4.25 bits (MXFP4).  A head's dim values of a token, padded with zeros to a multiple of 32, are groups of 32: each
+ * has a power of two 2^e, kept as the byte e + 127, and 32 codes of a sign and one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (value 2 j in the
+ * low half of byte j, 2 j + 1 in the high one).  A row of codes has 16 ceil(dim / 32) bytes; a row of scales has 2 bytes up to
+ * dim 64, 4 up to 128, 8 above, of which the first ceil(dim / 32) count.  A write takes the e that puts the group's largest magnitude m
+ * into [3.5, 7) 2^e, kept within -23 .. 13 (fp16) or -125 .. 125 (bf16), and the nearest codes, ties to the even one; larger
+ * values become 6 2^e.  A group with an infinity or a NaN gets the scale byte 255 and stands for NaN.
+ * Every value of a group is a value of the type it was written from.  `type` is that of keys, values, queries and results; a cache is
+ * read in the type it was written in (in fp16, scales that a bf16 write chose may overflow to infinities, and small ones to zeros).
+ * Strides are in bytes: of codes multiples of 16, of scales multiples of a scale row's size; k and v are 16-byte aligned and share
+ * shape and strides, so do their scales, which are aligned to a scale row's size.
+ */
+typedef struct gptq_hip_cache_mx {
+    void *k, *v, *k_scales, *v_scales;
+    int type;                 /* GPTQ_HIP_TYPE_* */
+    int blocks, block_size, heads, dim;
+    long long block_stride, slot_stride, head_stride, scale_block_stride, scale_slot_stride, scale_head_stride;
+} gptq_hip_cache_mx;
+
+/* As gptq_hip_cache_write and gptq_hip_cache_read.  Slots to be written are distinct: one that is named twice is left with parts of
+ * both tokens. */
+int gptq_hip_cache_write_mx(const gptq_hip_cache_mx *cache, const void *k, const void *v, long long k_token_stride,
+                            long long k_head_stride, long long v_token_stride, long long v_head_stride,
+                            const int32_t *slots, int tokens, void *stream);
+int gptq_hip_cache_read_mx(const gptq_hip_cache_mx *cache, const int32_t *slots, int tokens, void *k, void *v, void *stream);
+
 /*
  * Causal attention of a step's tokens over their requests' blocks.  starts and contexts as gptq_hip_cache_tables gives
  * them: request b has the tokens starts[b] .. starts[b + 1] - 1, the last of them at position contexts[b] - 1, and the

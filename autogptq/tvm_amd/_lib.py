@@ -56,6 +56,8 @@ ABI_SYMBOLS = (
     "gptq_hip_cache_read_mx",
     "gptq_hip_attention_workspace_bytes",
     "gptq_hip_attend",
+    "gptq_hip_attention_mx_workspace_bytes",
+    "gptq_hip_attend_mx",
     "gptq_hip_probe",
     "gptq_hip_strerror",
     "gptq_hip_abi_version",
@@ -238,6 +240,10 @@ def lib() -> ctypes.CDLL:
     l.gptq_hip_attention_workspace_bytes.argtypes = [ctypes.POINTER(Attention)]
     l.gptq_hip_attend.restype = i
     l.gptq_hip_attend.argtypes = [ctypes.POINTER(Attention), vp, sz, vp]
+    l.gptq_hip_attention_mx_workspace_bytes.restype = sz
+    l.gptq_hip_attention_mx_workspace_bytes.argtypes = [ctypes.POINTER(CacheMx), ctypes.POINTER(Attention)]
+    l.gptq_hip_attend_mx.restype = i
+    l.gptq_hip_attend_mx.argtypes = [ctypes.POINTER(CacheMx), ctypes.POINTER(Attention), vp, sz, vp]
     l.gptq_hip_probe.restype = i
     l.gptq_hip_probe.argtypes = [i, vp, sz, vp, sz, i, i, i, i, vp, vp, vp]
     l.gptq_hip_dequant.restype = i

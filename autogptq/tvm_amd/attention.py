@@ -92,7 +92,7 @@ def cache_read(k_cache: Cache, v_cache: Cache, slots: torch.Tensor, dim: Optiona
     return _call("cache_read", k_cache, v_cache, slots)
 
 
-def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, tables: torch.Tensor, starts: torch.Tensor,
+def paged_attention(q: torch.Tensor, k_cache: Cache, v_cache: Cache, tables: torch.Tensor, starts: torch.Tensor,
                     contexts: torch.Tensor, *, max_context: int = 0, window: int = 0, sinks: int = 0,
                     scale: Optional[float] = None) -> torch.Tensor:
     """[tokens, heads, dim]: the attention of the step's tokens.  Request b has the tokens ``starts[b] .. starts[b + 1]``, the
@@ -103,15 +103,20 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     tokens of no request (those from ``starts[-1]`` on: a step may be padded to a fixed size).  Query head n reads
     key/value head n // (heads / kv_heads).  ``max_context``: the longest context as the host knows it, by which the work is
     divided (0: the tables' width); results do not depend on it beyond the order of sums.  ``scale``: 1 / sqrt(dim) if None."""
+    if _packed(k_cache, v_cache):
+        return _call("paged_attention_mx", q, *k_cache, *v_cache, tables, starts, contexts, max_context, window, sinks, _scale(scale))
     return _call("paged_attention", q, k_cache, v_cache, tables, starts, contexts, max_context, window, sinks, _scale(scale))
 
 
-def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_blocks: torch.Tensor,
+def shared_prefix_attention(q: torch.Tensor, k_cache: Cache, v_cache: Cache, prefix_blocks: torch.Tensor,
                             prefix_length: int, tables: torch.Tensor, starts: torch.Tensor, contexts: torch.Tensor, *,
                             max_context: int = 0, scale: Optional[float] = None) -> torch.Tensor:
     """``paged_attention`` where every request stands behind the same ``prefix_length`` tokens, whose blocks are
     ``prefix_blocks``: all tokens see all of them, and they are read once for the batch.  ``tables``, ``contexts`` and
     ``max_context`` count a request's own tokens only."""
+    if _packed(k_cache, v_cache):
+        return _call("shared_prefix_attention_mx", q, *k_cache, *v_cache, prefix_blocks, prefix_length, tables, starts, contexts,
+                     max_context, _scale(scale))
     return _call("shared_prefix_attention", q, k_cache, v_cache, prefix_blocks, prefix_length, tables, starts, contexts,
                  max_context, _scale(scale))
 

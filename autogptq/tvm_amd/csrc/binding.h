@@ -92,5 +92,11 @@ Tensor paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_c
 Tensor shared_prefix_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &prefix_blocks,
                                int64_t prefix_length, const Tensor &tables, const Tensor &starts, const Tensor &contexts,
                                int64_t max_context, double scale);
+Tensor paged_attention_mx(const Tensor &q, const Tensor &k_codes, const Tensor &k_scales, const Tensor &v_codes, const Tensor &v_scales,
+                          const Tensor &tables, const Tensor &starts, const Tensor &contexts, int64_t max_context, int64_t window,
+                          int64_t sinks, double scale);
+Tensor shared_prefix_attention_mx(const Tensor &q, const Tensor &k_codes, const Tensor &k_scales, const Tensor &v_codes, const Tensor &v_scales,
+                                  const Tensor &prefix_blocks, int64_t prefix_length, const Tensor &tables, const Tensor &starts,
+                                  const Tensor &contexts, int64_t max_context, double scale);
 
 }  // namespace gptq_torch

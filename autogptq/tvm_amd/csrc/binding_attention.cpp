@@ -263,66 +263,111 @@ std::tuple<Tensor, Tensor> gptq_torch::cache_read_mx(const Tensor &k_codes, cons
     return {k, v};
 }
 
-static Tensor attend(const char *what, const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &prefix_blocks,
-              int64_t prefix_length, const Tensor &tables, const Tensor &starts, const Tensor &contexts, int64_t max_context,
-              int64_t window, int64_t sinks, double scale)
+// A call but for its cache.  `cache` is the shape that q has to fit; on_cache: a tensor of it.
+struct Call {
+    const Tensor &q, &prefix_blocks;
+    int64_t prefix_length;
+    const Tensor &tables, &starts, &contexts;
+    int64_t max_context, window, sinks;
+    double scale;
+};
+template <typename Launch>
+static Tensor attend(const Call &call, const gptq_hip_cache &cache, const Tensor &on_cache, Launch launch)
 {
-    on_gpu(k_cache, "k_cache", k_cache);
+    const Tensor &q = call.q, &tables = call.tables;
     gptq_hip_attention a;
-    a.cache = describe(k_cache, v_cache);
-    on_gpu(q, "q", k_cache);
-    no_grad(q, "q");
-    no_grad(k_cache, "k_cache");
-    no_grad(v_cache, "v_cache");
-    TORCH_CHECK(q.scalar_type() == k_cache.scalar_type(), "q is ", q.scalar_type(), ", the cache ", k_cache.scalar_type());
-    TORCH_CHECK(q.dim() == 3 && q.size(2) == a.cache.dim, "q must be [tokens, heads, ", a.cache.dim, "], got ", q.sizes());
-    TORCH_CHECK(q.size(1) > 0 && q.size(1) % a.cache.heads == 0, "q has ", q.size(1), " heads, no multiple of the cache's ", a.cache.heads);
-    need_ints(contexts, "contexts", -1, k_cache);
-    const int64_t B = contexts.size(0);
-    need_ints(starts, "starts", B + 1, k_cache);
-    need_tables(tables, B, k_cache);
+    a.cache = cache;
+    TORCH_CHECK(q.dim() == 3 && q.size(2) == cache.dim, "q must be [tokens, heads, ", cache.dim, "], got ", q.sizes());
+    TORCH_CHECK(q.size(1) > 0 && q.size(1) % cache.heads == 0, "q has ", q.size(1), " heads, no multiple of the cache's ", cache.heads);
+    need_ints(call.contexts, "contexts", -1, on_cache);
+    const int64_t B = call.contexts.size(0);
+    need_ints(call.starts, "starts", B + 1, on_cache);
+    need_tables(tables, B, on_cache);
     TORCH_CHECK(B > 0 || q.size(0) == 0, "q has tokens, but there is no request");
     TORCH_CHECK(q.size(0) * q.size(1) < (1LL << 30) && B < (1LL << 24), "too many tokens or requests");
-    for (const auto &[value, name] : {std::pair<int64_t, const char *>{max_context, "max_context"}, {window, "window"}, {sinks, "sinks"}, {prefix_length, "prefix_length"}})
+    for (const auto &[value, name] : {std::pair<int64_t, const char *>{call.max_context, "max_context"}, {call.window, "window"}, {call.sinks, "sinks"}, {call.prefix_length, "prefix_length"}})
         TORCH_CHECK(value >= 0 && value < (1LL << 31), name, " must not be negative, got ", value);
-    if (scale == 0.0) scale = 1.0 / std::sqrt((double)a.cache.dim);
+    const double scale = call.scale == 0.0 ? 1.0 / std::sqrt((double)cache.dim) : call.scale;
     TORCH_CHECK(std::isfinite(scale) && scale > 0, "scale must be positive, got ", scale);
     a.prefix_blocks = nullptr;
-    if (prefix_length > 0) {
-        need_ints(prefix_blocks, "prefix_blocks", -1, k_cache);
-        const int64_t blocks = (prefix_length + a.cache.block_size - 1) / a.cache.block_size;
-        TORCH_CHECK(prefix_blocks.size(0) >= blocks, "a prefix of ", prefix_length, " tokens takes ", blocks, " blocks, prefix_blocks has ",
-                    prefix_blocks.size(0));
-        a.prefix_blocks = (const int32_t *)prefix_blocks.data_ptr();
+    if (call.prefix_length > 0) {
+        need_ints(call.prefix_blocks, "prefix_blocks", -1, on_cache);
+        const int64_t blocks = (call.prefix_length + cache.block_size - 1) / cache.block_size;
+        TORCH_CHECK(call.prefix_blocks.size(0) >= blocks, "a prefix of ", call.prefix_length, " tokens takes ", blocks, " blocks, prefix_blocks has ",
+                    call.prefix_blocks.size(0));
+        a.prefix_blocks = (const int32_t *)call.prefix_blocks.data_ptr();
     }
     Tensor out = fresh(q.sizes(), q);
     if (q.size(0) == 0) return out;
-    const c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(on_cache.device());
     const Tensor qs = loadable(q);
     a.q = qs.data_ptr(), a.out = out.data_ptr();
-    a.tables = (const int32_t *)tables.data_ptr(), a.starts = (const int32_t *)starts.data_ptr(), a.contexts = (const int32_t *)contexts.data_ptr();
+    a.tables = (const int32_t *)tables.data_ptr(), a.starts = (const int32_t *)call.starts.data_ptr(), a.contexts = (const int32_t *)call.contexts.data_ptr();
     a.tokens = (int)q.size(0), a.requests = (int)B, a.heads = (int)q.size(1), a.table_width = (int)tables.size(1);
-    a.max_context = (int)max_context, a.window = (int)window, a.sinks = (int)sinks, a.prefix_length = (int)prefix_length;
+    a.max_context = (int)call.max_context, a.window = (int)call.window, a.sinks = (int)call.sinks, a.prefix_length = (int)call.prefix_length;
     a.q_token_stride = step(qs, 0), a.q_head_stride = step(qs, 1), a.table_stride = row_stride(tables);
     a.scale = (float)scale;
-    void *stream = current_stream(k_cache);
-    const WorkspaceLease ws(q, gptq_hip_attention_workspace_bytes(&a), stream, kAttentionWorkspace);
-    raised(gptq_hip_attend(&a, ws.data(), ws.size(), stream), what);
+    launch(a, current_stream(on_cache));
     return out;
+}
+
+static Tensor attend_plain(const char *what, const Tensor &k_cache, const Tensor &v_cache, const Call &call)
+{
+    on_gpu(k_cache, "k_cache", k_cache);
+    const gptq_hip_cache cache = describe(k_cache, v_cache);
+    on_gpu(call.q, "q", k_cache);
+    no_grad(call.q, "q");
+    no_grad(k_cache, "k_cache");
+    no_grad(v_cache, "v_cache");
+    TORCH_CHECK(call.q.scalar_type() == k_cache.scalar_type(), "q is ", call.q.scalar_type(), ", the cache ", k_cache.scalar_type());
+    return attend(call, cache, k_cache, [&](const gptq_hip_attention &a, void *stream) {
+        const WorkspaceLease ws(call.q, gptq_hip_attention_workspace_bytes(&a), stream, kAttentionWorkspace);
+        raised(gptq_hip_attend(&a, ws.data(), ws.size(), stream), what);
+    });
+}
+
+static Tensor attend_mx(const char *what, const Tensor &k_codes, const Tensor &k_scales, const Tensor &v_codes, const Tensor &v_scales, const Call &call)
+{
+    on_gpu(k_codes, "k_codes", k_codes);
+    on_gpu(call.q, "q", k_codes);
+    no_grad(call.q, "q");
+    TORCH_CHECK(call.q.dim() == 3, "q must be [tokens, heads, dim], got ", call.q.sizes());
+    const gptq_hip_cache_mx mx = describe_mx(k_codes, k_scales, v_codes, v_scales, call.q.size(2), call.q.scalar_type());
+    const gptq_hip_cache shape = {mx.k, mx.v, mx.type, mx.blocks, mx.block_size, mx.heads, mx.dim, 0, 0, 0};
+    return attend(call, shape, k_codes, [&](const gptq_hip_attention &a, void *stream) {
+        const WorkspaceLease ws(call.q, gptq_hip_attention_mx_workspace_bytes(&mx, &a), stream, kAttentionWorkspace);
+        raised(gptq_hip_attend_mx(&mx, &a, ws.data(), ws.size(), stream), what);
+    });
 }
 
 Tensor gptq_torch::paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &tables, const Tensor &starts,
                        const Tensor &contexts, int64_t max_context, int64_t window, int64_t sinks, double scale)
 {
-    return attend("gptq_hip_attend", q, k_cache, v_cache, Tensor(), 0, tables, starts, contexts, max_context, window, sinks, scale);
+    return attend_plain("gptq_hip_attend", k_cache, v_cache, {q, Tensor(), 0, tables, starts, contexts, max_context, window, sinks, scale});
 }
 
 Tensor gptq_torch::shared_prefix_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &prefix_blocks,
                                int64_t prefix_length, const Tensor &tables, const Tensor &starts, const Tensor &contexts,
                                int64_t max_context, double scale)
 {
-    return attend("gptq_hip_attend (shared prefix)", q, k_cache, v_cache, prefix_blocks, prefix_length, tables, starts, contexts,
-                  max_context, 0, 0, scale);
+    return attend_plain("gptq_hip_attend (shared prefix)", k_cache, v_cache,
+                        {q, prefix_blocks, prefix_length, tables, starts, contexts, max_context, 0, 0, scale});
+}
+
+Tensor gptq_torch::paged_attention_mx(const Tensor &q, const Tensor &k_codes, const Tensor &k_scales, const Tensor &v_codes, const Tensor &v_scales,
+                                      const Tensor &tables, const Tensor &starts, const Tensor &contexts, int64_t max_context, int64_t window,
+                                      int64_t sinks, double scale)
+{
+    return attend_mx("gptq_hip_attend_mx", k_codes, k_scales, v_codes, v_scales,
+                     {q, Tensor(), 0, tables, starts, contexts, max_context, window, sinks, scale});
+}
+
+Tensor gptq_torch::shared_prefix_attention_mx(const Tensor &q, const Tensor &k_codes, const Tensor &k_scales, const Tensor &v_codes,
+                                              const Tensor &v_scales, const Tensor &prefix_blocks, int64_t prefix_length, const Tensor &tables,
+                                              const Tensor &starts, const Tensor &contexts, int64_t max_context, double scale)
+{
+    return attend_mx("gptq_hip_attend_mx (shared prefix)", k_codes, k_scales, v_codes, v_scales,
+                     {q, prefix_blocks, prefix_length, tables, starts, contexts, max_context, 0, 0, scale});
 }
 
 using namespace gptq_torch;
@@ -341,6 +386,10 @@ TORCH_LIBRARY_FRAGMENT(gptq_hip, m)
           "int max_context, int window, int sinks, float scale) -> Tensor");
     m.def("shared_prefix_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor prefix_blocks, int prefix_length, "
           "Tensor tables, Tensor starts, Tensor contexts, int max_context, float scale) -> Tensor");
+    m.def("paged_attention_mx(Tensor q, Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, Tensor tables, Tensor starts, "
+          "Tensor contexts, int max_context, int window, int sinks, float scale) -> Tensor");
+    m.def("shared_prefix_attention_mx(Tensor q, Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, Tensor prefix_blocks, "
+          "int prefix_length, Tensor tables, Tensor starts, Tensor contexts, int max_context, float scale) -> Tensor");
 }
 
 // The CPU key gets the same functions, whose first check says that there is no CPU fallback.
@@ -353,6 +402,8 @@ TORCH_LIBRARY_IMPL(gptq_hip, CUDA, m)
     m.impl("cache_read_mx", &cache_read_mx);
     m.impl("paged_attention", &paged_attention);
     m.impl("shared_prefix_attention", &shared_prefix_attention);
+    m.impl("paged_attention_mx", &paged_attention_mx);
+    m.impl("shared_prefix_attention_mx", &shared_prefix_attention_mx);
 }
 
 TORCH_LIBRARY_IMPL(gptq_hip, CPU, m)
@@ -364,4 +415,6 @@ TORCH_LIBRARY_IMPL(gptq_hip, CPU, m)
     m.impl("cache_read_mx", &cache_read_mx);
     m.impl("paged_attention", &paged_attention);
     m.impl("shared_prefix_attention", &shared_prefix_attention);
+    m.impl("paged_attention_mx", &paged_attention_mx);
+    m.impl("shared_prefix_attention_mx", &shared_prefix_attention_mx);
 }

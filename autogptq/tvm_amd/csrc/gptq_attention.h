@@ -51,6 +51,10 @@ struct AttentionParams {
     float c;
     uint32_t group_magic;    // x / group = x * magic >> 16 for x < group + kTileRows; 0: groups that are divided by
     int block_shift;         // log2(block_size), or -1
+    // caches in MXFP4: the scales; their steps in units of a row of scales, head strides (of the codes, too) in bytes
+    const void *k_scales, *v_scales;
+    long long scale_head;
+    uint32_t scale_block, scale_slot;
 };
 
 // x / group for the rows of a tile, counted from its first token's
@@ -121,17 +125,31 @@ __device__ __forceinline__ bool all_see(const AttentionParams &p, const QueryTil
                              (p.window <= 0 || (i0 >= q.front + q.ns && key_position(q, i0) > last - p.window)));
 }
 
-// Where the row of entry i stands in a cache, in units of 16 bytes (head 0).  A block that the cache does not have counts
-// as its first: the values are then undefined, the addresses are not.
-__device__ __forceinline__ uint32_t key_row(const AttentionParams &p, const QueryTile &q, const int32_t *table, int i)
+// The block that the table names for entry i of the list, and the entry's slot in it.
+struct Entry {
+    uint32_t block, slot;
+};
+__device__ __forceinline__ Entry key_entry(const AttentionParams &p, const QueryTile &q, const int32_t *table, int i)
 {
     const bool front = i < q.front;
     const uint32_t at = (uint32_t)(front ? i : key_position(q, i));
     const uint32_t j = p.block_shift >= 0 ? at >> p.block_shift : at / (uint32_t)p.block_size;
-    const uint32_t slot = at - j * (uint32_t)p.block_size;
-    uint32_t block = (uint32_t)(front ? p.prefix_blocks : table)[j];
-    if (block >= (uint32_t)p.blocks) block = 0;
-    return block * p.block_step + slot * p.slot_step;   // (the host has seen to it that no row passes 2^32)
+    return {(uint32_t)(front ? p.prefix_blocks : table)[j], at - j * (uint32_t)p.block_size};
+}
+// Where its row stands in a cache, in units of 16 bytes (head 0), and that of its scales, in units of such a row.  A block that the
+// cache does not have counts as its first: the values are then undefined, the addresses are not.  (The host has seen to it that no
+// row passes 2^32.)
+__device__ __forceinline__ uint32_t row_of(const AttentionParams &p, Entry e)
+{
+    return (e.block < (uint32_t)p.blocks ? e.block : 0) * p.block_step + e.slot * p.slot_step;
+}
+__device__ __forceinline__ uint32_t scales_of(const AttentionParams &p, Entry e)
+{
+    return (e.block < (uint32_t)p.blocks ? e.block : 0) * p.scale_block + e.slot * p.scale_slot;
+}
+__device__ __forceinline__ uint32_t key_row(const AttentionParams &p, const QueryTile &q, const int32_t *table, int i)
+{
+    return row_of(p, key_entry(p, q, table, i));
 }
 
 // fp16 or bf16 operands of the matrix instructions
@@ -358,5 +376,9 @@ __device__ void join_parts(const AttentionParams &p, const QueryTile &q, int h, 
 
 int launch_attention_few(const AttentionParams &p, int type, int rt, void *stream);
 int launch_attention_tile(const AttentionParams &p, int type, void *stream);
+void launch_attention_join(const AttentionParams &p, int type, unsigned tiles, void *stream);   // of the tiles' parts, `tiles` of all heads
+// the same of a cache in MXFP4
+int launch_attention_few_mx(const AttentionParams &p, int type, int rt, void *stream);
+int launch_attention_tile_mx(const AttentionParams &p, int type, void *stream);
 
 }  // namespace gptq

@@ -136,10 +136,10 @@ int plan(const gptq_hip_attention &a, Plan &pl)
     return GPTQ_HIP_OK;
 }
 
-int check(const gptq_hip_attention *a)
+// rc: what the checks of the cache said
+int check(const gptq_hip_attention *a, int rc)
 {
     if (!a) return GPTQ_HIP_ERR_BAD_ARG;
-    const int rc = check_cache(&a->cache);
     if (rc != GPTQ_HIP_OK) return rc;
     if (a->tokens < 0 || a->requests < 0 || a->table_width < 0 || a->max_context < 0 || a->window < 0 || a->sinks < 0 ||
         a->prefix_length < 0)
@@ -157,32 +157,21 @@ int check(const gptq_hip_attention *a)
     return GPTQ_HIP_OK;
 }
 
-}  // namespace
-}  // namespace gptq
-
-extern "C" size_t gptq_hip_attention_workspace_bytes(const gptq_hip_attention *a)
+// mx: nullptr, or the cache in MXFP4, whose shape is a.cache's
+int attend(const gptq_hip_attention *a, const gptq_hip_cache_mx *mx, void *workspace, size_t workspace_bytes, void *stream)
 {
-    gptq::Plan pl;
-    if (gptq::check(a) != GPTQ_HIP_OK || a->tokens == 0 || gptq::plan(*a, pl) != GPTQ_HIP_OK) return 0;
-    return pl.bytes;
-}
-
-extern "C" int gptq_hip_attend(const gptq_hip_attention *a, void *workspace, size_t workspace_bytes, void *stream)
-{
-    int rc = gptq::check(a);
-    if (rc != GPTQ_HIP_OK || a->tokens == 0) return rc;
-    gptq::Plan pl;
-    rc = gptq::plan(*a, pl);
+    Plan pl;
+    int rc = plan(*a, pl);
     if (rc != GPTQ_HIP_OK) return rc;
     if (pl.bytes && (!workspace || (uintptr_t)workspace % 16 != 0 || workspace_bytes < pl.bytes)) return GPTQ_HIP_ERR_WORKSPACE;
 
-    gptq::AttentionParams p = {};
+    AttentionParams p = {};
     const gptq_hip_cache &c = a->cache;
     p.q = a->q, p.k = c.k, p.v = c.v, p.out = a->out;
     if (pl.bytes) {
         const size_t rows = pl.prefix_rows + pl.own_rows;
         p.counters = (int *)workspace;
-        p.stats = (float *)((char *)workspace + gptq::kAttentionCounters);
+        p.stats = (float *)((char *)workspace + kAttentionCounters);
         p.parts = (float *)((char *)p.stats + (rows * 8 + 255) / 256 * 256);
         p.own_stats = p.stats + 2 * pl.prefix_rows;
         p.own_parts = p.parts + pl.prefix_rows * c.dim;
@@ -190,13 +179,21 @@ extern "C" int gptq_hip_attend(const gptq_hip_attention *a, void *workspace, siz
     p.tokens = a->tokens, p.requests = a->requests, p.heads = a->heads, p.kv_heads = c.heads, p.group = a->heads / c.heads;
     p.dim = c.dim, p.blocks = c.blocks, p.block_size = c.block_size;
     p.q_token = a->q_token_stride, p.q_head = a->q_head_stride;
-    p.head_stride = c.head_stride, p.block_step = (uint32_t)(c.block_stride / 8), p.slot_step = (uint32_t)(c.slot_stride / 8);
+    if (mx) {
+        const long long scales = mx_scale_bytes(c.dim);
+        p.head_stride = mx->head_stride, p.block_step = (uint32_t)(mx->block_stride / 16), p.slot_step = (uint32_t)(mx->slot_stride / 16);
+        p.k_scales = mx->k_scales, p.v_scales = mx->v_scales, p.scale_head = mx->scale_head_stride;
+        p.scale_block = (uint32_t)(mx->scale_block_stride / scales), p.scale_slot = (uint32_t)(mx->scale_slot_stride / scales);
+    } else {
+        p.head_stride = c.head_stride, p.block_step = (uint32_t)(c.block_stride / 8), p.slot_step = (uint32_t)(c.slot_stride / 8);
+    }
     p.c = a->scale * 1.44269504088896340736f;
-    if ((long long)p.group * (p.group + gptq::kTileRows) < 65536) p.group_magic = 65535u / (uint32_t)p.group + 1u;
+    if ((long long)p.group * (p.group + kTileRows) < 65536) p.group_magic = 65535u / (uint32_t)p.group + 1u;
     p.block_shift = c.block_size & (c.block_size - 1) ? -1 : __builtin_ctz((unsigned)c.block_size);
-    auto launch = [&](const gptq::Division &d) {
+    auto launch = [&](const Division &d) {
         p.tiles = d.tiles, p.splits = d.splits, p.chunk = d.chunk, p.team = d.team, p.most_units = d.most_units;
-        return d.rt ? gptq::launch_attention_few(p, c.type, d.rt, stream) : gptq::launch_attention_tile(p, c.type, stream);
+        if (d.rt) return mx ? launch_attention_few_mx(p, c.type, d.rt, stream) : launch_attention_few(p, c.type, d.rt, stream);
+        return mx ? launch_attention_tile_mx(p, c.type, stream) : launch_attention_tile(p, c.type, stream);
     };
     p.prefix_blocks = a->prefix_blocks;
     if (pl.prefix) {
@@ -209,6 +206,50 @@ extern "C" int gptq_hip_attend(const gptq_hip_attention *a, void *workspace, siz
     }
     p.tables = a->tables, p.table_width = a->table_width, p.table_stride = a->table_stride;
     p.starts = a->starts, p.contexts = a->contexts;
-    p.window = std::min(a->window, gptq::kMostKeys), p.sinks = std::min(a->sinks, gptq::kMostKeys);
+    p.window = std::min(a->window, kMostKeys), p.sinks = std::min(a->sinks, kMostKeys);
     return launch(pl.own);
+}
+
+// a call on a cache in MXFP4, with that cache's shape
+gptq_hip_attention with_shape_of(const gptq_hip_attention &a, const gptq_hip_cache_mx &mx)
+{
+    gptq_hip_attention b = a;
+    b.cache = {mx.k, mx.v, mx.type, mx.blocks, mx.block_size, mx.heads, mx.dim, 0, 0, 0};
+    return b;
+}
+
+}  // namespace
+}  // namespace gptq
+
+extern "C" size_t gptq_hip_attention_workspace_bytes(const gptq_hip_attention *a)
+{
+    gptq::Plan pl;
+    if (!a || gptq::check(a, gptq::check_cache(&a->cache)) != GPTQ_HIP_OK || a->tokens == 0 || gptq::plan(*a, pl) != GPTQ_HIP_OK) return 0;
+    return pl.bytes;
+}
+
+extern "C" int gptq_hip_attend(const gptq_hip_attention *a, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!a) return GPTQ_HIP_ERR_BAD_ARG;
+    const int rc = gptq::check(a, gptq::check_cache(&a->cache));
+    if (rc != GPTQ_HIP_OK || a->tokens == 0) return rc;
+    return gptq::attend(a, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t gptq_hip_attention_mx_workspace_bytes(const gptq_hip_cache_mx *cache, const gptq_hip_attention *given)
+{
+    if (!cache || !given) return 0;
+    const gptq_hip_attention a = gptq::with_shape_of(*given, *cache);
+    gptq::Plan pl;
+    if (gptq::check(&a, gptq::check_cache_mx(cache)) != GPTQ_HIP_OK || a.tokens == 0 || gptq::plan(a, pl) != GPTQ_HIP_OK) return 0;
+    return pl.bytes;
+}
+
+extern "C" int gptq_hip_attend_mx(const gptq_hip_cache_mx *cache, const gptq_hip_attention *given, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!cache || !given) return GPTQ_HIP_ERR_BAD_ARG;
+    const gptq_hip_attention a = gptq::with_shape_of(*given, *cache);
+    const int rc = gptq::check(&a, gptq::check_cache_mx(cache));
+    if (rc != GPTQ_HIP_OK || a.tokens == 0) return rc;
+    return gptq::attend(&a, cache, workspace, workspace_bytes, stream);
 }

@@ -460,9 +460,46 @@ PyObject *call_shared_prefix_attention(PyObject *, PyObject *const *args, Py_ssi
     END_HANDLE_TH_ERRORS
 }
 
+PyObject *call_paged_attention_mx(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    Arguments a(args, n, 12);
+    const Tensor &q = a.tensor(0), &kc = a.tensor(1), &ks = a.tensor(2), &vc = a.tensor(3), &vs = a.tensor(4), &tables = a.tensor(5),
+                 &starts = a.tensor(6), &contexts = a.tensor(7);
+    const int64_t most = a.integer(8), window = a.integer(9), sinks = a.integer(10);
+    const double scale = a.real(11);
+    if (!a.plain) Py_RETURN_NOTIMPLEMENTED;
+    Tensor out;
+    {
+        const WithoutInterpreter free;
+        out = paged_attention_mx(q, kc, ks, vc, vs, tables, starts, contexts, most, window, sinks, scale);
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *call_shared_prefix_attention_mx(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    Arguments a(args, n, 12);
+    const Tensor &q = a.tensor(0), &kc = a.tensor(1), &ks = a.tensor(2), &vc = a.tensor(3), &vs = a.tensor(4), &blocks = a.tensor(5),
+                 &tables = a.tensor(7), &starts = a.tensor(8), &contexts = a.tensor(9);
+    const int64_t length = a.integer(6), most = a.integer(10);
+    const double scale = a.real(11);
+    if (!a.plain) Py_RETURN_NOTIMPLEMENTED;
+    Tensor out;
+    {
+        const WithoutInterpreter free;
+        out = shared_prefix_attention_mx(q, kc, ks, vc, vs, blocks, length, tables, starts, contexts, most, scale);
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 #define GPTQ_FAST(NAME) {#NAME, (PyCFunction)(void (*)(void))call_##NAME, METH_FASTCALL, "torch.ops.gptq_hip." #NAME " on plain tensors, else NotImplemented."}
 PyMethodDef functions[] = {GPTQ_FAST(cache_tables), GPTQ_FAST(cache_write), GPTQ_FAST(cache_read), GPTQ_FAST(cache_write_mx), GPTQ_FAST(cache_read_mx),
                            GPTQ_FAST(paged_attention), GPTQ_FAST(shared_prefix_attention),
+                           GPTQ_FAST(paged_attention_mx), GPTQ_FAST(shared_prefix_attention_mx),
                            {"capture", capture, METH_O, "capture(stream): 0, or a number of the graph capture that the stream is in."},
                            {"aside", aside, METH_VARARGS, "aside(fn, *args): fn(*args), hidden from tracing and dispatch modes."},
                            {"install", install, METH_O, "Makes the call in C the one of a QuantLinear class."}, {nullptr, nullptr, 0, nullptr}};

@@ -498,6 +498,8 @@ def _register_torch_ops():
         meta.impl("cache_read_mx", _meta_cache_read_mx)
         meta.impl("paged_attention", lambda q, *args: q.new_empty(q.shape))
         meta.impl("shared_prefix_attention", lambda q, *args: q.new_empty(q.shape))
+        meta.impl("paged_attention_mx", lambda q, *args: q.new_empty(q.shape))
+        meta.impl("shared_prefix_attention_mx", lambda q, *args: q.new_empty(q.shape))
     keep.append(meta)
     return keep
 

@@ -459,6 +459,11 @@ typedef struct gptq_hip_attention {
 size_t gptq_hip_attention_workspace_bytes(const gptq_hip_attention *a);
 int gptq_hip_attend(const gptq_hip_attention *a, void *workspace, size_t workspace_bytes, void *stream);
 
+/* The same over a cache in MXFP4; a->cache is not read.  What a token does not see may stand for NaN among the keys, and must be finite
+ * among the values, as above. */
+size_t gptq_hip_attention_mx_workspace_bytes(const gptq_hip_cache_mx *cache, const gptq_hip_attention *a);
+int gptq_hip_attend_mx(const gptq_hip_cache_mx *cache, const gptq_hip_attention *a, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Human-readable text for a gptq_hip_status. */
 const char *gptq_hip_strerror(int status);
 

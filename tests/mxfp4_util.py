@@ -3,6 +3,8 @@ import math
 
 import torch
 
+from tests.attention_util import Step
+
 VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 EXPONENTS = {torch.float16: (-23, 13), torch.bfloat16: (-125, 125)}
 
@@ -57,3 +59,27 @@ def empty(blocks, block_size, heads, dim, layout="head", device="cuda", code=0x7
         both = torch.full(shape, fill, dtype=torch.uint8, device=device)
         made.append(both if layout == "token" else both.transpose(2, 3))
     return Mxfp4(made[0][0], made[1][0]), Mxfp4(made[0][1], made[1][1])
+
+
+class MxStep(Step):
+    """A ``Step`` whose cache is held in MXFP4: what the oracle sees are the values that the codes stand for.  (What no token may read
+    is NaN here, too.)"""
+
+    def __init__(self, *args, **more):
+        super().__init__(*args, **more)
+        self.quantise()
+
+    def quantise(self):
+        from autogptq.tvm_amd.attention import Mxfp4
+
+        packed = []
+        for cache in (self.k_cache, self.v_cache):
+            codes, scales = encode(cache)
+            n = widths(self.dim)[1]
+            scales = torch.nn.functional.pad(scales, (0, n - scales.shape[-1]), value=255)
+            # in the memory order of the cache
+            heads_first = cache.stride(2) > cache.stride(1)
+            order = (lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)) if heads_first else (lambda t: t.contiguous())
+            packed.append(Mxfp4(order(codes), order(scales)))
+        self.k_cache, self.v_cache = packed
+        self.k, self.v = ([decode(*encode(x), self.dim) for x in rows] for rows in (self.k, self.v))

@@ -29,14 +29,25 @@ class Step(NamedTuple):
 
 class PagedCache:
     """``blocks`` blocks of ``block_size`` tokens in ``layers`` layers, for up to ``max_requests`` requests at a time, each of up to
-    ``max_context`` tokens.  A request is a number below ``max_requests``; it exists from its first ``step`` to ``free``."""
+    ``max_context`` tokens.  A request is a number below ``max_requests``; it exists from its first ``step`` to ``free``.
+
+    ``dtype`` is that of keys, values and queries.  ``quantize="mxfp4"`` holds them in 4.25 bits a value (``attention.Mxfp4``): 3.76 times the
+    tokens in the same memory, read that much faster when decoding, with a root mean square error of 0.11 of a group's."""
 
     def __init__(self, layers: int, blocks: int, block_size: int, kv_heads: int, dim: int, max_requests: int, max_context: int,
-                 dtype=torch.float16, device="cuda:0"):
-        self.block_size = block_size
+                 dtype=torch.float16, device="cuda:0", quantize: Optional[str] = None):
+        if quantize not in (None, "mxfp4"):
+            raise ValueError(f"quantize must be None or 'mxfp4', got {quantize!r}")
+        if quantize and dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"an MXFP4 cache holds float16 or bfloat16 values, not {dtype}")
+        self.block_size, self.dim, self.dtype, self.quantize = block_size, dim, dtype, quantize
         # a block's keys (or values) of a head lie together: whole kilobytes for the kernels that read one head
-        both = torch.empty((layers, 2, blocks, kv_heads, block_size, dim), dtype=dtype, device=device).transpose(3, 4)
-        self.k, self.v = both[:, 0], both[:, 1]
+        if quantize:
+            made = [attention.mxfp4_cache(blocks, block_size, kv_heads, dim, device) for _ in range(layers)]
+            self.k, self.v = [k for k, _ in made], [v for _, v in made]
+        else:
+            both = torch.empty((layers, 2, blocks, kv_heads, block_size, dim), dtype=dtype, device=device).transpose(3, 4)
+            self.k, self.v = both[:, 0], both[:, 1]
         width = -(-max_context // block_size)
         self.tables = torch.full((max_requests, width), -1, dtype=torch.int32, device=device)
         self._free = torch.arange(blocks, dtype=torch.int32, device=device)
@@ -121,12 +132,14 @@ class PagedCache:
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, step: Step) -> None:
         """The step's keys and values [tokens, kv_heads, dim] of a layer."""
+        self._in_type(k=k, v=v)
         attention.cache_write(k, v, self.k[layer], self.v[layer], step.slots)
 
     def attend(self, layer: int, q: torch.Tensor, step: Step, window: int = 0, sinks: int = 0,
                scale: Optional[float] = None) -> torch.Tensor:
         """The attention of the step's queries [tokens, heads, dim] in a layer, after ``write``."""
         k, v = self.k[layer], self.v[layer]
+        self._in_type(q=q)
         if step.window and not (0 < window <= step.window and sinks <= step.sinks):
             raise ValueError(f"what trim has left of these requests suffices for windows of at most {step.window} tokens and {step.sinks} "
                              f"sinks, not for window={window}, sinks={sinks}")
@@ -137,6 +150,23 @@ class PagedCache:
             raise NotImplementedError("a sliding window behind a shared prefix")
         return attention.shared_prefix_attention(q, k, v, step.prefix[0], step.prefix[1], step.tables, step.starts, step.contexts,
                                                  max_context=step.max_context, scale=scale)
+
+    def read(self, layer: int, request: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values [length, kv_heads, dim] of a request's own tokens in a layer, as attention sees them; zeros for tokens whose
+        blocks trim() has given back."""
+        self._known(request)
+        at = torch.arange(self._lengths[request], dtype=torch.int32, device=self.tables.device)
+        block = torch.div(at, self.block_size, rounding_mode="floor")
+        slots = self.tables[request][block] * self.block_size + at - block * self.block_size     # (of a block -1: below 0)
+        if self.quantize:
+            return attention.cache_read(self.k[layer], self.v[layer], slots, self.dim, self.dtype)
+        return attention.cache_read(self.k[layer], self.v[layer], slots)
+
+    def _in_type(self, **tensors: torch.Tensor) -> None:
+        """(The codes of a quantised cache do not say which type they were written from.)"""
+        for name, t in tensors.items():
+            if self.quantize and t.dtype != self.dtype:
+                raise ValueError(f"{name} is {t.dtype}, the cache holds values of {self.dtype}")
 
     def _forget(self, request: int, first: int, last: Optional[int] = None) -> None:
         """Takes entries out of a request's table.  (Steps keep theirs; the entries that later steps add lie past their contexts.)"""

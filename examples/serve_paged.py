@@ -5,7 +5,9 @@ long conversation under a sliding window.
 
 Random weights of random layers (there is no checkpoint here), the quantised layers of this package for every product, and
 ``PagedCache`` with the attention that reads it between them.  Every step's logits are compared with a plain evaluation of the
-same model over the whole sequences."""
+same model over the whole sequences.  Then the same from a cache in 4 bits, where every layer's attention is compared with a plain one
+over the keys and values that the cache gives back.  (Not the logits: a value that two evaluations put a hair apart may be rounded to
+different codes, and layers upon layers of a random model make much of it.)"""
 import math
 import os
 import sys
@@ -73,55 +75,79 @@ class Decoder(nn.Module):
         return _normed(h).float() @ self.embedding.float().t()
 
     @torch.no_grad()
-    def step(self, cache, requests, tokens, window=0, sinks=0):
+    def step(self, cache, requests, tokens, window=0, sinks=0, watch=None):
         """Logits of the new tokens (one 1-D tensor a request), which are in the cache afterwards."""
         step = cache.step(requests, [t.numel() for t in tokens])
 
         def attend(layer, q, k, v):
             cache.write(layer, k, v, step)
-            return cache.attend(layer, q, step, window=window, sinks=sinks)
+            out = cache.attend(layer, q, step, window=window, sinks=sinks)
+            if watch:
+                watch(layer, q, out)
+            return out
         return self._run(torch.cat(tokens), step.positions, attend)
 
     @torch.no_grad()
     def plain(self, tokens, window=0, sinks=0):
         """The same over one whole sequence, with the attention as torch operations in 32 bits."""
         p = torch.arange(tokens.numel(), device=tokens.device)
-        sees = p[None] <= p[:, None]
-        if window:
-            sees &= (p[None] > p[:, None] - window) | (p[None] < sinks)
-
-        def attend(layer, q, k, v):
-            k, v = (x.float().repeat_interleave(HEADS // KV_HEADS, 1).transpose(0, 1).contiguous() for x in (k, v))
-            s = q.float().transpose(0, 1) @ k.transpose(1, 2).contiguous() / math.sqrt(DIM)
-            return (torch.softmax(s.masked_fill(~sees, -math.inf), -1) @ v).transpose(0, 1).half()
-        return self._run(tokens, p, attend)
+        return self._run(tokens, p, lambda layer, q, k, v: _attention(q, k, v, window, sinks))
 
 
-def main(device="cuda:0", verbose=True):
+def _attention(q, k, v, window=0, sinks=0):
+    """Causal attention of the last len(q) of len(k) tokens."""
+    j = torch.arange(len(k), device=q.device)
+    p = j[len(k) - len(q):, None]
+    sees = j[None] <= p
+    if window:
+        sees &= (j[None] > p - window) | (j[None] < sinks)
+    k, v = (x.float().repeat_interleave(HEADS // KV_HEADS, 1).transpose(0, 1).contiguous() for x in (k, v))
+    s = q.float().transpose(0, 1) @ k.transpose(1, 2).contiguous() / math.sqrt(DIM)
+    return (torch.softmax(s.masked_fill(~sees, -math.inf), -1) @ v).transpose(0, 1).half()
+
+
+def main(device="cuda:0", verbose=True, quantize=None):
     model = Decoder().to(device).eval()
     fuse_shared_input_layers(model)
     gen = torch.Generator().manual_seed(3)
     draw = lambda n: torch.randint(0, VOCAB, (n,), generator=gen).to(device)
-    cache = PagedCache(LAYERS, blocks=96, block_size=16, kv_heads=KV_HEADS, dim=DIM, max_requests=6, max_context=640, device=device)
+    cache = PagedCache(LAYERS, blocks=96, block_size=16, kv_heads=KV_HEADS, dim=DIM, max_requests=6, max_context=640, device=device,
+                       quantize=quantize)
     worst = 0.0
 
-    def check(got, whole, what, **mask):
+    def compare(got, want, what):
         nonlocal worst
-        want = model.plain(whole, **mask)[-got.shape[0]:]
-        off = float((got - want).norm() / want.norm())
+        off = float((got.float() - want.float()).norm() / want.float().norm())
         worst = max(worst, off)
         assert off < 2e-2, f"{what}: {off}"
         if verbose:
             print(f"{what}: relative difference {off:.2g}", flush=True)
 
+    def check(got, whole, what, **mask):
+        if not quantize:
+            compare(got, model.plain(whole, **mask)[-got.shape[0]:], what)
+
+    def step(requests, tokens, **mask):
+        def watch(layer, q, out):
+            at = 0
+            for r, n in zip(requests, map(len, tokens)):
+                k, v = cache.read(layer, r)
+                if r in behind:
+                    k, v = (torch.cat([a[:behind[r]], b]) for a, b in zip(cache.read(layer, 0), (k, v)))
+                compare(out[at:at + n], _attention(q[at:at + n], k, v, **mask), f"layer {layer} of request {r} at {len(k)} tokens")
+                at += n
+        return model.step(cache, requests, tokens, watch=watch if quantize else None, **mask)
+    behind = {}         # tokens of request 0 that a request stands behind
+
     # an instruction prompt, then four requests behind it with prompts of their own, then decoding together
     instructions = draw(100)
-    check(model.step(cache, [0], [instructions]), instructions, "instructions of 100 tokens")
+    check(step([0], [instructions]), instructions, "instructions of 100 tokens")
     requests = [1, 2, 3, 4]
     for r in requests:
         cache.share(0, r)
+        behind[r] = instructions.numel()
     texts = [draw(n) for n in (7, 33, 1, 64)]
-    logits = model.step(cache, requests, texts)
+    logits = step(requests, texts)
     ends = torch.tensor([t.numel() for t in texts]).cumsum(0) - 1
     for n in range(8):
         for i, r in enumerate(requests):
@@ -129,18 +155,18 @@ def main(device="cuda:0", verbose=True):
             check(rows, torch.cat([instructions, texts[i]]), f"request {r} at {100 + texts[i].numel()} tokens")
         new = [logits[e].argmax()[None] for e in ends]
         texts = [torch.cat([t, x]) for t, x in zip(texts, new)]
-        logits, ends = model.step(cache, requests, new), torch.arange(4)
+        logits, ends = step(requests, new), torch.arange(4)
     for r in requests:
         cache.free(r)
 
     # a long conversation under a window of 48 tokens and 4 sinks, its old blocks given back as it goes
     text, mask = draw(200), dict(window=48, sinks=4)
-    check(model.step(cache, [5], [text], **mask), text, "conversation of 200 tokens under a window", **mask)
+    check(step([5], [text], **mask), text, "conversation of 200 tokens under a window", **mask)
     for n in range(24):
         cache.trim(5, **mask)
         new = draw(1 + n % 3)
         text = torch.cat([text, new])
-        check(model.step(cache, [5], [new], **mask), text, f"conversation of {text.numel()} tokens", **mask)
+        check(step([5], [new], **mask), text, f"conversation of {text.numel()} tokens", **mask)
     cache.free(5)
     cache.free(0)
     assert cache.free_blocks == 96
@@ -149,3 +175,4 @@ def main(device="cuda:0", verbose=True):
 
 if __name__ == "__main__":
     print(f"done, largest relative difference {main():.2g}")
+    print(f"from a cache in 4 bits, largest relative difference of an attention {main(quantize='mxfp4'):.2g}")

@@ -29,6 +29,13 @@ namespace gptq {
 constexpr int kTileRows = 128;       // of a tile at most
 constexpr int kMostKeys = 1 << 29;   // of a request, a prefix, a window: sums of positions and widths stay within 32 bits
 
+// Workgroups of the few-rows kernel that a CU holds, by its registers: rt 16-row operands a wave, heads of up to `dim`.
+constexpr int few_resident(int rt, int dim, bool mx)
+{
+    if (mx) return dim > 128 ? 2 : rt == 1 ? 4 : dim > 64 ? 2 : 3;
+    return dim > 128 ? 1 : (rt == 1 ? 3 : 2) + (dim <= 64);
+}
+
 struct AttentionParams {
     const void *q, *k, *v;
     void *out;
@@ -55,6 +62,10 @@ struct AttentionParams {
     const void *k_scales, *v_scales;
     long long scale_head;
     uint32_t scale_block, scale_slot;
+    // x / block_size = (8 x magic >> 32) >> bits for x < 2^29: with bits = ceil(log2(block_size)) and magic = ceil(2^(29 + bits) / block_size)
+    // the excess of the product, x times less than block_size, stays below 2^(29 + bits)
+    uint32_t block_magic;
+    int block_bits;
 };
 
 // x / group for the rows of a tile, counted from its first token's
@@ -129,11 +140,13 @@ __device__ __forceinline__ bool all_see(const AttentionParams &p, const QueryTil
 struct Entry {
     uint32_t block, slot;
 };
+// (MAGIC: the division without a branch, see block_magic)
+template <bool MAGIC>
 __device__ __forceinline__ Entry key_entry(const AttentionParams &p, const QueryTile &q, const int32_t *table, int i)
 {
     const bool front = i < q.front;
     const uint32_t at = (uint32_t)(front ? i : key_position(q, i));
-    const uint32_t j = p.block_shift >= 0 ? at >> p.block_shift : at / (uint32_t)p.block_size;
+    const uint32_t j = MAGIC ? __umulhi(at << 3, p.block_magic) >> p.block_bits : p.block_shift >= 0 ? at >> p.block_shift : at / (uint32_t)p.block_size;
     return {(uint32_t)(front ? p.prefix_blocks : table)[j], at - j * (uint32_t)p.block_size};
 }
 // Where its row stands in a cache, in units of 16 bytes (head 0), and that of its scales, in units of such a row.  A block that the
@@ -149,7 +162,7 @@ __device__ __forceinline__ uint32_t scales_of(const AttentionParams &p, Entry e)
 }
 __device__ __forceinline__ uint32_t key_row(const AttentionParams &p, const QueryTile &q, const int32_t *table, int i)
 {
-    return row_of(p, key_entry(p, q, table, i));
+    return row_of(p, key_entry<false>(p, q, table, i));
 }
 
 // fp16 or bf16 operands of the matrix instructions
@@ -184,6 +197,14 @@ __device__ __forceinline__ f2 swap_quarters(float x)
     const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
     const uint32_t a = r[0], b = r[1];
     return (f2){__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
+}
+// The larger of two numbers, as the median of them and infinity.  (fmaxf would first make a quiet NaN of each operand that the compiler
+// knows nothing about, and so would a median with an infinity that it knows.)
+__device__ __forceinline__ float max2(float a, float b)
+{
+    float infinity = __builtin_inff();
+    asm("" : "+v"(infinity));
+    return __builtin_amdgcn_fmed3f(a, b, infinity);
 }
 __device__ __forceinline__ float max_halves(float x) { const f2 r = swap_halves(x); return fmaxf(r[0], r[1]); }
 __device__ __forceinline__ float add_halves(float x) { const f2 r = swap_halves(x); return r[0] + r[1]; }

@@ -27,6 +27,8 @@
 #include "gptq_attention.h"
 #include "gptq_mx.h"
 
+#include <type_traits>
+
 namespace gptq {
 
 constexpr int kFewWaves = 4, kFewUnit = 256;
@@ -73,7 +75,7 @@ __device__ __forceinline__ int sum_upto(int x)
 // DP: compiled width, the dims past p.dim do not count; FULL: there are none; RT: 16-row operands a wave holds; SHARED: the parts of a
 // shared prefix; MX: a cache in MXFP4
 template <typename E, int DP, bool FULL, int RT, bool SHARED, bool MX>
-__global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + (DP == 64)) void attention_few_kernel(const AttentionParams given)
+__global__ __launch_bounds__(64 * kFewWaves, few_resident(RT, DP, MX)) void attention_few_kernel(const AttentionParams given)
 {
     typedef typename Vec<E>::e8 e8;
     constexpr int R = 16 * RT, NW = kFewWaves;
@@ -84,8 +86,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
     constexpr int VW = VE / 2;                     // dwords of that
     constexpr int OD = DP + 4;                     // row of O in LDS
     constexpr int GW = DP > 128 ? 2 : 1;           // MX: words of a row's scales
-    constexpr int AHEAD = MX ? 2 : 1;              // blocks of a wave whose keys and values are in flight or in registers
-    __shared__ uint32_t plain_list[MX ? 1 : NW][2][64];
+    __shared__ uint32_t list[MX ? 1 : NW][2][64];
     __shared__ float stat_m[NW][16 * RT], stat_l[NW][16 * RT];
     __shared__ __align__(16) float join[NW * 16 * OD];
     __shared__ int flag;
@@ -104,6 +105,17 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
         // (Whole tiles of two units rather than their halves, once every CU has a workgroup: the second unit costs less than
         // the join.  32 contexts of 300 tokens, 8 heads: 12.0 us, in halves 13.9; 4 of 512, where CUs are left, 10.4 in halves.)
         share = max((total + given.team - 1) / given.team, total * given.kv_heads > 256 && total <= 2 * given.requests ? 2 : 1);
+        if constexpr (MX) {
+            // A part costs a workgroup some 6 us around its keys, 256 of them 1.2 (a quarter of the bytes, but as many steps as of a cache in
+            // 16 bits), and its join a tenth: fewer and longer parts where a tile has many units, more so once memory is the
+            // bound, and whole tiles where each CU has two of them.  (8 key/value heads, us with the shortest parts and so: 1
+            // context of 32768 29.2 / 17.6, of 8192 12.4 / 11.2; 4 of 32768 38.7 / 33.0, 16 of 8192 34.4 / 31.8; 64 of 1024 19.7 / 16.4.)
+            const int tile_units = (total + given.requests - 1) / given.requests;
+            int least = (int)__builtin_sqrtf((float)(total / given.requests) * 0.125f);
+            if ((long long)total * given.kv_heads >= 4096 && tile_units >= 8) least = max(least, 8);
+            if ((long long)given.requests * given.kv_heads >= 512 && tile_units <= 4) least = max(least, tile_units);
+            share = max(share, least);
+        }
         at = member * share;
         stop = min(at + share, total);
         if (at >= stop) return;
@@ -120,13 +132,6 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
         const int dim = FULL ? DP : p.dim;
         const char *kbase = (const char *)p.k + (long long)h * p.head_stride * (MX ? 1 : 2);
         const char *vbase = (const char *)p.v + (long long)h * p.head_stride * (MX ? 1 : 2);
-        // MX: a wave's lists lie where its sums go at the end
-        auto list = [&](int turn) { return MX ? (uint32_t *)(join + wave * 16 * OD) + 64 * turn : plain_list[MX ? 0 : wave][turn]; };
-        auto key_scales = [&](int turn, int word) { return (uint32_t *)(join + wave * 16 * OD) + 64 * (2 + 2 * word + turn); };
-        auto value_scales = [&](int turn, int word) { return (uint32_t *)(join + wave * 16 * OD) + 64 * (2 + 2 * GW + 2 * word + turn); };
-        static_assert(64 * (2 + 4 * GW) <= 16 * OD, "");
-        const int groups = MX ? mx_groups(dim) : 0;
-
         // a tile and a part [begin, end) of its list; the tile's parts belong to the members from `first` on
         QueryTile q;
         int begin, end, first = member, parts = 1, context = p.prefix, keys = p.chunk;
@@ -163,34 +168,11 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
         const int32_t *table = p.tables + (long long)q.b * p.table_stride;
         // blocks of 32 keys: a wave takes every fourth, and looks two of its own up at a time, one a half of its lanes (past
         // the end: the last key's row again)
-        const int blocks = (end - begin + 31) / 32, busy = min(blocks, NW);   // ... waves that have keys
-        auto entry_of = [&](int n) { return key_entry(p, q, table, min(begin + (n + (lane >> 5) * NW) * 32 + (lane & 31), end - 1)); };
-        auto look_up = [&](int n) { return row_of(p, entry_of(n)); };
+        // (MX: blocks of 64, so that what a wave asks for at a time lies together)
+        const int blocks = MX ? (end - begin + 63) / 64 : (end - begin + 31) / 32, busy = min(blocks, NW);   // ... waves that have keys
+        auto look_up = [&](int n) { return key_row(p, q, table, min(begin + (n + (lane >> 5) * NW) * 32 + (lane & 31), end - 1)); };
         uint32_t next = 0;
-        Entry entry = {0, 0};
-        if (MX && wave < blocks) entry = entry_of(wave);
         if (!MX && wave < blocks) next = look_up(wave);
-        // MX: the scales of the lane's key and value
-        uint32_t next_scales[2][GW];
-        auto load_scales = [&]() {
-            const unsigned long long at = scales_of(p, entry);
-            const long long head = (long long)h * p.scale_head;
-            for (int kv = 0; kv < 2; kv++) {
-                const char *from = (const char *)(kv ? p.v_scales : p.k_scales) + head + at * (DP / 32);
-                if constexpr (DP == 64) {
-                    next_scales[kv][0] = *(const uint16_t *)from;
-                } else if constexpr (DP == 128) {
-                    next_scales[kv][0] = *(const uint32_t *)from;
-                } else {
-                    const u2 x = *(const u2 *)from;
-                    next_scales[kv][0] = x[0], next_scales[kv][GW - 1] = x[1];
-                }
-            }
-        };
-        auto enter_scales = [&](int turn) {
-#pragma unroll
-            for (int w = 0; w < GW; w++) key_scales(turn, w)[lane] = next_scales[0][w], value_scales(turn, w)[lane] = next_scales[1][w];
-        };
 
         // the query rows as B operands, and what they see
         e8 qf[RT][KS];
@@ -231,49 +213,6 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                 for (int s = FIRST; s < KS; s++) kr[a][s] = (u4){0u, 0u, 0u, 0u};
         }
         uint32_t vr[8][VH][VW];
-        // MX: a lane's operands of a key are the groups g, 4 + g (a half of one at rows of two), which lie side by side, so that its order
-        // of dims is that of the groups; of a value it has the same dims as above
-        uint32_t kc[AHEAD][2][KS], vc[AHEAD][8][VH];
-        if constexpr (!FULL && MX) {
-#pragma unroll
-            for (int b = 0; b < AHEAD; b++)
-#pragma unroll
-                for (int a = 0; a < 2; a++)
-#pragma unroll
-                    for (int s = 0; s < KS; s++) kc[b][a][s] = 0u;
-        }
-        auto has_group = [&](int u) { return FULL || (DP == 64 ? g / 2 : 4 * u + g) < groups; };
-        auto load_key_codes = [&](const uint32_t *rows, int b) {
-#pragma unroll
-            for (int a = 0; a < 2; a++) {
-                const char *src = kbase + (unsigned long long)rows[16 * a + i16] * 16;
-                if constexpr (DP == 64) {
-                    if (has_group(0)) {
-                        const u2 x = *(const u2 *)(src + 8 * g);
-                        kc[b][a][0] = x[0], kc[b][a][1] = x[1];
-                    }
-                } else {
-#pragma unroll
-                    for (int u = 0; u < KS / 4; u++)
-                        if (has_group(u)) {
-                            const u4 x = *(const u4 *)(src + 64 * u + 16 * g);
-#pragma unroll
-                            for (int w = 0; w < 4; w++) kc[b][a][4 * u + w] = x[w];
-                        }
-                }
-            }
-        };
-        auto load_value_codes = [&](const uint32_t *rows, int b) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const char *src = vbase + (unsigned long long)rows[16 * (j / 4) + 4 * g + j % 4] * 16;
-#pragma unroll
-                for (int vh = 0; vh < VH; vh++) {
-                    const char *from = src + (FULL ? 64 * vh + VE / 2 * i16 : min(64 * vh + VE / 2 * i16, 16 * groups - VE / 2));
-                    vc[b][j][vh] = VE == 8 ? *(const uint32_t *)from : *(const uint16_t *)from;
-                }
-            }
-        };
         auto load_keys = [&](const uint32_t *rows) {
 #pragma unroll
             for (int a = 0; a < 2; a++) {
@@ -303,64 +242,239 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                 }
             }
         };
-        const uint32_t key_turn = mx_turn(DP == 64 ? g / 2 : g), value_turn = mx_turn(DP == 64 ? i16 / 8 : i16 / 4);
         auto hand_over = [&]() {   // what lanes of this wave wrote to LDS is there for the others of it
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         };
 
-        if (wave < blocks) {
-            if constexpr (MX) {
-                // places two steps of 64 keys ahead, scales one
-                list(0)[lane] = row_of(p, entry);
-                load_scales();
-                if (wave + 2 * NW < blocks) entry = entry_of(wave + 2 * NW);
-                hand_over();
-                load_key_codes(list(0), 0);
-                load_value_codes(list(0), 0);
-                if (wave + NW < blocks) {
-                    load_key_codes(list(0) + 32, 1);
-                    load_value_codes(list(0) + 32, 1);
+        if constexpr (MX) {
+            // Keys and values are codes.  A lane's of a key are the groups g and 4 + g (half of one at rows of two), which lie side by side: the
+            // order of dims in the first product is theirs.  Of a value a lane has the same dims as above.  While a wave uses 32 keys the next
+            // 32 are on their way (a second set of registers for 64 brings nothing: what bounds a long call is how fast
+            // workgroups that each stream their own blocks are served, 6.0 TB/s; a fourth workgroup a CU in their place lets
+            // 64 contexts of 1024 take 20.0 us in place of 24.2), and the scales and places of the step behind it; the table's entries two steps
+            // ahead.  None of this stands behind a condition, for which the compiler would wait for all of it: past the end
+            // every lane asks for the last key again, which no row sees there.
+            typedef unsigned long long u64;
+            constexpr int GW = DP > 128 ? 2 : 1;           // words of a row's scales
+            const int groups = mx_groups(dim);
+            auto has_group = [&](int u) { return FULL || (DP == 64 ? g / 2 : 4 * u + g) < groups; };
+            // the wave's lists, which lie where its sums go at the end: where rows stand, and their scales
+            u64 *const places = (u64 *)(join + wave * 16 * OD);
+            uint32_t *const scales = (uint32_t *)(places + 2 * 64);
+            static_assert(2 * 64 * 8 + 2 * 2 * GW * 64 * 4 <= 16 * OD * 4, "");
+            auto scales_at = [&](int turn, int kv, int word) { return scales + ((turn * 2 + kv) * GW + word) * 64; };
+            const uint32_t value_turn = mx_turn(DP == 64 ? i16 / 8 : i16 / 4);
+            const char *const key_base = kbase + (DP == 64 ? 8 : 16) * g;
+            const char *const value_base = vbase + (FULL ? VE / 2 * i16 : min(VE / 2 * i16, 16 * groups - VE / 2));
+            const int value_step = FULL ? 64 : min(64, 16 * groups - VE / 2 - min(VE / 2 * i16, 16 * groups - VE / 2));   // to a lane's second eight dims
+
+            float c = p.c;                                 // (in a vector register, not asked for again at every step)
+            asm("" : "+v"(c));
+
+            struct Scales {
+                uint32_t word[2][GW];
+            };
+            // (In 64 bits throughout: of a 32-bit product and sum the compiler takes the upper half from any register, and waits for
+            // what is on its way there.)
+            auto entry_of = [&](int n) { return key_entry<true>(p, q, table, min(begin + n * 64 + lane, end - 1)); };
+            auto block_of = [&](Entry e) { return (u64)(e.block < (uint32_t)p.blocks ? e.block : 0); };
+            auto place_of = [&](Entry e) { return (block_of(e) * p.block_step + (u64)e.slot * p.slot_step) * 16; };
+            auto load_scales = [&](Entry e) {
+                Scales x;
+                const u64 at = (block_of(e) * p.scale_block + (u64)e.slot * p.scale_slot) * (DP / 32);
+#pragma unroll
+                for (int kv = 0; kv < 2; kv++) {
+                    const char *from = (const char *)(kv ? p.v_scales : p.k_scales) + (long long)h * p.scale_head + at;
+                    if constexpr (DP == 64) {
+                        x.word[kv][0] = *(const uint16_t *)from;
+                    } else if constexpr (DP == 128) {
+                        x.word[kv][0] = *(const uint32_t *)from;
+                    } else {
+                        const u2 y = *(const u2 *)from;
+                        x.word[kv][0] = y[0], x.word[kv][GW - 1] = y[1];
+                    }
                 }
-                enter_scales(0);
-                if (wave + 2 * NW < blocks) {
-                    next = row_of(p, entry);
-                    load_scales();
-                    if (wave + 4 * NW < blocks) entry = entry_of(wave + 4 * NW);
-                }
-                hand_over();
-            } else {
-                list(0)[lane] = next;
-                hand_over();
-                load_keys(list(0));
-                load_values(list(0));
-                if (wave + 2 * NW < blocks) next = look_up(wave + 2 * NW);
+                return x;
+            };
+            auto enter = [&](int turn, u64 place, const Scales &x) {
+                places[turn * 64 + lane] = place;
+#pragma unroll
+                for (int kv = 0; kv < 2; kv++)
+#pragma unroll
+                    for (int w = 0; w < GW; w++) scales_at(turn, kv, w)[lane] = x.word[kv][w];
+            };
+            uint32_t kc[2][KS], vc[8][VH];
+            if constexpr (!FULL) {
+#pragma unroll
+                for (int a = 0; a < 2; a++)
+#pragma unroll
+                    for (int s = 0; s < KS; s++) kc[a][s] = 0u;
             }
+            auto load_key_codes = [&](const u64 *rows, uint32_t (&to)[2][KS]) {
+#pragma unroll
+                for (int a = 0; a < 2; a++) {
+                    const char *src = key_base + rows[16 * a + i16];
+                    if constexpr (DP == 64) {
+                        if (has_group(0)) {
+                            const u2 x = *(const u2 *)src;
+                            to[a][0] = x[0], to[a][1] = x[1];
+                        }
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < KS / 4; u++)
+                            if (has_group(u)) {
+                                const u4 x = *(const u4 *)(src + 64 * u);
+#pragma unroll
+                                for (int w = 0; w < 4; w++) to[a][4 * u + w] = x[w];
+                            }
+                    }
+                }
+            };
+            auto load_value_codes = [&](const u64 *rows, uint32_t (&to)[8][VH]) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const char *src = value_base + rows[16 * (j / 4) + 4 * g + j % 4];
+#pragma unroll
+                    for (int vh = 0; vh < VH; vh++) to[j][vh] = VE == 8 ? *(const uint32_t *)(src + vh * value_step) : *(const uint16_t *)src;
+                }
+            };
+
+            if (wave < blocks) {
+                Entry entry = entry_of(wave), after = entry_of(wave + NW);
+                Scales these = load_scales(entry), next_scales = load_scales(after);
+                enter(0, place_of(entry), these);
+                u64 next_place = place_of(after);
+                entry = entry_of(wave + 2 * NW);
+                hand_over();
+                load_key_codes(places, kc);
+                asm volatile("" ::: "memory");     // (in the order of the loop's: its waits count from either)
+                load_value_codes(places, vc);
+                asm volatile("" ::: "memory");
+                int turn = 0;
+                for (int n = wave; n < blocks; n += NW, turn ^= 1) {
+                    enter(turn ^ 1, next_place, next_scales);
+                    next_place = place_of(entry);
+                    next_scales = load_scales(entry);
+                    entry = entry_of(n + 3 * NW);
+                    hand_over();
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        const int v0 = begin + n * 64 + half * 32;
+                        const u64 *rows = half ? places + (turn ^ 1) * 64 : places + turn * 64 + 32;
+                        // S^T
+                        f4 s[RT][2];
+#pragma unroll
+                        for (int a = 0; a < 2; a++)
+#pragma unroll
+                            for (int u = 0; u < (KS + 3) / 4; u++) {
+                                // (a lane without a group has zeros, of which no scale must make anything else)
+                                uint32_t scale = (uint32_t)((const unsigned char *)scales_at(turn, 0, u))[4 * (32 * half + 16 * a + i16) + (DP == 64 ? g / 2 : g)] << 23;
+                                if (!has_group(u)) scale = 127u << 23;
+#pragma unroll
+                                for (int x = 4 * u; x < KS && x < 4 * u + 4; x++) {
+                                    const e8 key = __builtin_bit_cast(e8, mx_values<E>(kc[a][x], scale));
+#pragma unroll
+                                    for (int rt = 0; rt < RT; rt++) s[rt][a] = mfma16(key, qf[rt][x], x == 0 ? (f4){0.0f, 0.0f, 0.0f, 0.0f} : s[rt][a]);
+                                }
+                            }
+                        load_key_codes(rows, kc);
+                        // what a row does not see
+                        if (v0 + 32 > end || (q.t0 != q.t1 && !all_see(p, q, v0, v0 + 32, q.position + q.t0, q.position + q.t1))) {
+#pragma unroll
+                            for (int a = 0; a < 2; a++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++)
+#pragma unroll
+                                    for (int rt = 0; rt < RT; rt++)
+                                        if (!my[rt].sees(v0 + 16 * a + 4 * g + e)) s[rt][a][e] = kNone;
+                        }
+                        e8 pe[RT];
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++) {
+                            float top = max2(max2(max2(s[rt][0][0], s[rt][0][1]), max2(s[rt][0][2], s[rt][0][3])),
+                                             max2(max2(s[rt][1][0], s[rt][1][1]), max2(s[rt][1][2], s[rt][1][3])));
+                            f2 two = swap_halves(top);
+                            two = swap_quarters(max2(two[0], two[1]));
+                            top = max2(two[0], two[1]) * c;
+                            if (__ballot(top > m[rt] + Shares<E>::most)) {
+                                const float up = fmaxf(m[rt], top - Shares<E>::lift);
+                                const float down = __builtin_amdgcn_exp2f(m[rt] - reference(up));
+                                m[rt] = up;
+                                l[rt] *= down;
+#pragma unroll
+                                for (int vh = 0; vh < VH; vh++)
+#pragma unroll
+                                    for (int t = 0; t < VE; t++) o[rt][vh][t] *= down;
+                            }
+                            const float ref = reference(m[rt]);
+                            f8 pr;
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                pr[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][j / 4][j % 4], c, -ref));
+                                l[rt] += pr[j];
+                            }
+                            pe[rt] = __builtin_convertvector(pr, e8);
+                        }
+                        // the operands of V: 8 keys of this lane's group, one dim each
+#pragma unroll
+                        for (int vh = 0; vh < VH; vh++) {
+                            uint32_t scale[8];
+#pragma unroll
+                            for (int j = 0; j < 8; j += 4) {
+                                const u4 words = *(const u4 *)(scales_at(turn, 1, vh) + 32 * half + 4 * j + 4 * g);
+#pragma unroll
+                                for (int k = 0; k < 4; k++) scale[j + k] = mx_scale(words[k], value_turn);
+                            }
+                            auto two_dims = [&](auto which) {
+                                constexpr int W = decltype(which)::value;
+                                u4 even, odd;
+#pragma unroll
+                                for (int j = 0; j < 4; j++) {
+                                    const uint32_t a = mx_pair<E, W>(vc[2 * j][vh], scale[2 * j]), b = mx_pair<E, W>(vc[2 * j + 1][vh], scale[2 * j + 1]);
+                                    even[j] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+                                    odd[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+                                }
+#pragma unroll
+                                for (int rt = 0; rt < RT; rt++) {
+                                    o[rt][vh][2 * W] = mfma16(__builtin_bit_cast(e8, even), pe[rt], o[rt][vh][2 * W]);
+                                    o[rt][vh][2 * W + 1] = mfma16(__builtin_bit_cast(e8, odd), pe[rt], o[rt][vh][2 * W + 1]);
+                                }
+                            };
+                            two_dims(std::integral_constant<int, 0>());
+                            two_dims(std::integral_constant<int, 1>());
+                            if constexpr (VW == 4) {
+                                two_dims(std::integral_constant<int, 2>());
+                                two_dims(std::integral_constant<int, 3>());
+                            }
+                        }
+                        load_value_codes(rows, vc);
+                        asm volatile("" ::: "memory");      // (these are asked for here, not where they are used)
+                    }
+                }
+                hand_over();      // (the lists are read before sums go where they are)
+            }
+        } else if (wave < blocks) {
+            list[wave][0][lane] = next;
+            hand_over();
+            load_keys(list[wave][0]);
+            load_values(list[wave][0]);
+            if (wave + 2 * NW < blocks) next = look_up(wave + 2 * NW);
             int turn = 0;
             for (int n = wave; n < blocks; n += 2 * NW, turn ^= 1) {
                 if (n + 2 * NW < blocks) {
-                    list(turn ^ 1)[lane] = next;
-                    if constexpr (MX) enter_scales(turn ^ 1);
+                    list[wave][turn ^ 1][lane] = next;
                     hand_over();
-                    if (n + 4 * NW < blocks) {
-                        if constexpr (MX) {
-                            next = row_of(p, entry);
-                            load_scales();
-                            if (n + 6 * NW < blocks) entry = entry_of(n + 6 * NW);
-                        } else {
-                            next = look_up(n + 4 * NW);
-                        }
-                    }
+                    if (n + 4 * NW < blocks) next = look_up(n + 4 * NW);
                 }
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     const int block = n + half * NW, v0 = begin + block * 32;
                     if (half == 1 && block >= blocks) break;
-                    // the rows of this wave's next block (MX: the one behind it, whose operands go where this one's are)
-                    const uint32_t *rows = MX ? list(turn ^ 1) + 32 * half : half ? list(turn ^ 1) : list(turn) + 32;
-                    const bool load = block + AHEAD * NW < blocks;
-                    const int b = MX ? half : 0;
+                    // the rows of this wave's next block
+                    const uint32_t *rows = half ? list[wave][turn ^ 1] : list[wave][turn] + 32;
+                    const bool load = block + NW < blocks;
                     // S^T
                     f4 s[RT][2];
 #pragma unroll
@@ -368,27 +482,10 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
 #pragma unroll
                         for (int a = 0; a < 2; a++) {
                             s[rt][a] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-                            if constexpr (!MX) {
 #pragma unroll
-                                for (int x = 0; x < KS; x++) s[rt][a] = mfma16(__builtin_bit_cast(e8, kr[a][x]), qf[rt][x], s[rt][a]);
-                            }
+                            for (int x = 0; x < KS; x++) s[rt][a] = mfma16(__builtin_bit_cast(e8, kr[a][x]), qf[rt][x], s[rt][a]);
                         }
-                    if constexpr (MX) {
-#pragma unroll
-                        for (int a = 0; a < 2; a++)
-#pragma unroll
-                            for (int x = 0; x < KS; x++) {
-                                // (a lane without a group has zeros, of which no scale must make anything else)
-                                uint32_t scale = mx_scale(key_scales(turn, x / 4)[32 * half + 16 * a + i16], key_turn);
-                                if (!has_group(x / 4)) scale = 127u << 23;
-                                const e8 keys8 = __builtin_bit_cast(e8, mx_values<E>(kc[b][a][x], scale));
-#pragma unroll
-                                for (int rt = 0; rt < RT; rt++) s[rt][a] = mfma16(keys8, qf[rt][x], s[rt][a]);
-                            }
-                        if (load) load_key_codes(rows, b);
-                    } else {
-                        if (load) load_keys(rows);
-                    }
+                    if (load) load_keys(rows);
                     // what a row does not see
                     const bool tail = v0 + 32 > end;
                     const bool mixed = q.t0 != q.t1 && !all_see(p, q, v0, v0 + 32, q.position + q.t0, q.position + q.t1);
@@ -434,23 +531,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                     }
                     // the operands of V: 8 keys of this lane's group, one dim each
 #pragma unroll
-                    for (int vh = 0; vh < VH; vh++) {
-                        if constexpr (MX) {
-#pragma unroll
-                            for (int j0 = 0; j0 < 8; j0 += 4) {
-                                const u4 words = *(const u4 *)(value_scales(turn, vh) + 32 * half + 4 * j0 + 4 * g);
-#pragma unroll
-                                for (int j = 0; j < 4; j++) {
-                                    const uint32_t scale = mx_scale(words[j], value_turn), codes = vc[b][j0 + j][vh];
-                                    vr[j0 + j][vh][0] = mx_pair<E, 0>(codes, scale);
-                                    vr[j0 + j][vh][1] = mx_pair<E, 1>(codes, scale);
-                                    if constexpr (VW == 4) {
-                                        vr[j0 + j][vh][2] = mx_pair<E, 2>(codes, scale);
-                                        vr[j0 + j][vh][VW - 1] = mx_pair<E, 3>(codes, scale);
-                                    }
-                                }
-                            }
-                        }
+                    for (int vh = 0; vh < VH; vh++)
 #pragma unroll
                         for (int w = 0; w < VW; w++) {
                             u4 even, odd;
@@ -465,17 +546,10 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                                 o[rt][vh][2 * w + 1] = mfma16(__builtin_bit_cast(e8, odd), pe[rt], o[rt][vh][2 * w + 1]);
                             }
                         }
-                    }
-                    if constexpr (MX) {
-                        if (load) load_value_codes(rows, b);
-                    } else {
-                        if (load) load_values(rows);
-                    }
+                    if (load) load_values(rows);
                 }
             }
         }
-
-        if constexpr (MX) hand_over();      // (the lists are read before sums go where they are)
 
         // the four waves, 16 rows at a time
         const bool whole = parts == 1 && !SHARED;
@@ -500,7 +574,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : (RT == 1 ? 3 : 2) + 
                             *(f4 *)(to + 128 * vh + VE * (4 * g + e) + t) = (f4){o[rt][vh][t][e], o[rt][vh][t + 1][e], o[rt][vh][t + 2][e], o[rt][vh][t + 3][e]};
             }
             __syncthreads();
-            for (int x = threadIdx.x; x < 16 * (DP / 4); x += 64 * NW) {
+            for (int x = MX ? thread : (int)threadIdx.x; x < 16 * (DP / 4); x += 64 * NW) {
                 const int r = x / (DP / 4), d = x % (DP / 4) * 4, row = 16 * rt + r;
                 if (row >= q.rows || d >= dim) continue;
                 float top = kNone, sum = 0.0f, ms[NW];

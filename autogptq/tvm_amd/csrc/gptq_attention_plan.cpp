@@ -65,9 +65,6 @@ int few_operands(long long rows, int dim)
     if (rows <= 32 && dim <= 128) return 2;
     return 0;
 }
-// workgroups of the few-rows kernel that a CU holds (registers)
-int few_resident(int rt, int dim) { return dim > 128 ? 1 : (rt == 1 ? 3 : 2) + (dim <= 64); }
-
 // Parts of tiles that see `keys` keys: enough that `busy` workgroups become `want`, none of fewer than 256 keys.
 void divide(Division &d, long long want, long long busy, long long keys, long long most_parts)
 {
@@ -91,7 +88,8 @@ struct Plan {
     size_t prefix_rows = 0, own_rows = 0, bytes = 0;     // rows of the parts in the workspace
 };
 
-int plan(const gptq_hip_attention &a, Plan &pl)
+// mx: the cache is held in MXFP4
+int plan(const gptq_hip_attention &a, bool mx, Plan &pl)
 {
     const long long group = a.heads / a.cache.heads, T = a.tokens, B = a.requests, H = a.cache.heads;
     const long long all = T * a.heads, row = a.cache.dim * 4 + 8;
@@ -124,7 +122,7 @@ int plan(const gptq_hip_attention &a, Plan &pl)
         if (most > 1ll << 30) return GPTQ_HIP_ERR_UNSUPPORTED;
         d.most_units = (int)std::min((1ll << 30) / most, 1ll << 20);
         const long long units = (d.tiles + 0ll) * std::max(1ll, ceil_div(keys, 256));
-        d.team = (int)std::max(1ll, std::min(256ll * few_resident(d.rt, a.cache.dim) / H, units));
+        d.team = (int)std::max(1ll, std::min(256ll * few_resident(d.rt, a.cache.dim, mx) / H, units));
         if (d.team * H > (long long)(kAttentionCounters / 4)) return GPTQ_HIP_ERR_UNSUPPORTED;
         pl.own_rows = (size_t)(2 * d.team * H * d.rows());
     } else {
@@ -161,7 +159,7 @@ int check(const gptq_hip_attention *a, int rc)
 int attend(const gptq_hip_attention *a, const gptq_hip_cache_mx *mx, void *workspace, size_t workspace_bytes, void *stream)
 {
     Plan pl;
-    int rc = plan(*a, pl);
+    int rc = plan(*a, mx != nullptr, pl);
     if (rc != GPTQ_HIP_OK) return rc;
     if (pl.bytes && (!workspace || (uintptr_t)workspace % 16 != 0 || workspace_bytes < pl.bytes)) return GPTQ_HIP_ERR_WORKSPACE;
 
@@ -190,6 +188,8 @@ int attend(const gptq_hip_attention *a, const gptq_hip_cache_mx *mx, void *works
     p.c = a->scale * 1.44269504088896340736f;
     if ((long long)p.group * (p.group + kTileRows) < 65536) p.group_magic = 65535u / (uint32_t)p.group + 1u;
     p.block_shift = c.block_size & (c.block_size - 1) ? -1 : __builtin_ctz((unsigned)c.block_size);
+    while (p.block_bits < 31 && 1ll << p.block_bits < c.block_size) p.block_bits++;
+    p.block_magic = (uint32_t)(((1ull << (29 + p.block_bits)) + (unsigned)c.block_size - 1) / (unsigned)c.block_size);
     auto launch = [&](const Division &d) {
         p.tiles = d.tiles, p.splits = d.splits, p.chunk = d.chunk, p.team = d.team, p.most_units = d.most_units;
         if (d.rt) return mx ? launch_attention_few_mx(p, c.type, d.rt, stream) : launch_attention_few(p, c.type, d.rt, stream);
@@ -224,7 +224,7 @@ gptq_hip_attention with_shape_of(const gptq_hip_attention &a, const gptq_hip_cac
 extern "C" size_t gptq_hip_attention_workspace_bytes(const gptq_hip_attention *a)
 {
     gptq::Plan pl;
-    if (!a || gptq::check(a, gptq::check_cache(&a->cache)) != GPTQ_HIP_OK || a->tokens == 0 || gptq::plan(*a, pl) != GPTQ_HIP_OK) return 0;
+    if (!a || gptq::check(a, gptq::check_cache(&a->cache)) != GPTQ_HIP_OK || a->tokens == 0 || gptq::plan(*a, false, pl) != GPTQ_HIP_OK) return 0;
     return pl.bytes;
 }
 
@@ -241,7 +241,7 @@ extern "C" size_t gptq_hip_attention_mx_workspace_bytes(const gptq_hip_cache_mx 
     if (!cache || !given) return 0;
     const gptq_hip_attention a = gptq::with_shape_of(*given, *cache);
     gptq::Plan pl;
-    if (gptq::check(&a, gptq::check_cache_mx(cache)) != GPTQ_HIP_OK || a.tokens == 0 || gptq::plan(a, pl) != GPTQ_HIP_OK) return 0;
+    if (gptq::check(&a, gptq::check_cache_mx(cache)) != GPTQ_HIP_OK || a.tokens == 0 || gptq::plan(a, true, pl) != GPTQ_HIP_OK) return 0;
     return pl.bytes;
 }
 

@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
     // Rows of tile n for the requests: four tiles at a time, one a wave.  A thread's rows of a tile stand side by side.
     auto look_up = [&](int n) {
         const int i = min(begin + min(n, tiles - 1) * KT + lane, end - 1);
-        if constexpr (MX) return key_entry(p, q, table, i);
+        if constexpr (MX) return key_entry<true>(p, q, table, i);
         else return key_row(p, q, table, i);
     };
     auto enter = [&](int n, auto place) {

@@ -104,10 +104,11 @@ int plan(const gptq_hip_attention &a, bool mx, Plan &pl)
     // A short prefix stands in front of every request's keys instead of taking a launch of its own, which costs 4 us and less
     // as the tiles read it again (32 heads in groups of 4, dim 128): 8 requests behind 1000 keys 11.3 us against 15.4, 16
     // behind 1000 14.1 / 17.5, 64 behind 250 17.1 / 22.0, 8 behind 4000 17.2 / 17.8, 16 behind 2000 21.5 / 18.0, 32 behind 1000
-    // 23.8 / 18.9.
+    // 23.8 / 18.9.  A cache in MXFP4, whose re-reads are a quarter of the bytes, has it there a little longer: 16 behind 2000 14.2 / 20.5,
+    // behind 4000 18.3 / 21.7, 64 behind 1000 21.9 / 27.0, 8 behind 16000 30.3 / 28.8.
     const bool alone = B == 1 && T * group <= d.rows();      // no other reader
     pl.prefix = a.prefix_length > 0 &&
-                !(d.rt && (alone || (long long)d.tiles * a.prefix_length * H * a.cache.dim * 4 <= 256ll << 20));
+                !(d.rt && (alone || (long long)d.tiles * a.prefix_length * H * a.cache.dim * 4 <= (mx ? 384ll : 256ll) << 20));
     if (pl.prefix) {
         Division &s = pl.shared;
         s.rt = few_operands(T * group, a.cache.dim);

@@ -218,16 +218,18 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
         }
         return x;
     };
-    auto put = [&](const Coded &x, uint32_t to, int twist) {
+    // (words [w0, w1) of a part)
+    auto put = [&](const Coded &x, int w0, int w1, uint32_t to, int twist) {
         const int thread = this_thread(), code_row = thread / 4, code_part = thread % 4;
         const int turned = (twist * code_row) & (CH - 1);
         const uint32_t row = to + code_row * (DP * 2) + (((code_part * DW) ^ turned) * 16);
 #pragma unroll
         for (int w = 0; w < DW; w++)
-            *(__attribute__((address_space(3))) u4 *)(uintptr_t)(row ^ (w * 16)) = mx_values<E>(x.codes[w], (w < 4 ? x.scales : x.scales >> 8) << 23);
+            if (w >= w0 && w < w1)
+                *(__attribute__((address_space(3))) u4 *)(uintptr_t)(row ^ (w * 16)) = mx_values<E>(x.codes[w], (w < 4 ? x.scales : x.scales >> 8) << 23);
     };
-    auto put_keys = [&](const Coded &x, int buf) { put(x, lds + buf * TILE, 1); };
-    auto put_values = [&](const Coded &x, int buf) { put(x, lds + (2 + buf) * TILE, 2); };
+    auto put_keys = [&](const Coded &x, int buf, int w0 = 0, int w1 = 8) { put(x, w0, w1, lds + buf * TILE, 1); };
+    auto put_values = [&](const Coded &x, int buf, int w0 = 0, int w1 = 8) { put(x, w0, w1, lds + (2 + buf) * TILE, 2); };
     auto meet_lds = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
     float m = kNone, l = 0.0f;
@@ -268,8 +270,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
                 for (int a = 0; a < KA; a++) s[a] = mfma32(__builtin_bit_cast(e8, kf[x - x0][a]), qf[x], s[a]);
         }
     };
-    // softmax of tile n, whose scores are in s, and its products with the values in the buffer BUF; then the next scores
-    auto sum = [&](int n, auto buf) {
+    // softmax of tile n, whose scores are in s, and its products with the values in the buffer BUF; then the next scores.  `beside`
+    // is called between the products, four times.
+    auto sum = [&](int n, auto buf, auto beside) {
         constexpr int BUF = decltype(buf)::value * TILE;
         u2 vf[PX][DT][2];
         auto read_values = [&](int x) {
@@ -323,6 +326,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
                 const u4 y = {vf[x][dt][0][0], vf[x][dt][0][1], vf[x][dt][1][0], vf[x][dt][1][1]};
                 o[dt] = mfma32(__builtin_bit_cast(e8, y), pe, o[dt]);
             }
+            beside(x);
         }
         scores(std::integral_constant<int, 1 - decltype(buf)::value>());
     };
@@ -342,18 +346,27 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
             meet_lds();
             if (works) scores(std::integral_constant<int, 0>());
             meet_lds();
-            // tile n: the keys of n + 2 and the values of n + 1, which came while tile n - 1 was summed, go where those of n and n - 1 were
+            // Tile n: the keys of n + 2 and the values of n + 1, which came while tile n - 1 was summed, go where those of n and n - 1 were.
+            // They are turned into values between the products: the matrix pipes are busy then.
             auto step = [&](int n, auto buf) {
                 constexpr int BUF = decltype(buf)::value;
-                if (n + 2 < tiles) put_keys(keys, BUF);
-                if (n + 1 < tiles) put_values(values, 1 - BUF);
-                if (n + 3 < tiles) keys = fetch(n + 3, kbase, p.k_scales);
-                if (n + 2 < tiles) values = fetch(n + 2, vbase, p.v_scales);
                 if ((n & 3) == 0) {      // (the places of tile n + 4 are read a tile from here at the earliest)
                     enter(n + 4 + wave, next);
                     next = look_up(n + 8 + wave);
                 }
-                if (works) sum(n, buf);
+                // (past the end: the last key's row, into buffers that nobody reads)
+                auto stage = [&](int x) {
+                    static_assert(PX == 4, "");
+                    if (x < 2) put_keys(keys, BUF, x * DW / 2, (x + 1) * DW / 2);
+                    else put_values(values, 1 - BUF, (x - 2) * DW / 2, (x - 1) * DW / 2);
+                    if (x == 1) keys = fetch(n + 3, kbase, p.k_scales);
+                    if (x == 3) values = fetch(n + 2, vbase, p.v_scales);
+                };
+                if (works) {
+                    sum(n, buf, stage);
+                } else {
+                    for (int x = 0; x < 4; x++) stage(x);
+                }
                 meet_lds();
             };
             for (int n = 0; n < tiles; n += 2) {
@@ -388,7 +401,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
                 enter(n + 4 + wave, next);
                 next = look_up(n + 8 + wave);
             }
-            if (works) sum(n, buf);
+            if (works) sum(n, buf, [](int) {});
             meet();
         };
         for (int n = 0; n < tiles; n += 2) {
@@ -401,8 +414,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
     const bool whole = parts == 1 && p.prefix_parts == 0 && !p.shared;
     const long long all = (long long)p.tokens * p.heads;
     float *stats = p.shared ? p.stats : p.own_stats, *outs = p.shared ? p.parts : p.own_parts;
-    if (r < q.rows) {
-        const long long at = out_row(p, q, h, r);
+    const int row = MX ? 32 * wave + (this_thread() & 31) : r;
+    if (row < q.rows) {
+        const long long at = out_row(p, q, h, row);
         const long long slot = split * all;
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
         if (!whole && hh == 0) put_stats<false>(stats + 2 * (slot + at), m, l);

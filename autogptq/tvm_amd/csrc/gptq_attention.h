@@ -66,6 +66,7 @@ struct AttentionParams {
     // the excess of the product, x times less than block_size, stays below 2^(29 + bits)
     uint32_t block_magic;
     int block_bits;
+    int unit_bits;           // few-rows kernel on a cache in MXFP4: log2 of the keys of a unit
 };
 
 // x / group for the rows of a tile, counted from its first token's

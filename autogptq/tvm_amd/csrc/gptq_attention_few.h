@@ -39,7 +39,7 @@ struct Requests {
     int units, keys;       // of a tile: units, and the keys of one
     int total;             // units of all its tiles
 };
-template <int R>
+template <int R, bool MX>
 __device__ __forceinline__ Requests look_at(const AttentionParams &p, int base)
 {
     // what the tensors say is cut to what the other arguments allow: wrong lengths give wrong sums, not wrong addresses
@@ -53,7 +53,7 @@ __device__ __forceinline__ Requests look_at(const AttentionParams &p, int base)
     const int hi = max(min(r.context, held_keys(p)), 0);
     const int lo = p.window > 0 ? min(max(r.context - r.count - p.window + 1, 0), hi) : 0;
     const int seen = p.front + min(p.sinks, lo) + hi - lo;
-    r.units = min(max(1, (seen + kFewUnit - 1) / kFewUnit), p.most_units);
+    r.units = min(max(1, MX ? (seen + (1 << p.unit_bits) - 1) >> p.unit_bits : (seen + kFewUnit - 1) / kFewUnit), p.most_units);
     r.keys = max(32, ((seen + r.units - 1) / r.units + 31) / 32 * 32);
     r.total = (int)(((uint32_t)r.count * (uint32_t)p.group + R - 1) / R) * r.units;
     return r;
@@ -97,11 +97,11 @@ __global__ __launch_bounds__(64 * kFewWaves, few_resident(RT, DP, MX)) void atte
     int at = 0, stop = 1, share = 1, base = 0, before = 0, upto = 0;
     Requests look = {};
     if (!SHARED) {
-        look = look_at<R>(given, 0);
+        look = look_at<R, MX>(given, 0);
         clear_rest(given, given.starts[0], given.starts[given.requests], blockIdx.x * (64ll * kFewWaves) + threadIdx.x, gridDim.x * (64ll * kFewWaves));
         upto = sum_upto(look.total);
         int total = __builtin_amdgcn_readlane(upto, 63);
-        for (int b = 64; b < given.requests; b += 64) total += __builtin_amdgcn_readlane(sum_upto(look_at<R>(given, b).total), 63);
+        for (int b = 64; b < given.requests; b += 64) total += __builtin_amdgcn_readlane(sum_upto(look_at<R, MX>(given, b).total), 63);
         // (Whole tiles of two units rather than their halves, once every CU has a workgroup: the second unit costs less than
         // the join.  32 contexts of 300 tokens, 8 heads: 12.0 us, in halves 13.9; 4 of 512, where CUs are left, 10.4 in halves.)
         share = max((total + given.team - 1) / given.team, total * given.kv_heads > 256 && total <= 2 * given.requests ? 2 : 1);
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_resident(RT, DP, MX)) void atte
             while (at - before >= __builtin_amdgcn_readlane(upto, 63)) {
                 before += __builtin_amdgcn_readlane(upto, 63);
                 base += 64;
-                look = look_at<R>(p, base);
+                look = look_at<R, MX>(p, base);
                 upto = sum_upto(look.total);
             }
             const int owner = __popcll(__ballot(upto <= at - before));
@@ -168,8 +168,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_resident(RT, DP, MX)) void atte
         const int32_t *table = p.tables + (long long)q.b * p.table_stride;
         // blocks of 32 keys: a wave takes every fourth, and looks two of its own up at a time, one a half of its lanes (past
         // the end: the last key's row again)
-        // (MX: blocks of 64, so that what a wave asks for at a time lies together)
-        const int blocks = MX ? (end - begin + 63) / 64 : (end - begin + 31) / 32, busy = min(blocks, NW);   // ... waves that have keys
+        const int blocks = (end - begin + 31) / 32, busy = min(blocks, NW);   // ... waves that have keys
         auto look_up = [&](int n) { return key_row(p, q, table, min(begin + (n + (lane >> 5) * NW) * 32 + (lane & 31), end - 1)); };
         uint32_t next = 0;
         if (!MX && wave < blocks) next = look_up(wave);
@@ -278,7 +277,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_resident(RT, DP, MX)) void atte
             };
             // (In 64 bits throughout: of a 32-bit product and sum the compiler takes the upper half from any register, and waits for
             // what is on its way there.)
-            auto entry_of = [&](int n) { return key_entry<true>(p, q, table, min(begin + n * 64 + lane, end - 1)); };
+            auto entry_of = [&](int n) { return key_entry<true>(p, q, table, min(begin + (n + (lane >> 5) * NW) * 32 + (lane & 31), end - 1)); };
             auto block_of = [&](Entry e) { return (u64)(e.block < (uint32_t)p.blocks ? e.block : 0); };
             auto place_of = [&](Entry e) { return (block_of(e) * p.block_step + (u64)e.slot * p.slot_step) * 16; };
             auto load_scales = [&](Entry e) {
@@ -298,8 +297,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_resident(RT, DP, MX)) void atte
                 }
                 return x;
             };
-            auto enter = [&](int turn, u64 place, const Scales &x) {
-                places[turn * 64 + lane] = place;
+            auto enter_scales = [&](int turn, const Scales &x) {
 #pragma unroll
                 for (int kv = 0; kv < 2; kv++)
 #pragma unroll
@@ -342,26 +340,30 @@ __global__ __launch_bounds__(64 * kFewWaves, few_resident(RT, DP, MX)) void atte
             };
 
             if (wave < blocks) {
-                Entry entry = entry_of(wave), after = entry_of(wave + NW);
+                Entry entry = entry_of(wave), after = entry_of(wave + 2 * NW);
                 Scales these = load_scales(entry), next_scales = load_scales(after);
-                enter(0, place_of(entry), these);
+                places[lane] = place_of(entry);
                 u64 next_place = place_of(after);
-                entry = entry_of(wave + 2 * NW);
+                entry = entry_of(wave + 4 * NW);
                 hand_over();
                 load_key_codes(places, kc);
                 asm volatile("" ::: "memory");     // (in the order of the loop's: its waits count from either)
                 load_value_codes(places, vc);
                 asm volatile("" ::: "memory");
+                enter_scales(0, these);
+                hand_over();
                 int turn = 0;
-                for (int n = wave; n < blocks; n += NW, turn ^= 1) {
-                    enter(turn ^ 1, next_place, next_scales);
+                for (int n = wave; n < blocks; n += 2 * NW, turn ^= 1) {
+                    places[(turn ^ 1) * 64 + lane] = next_place;
+                    enter_scales(turn ^ 1, next_scales);
                     next_place = place_of(entry);
                     next_scales = load_scales(entry);
-                    entry = entry_of(n + 3 * NW);
+                    entry = entry_of(n + 6 * NW);
                     hand_over();
 #pragma unroll
                     for (int half = 0; half < 2; half++) {
-                        const int v0 = begin + n * 64 + half * 32;
+                        const int v0 = begin + (n + half * NW) * 32;
+                        if (half == 1 && v0 >= end) goto summed;       // (not around the loop's head: its waits count on both halves)
                         const u64 *rows = half ? places + (turn ^ 1) * 64 : places + turn * 64 + 32;
                         // S^T
                         f4 s[RT][2];
@@ -453,6 +455,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_resident(RT, DP, MX)) void atte
                         asm volatile("" ::: "memory");      // (these are asked for here, not where they are used)
                     }
                 }
+            summed:
                 hand_over();      // (the lists are read before sums go where they are)
             }
         } else if (wave < blocks) {
@@ -611,7 +614,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_resident(RT, DP, MX)) void atte
                 return (long long)((2 * (first + part) + (part == 0)) * p.kv_heads + h) * R + r;
             });
         if (at >= stop) break;
-        look = look_at<R>(p, base);
+        look = look_at<R, MX>(p, base);
         upto = sum_upto(look.total);
         __syncthreads();
     }

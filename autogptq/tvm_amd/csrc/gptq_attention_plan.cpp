@@ -54,7 +54,7 @@ struct Division {
     int rt = 0;        // 16-row operands a wave of the few-rows kernel, 0: the tile kernel
     int tiles = 0;     // of rows: all there can be
     int splits = 1, chunk = 1;          // parts of a tile at most, keys of a part
-    int team = 1, most_units = 1;       // few-rows kernel on own contexts: see there
+    int team = 1, most_units = 1, unit_bits = 8;       // few-rows kernel on own contexts: see there
     int rows() const { return rt ? 16 * rt : kTileRows; }
 };
 
@@ -122,8 +122,12 @@ int plan(const gptq_hip_attention &a, bool mx, Plan &pl)
         const long long most = B * (T * group / d.rows() + 1);    // tiles, whatever the lengths on the GPU say
         if (most > 1ll << 30) return GPTQ_HIP_ERR_UNSUPPORTED;
         d.most_units = (int)std::min((1ll << 30) / most, 1ll << 20);
-        const long long units = (d.tiles + 0ll) * std::max(1ll, ceil_div(keys, 256));
-        d.team = (int)std::max(1ll, std::min(256ll * few_resident(d.rt, a.cache.dim, mx) / H, units));
+        // (MXFP4: up to 512 keys in units of 128 where there are workgroups for all of them, since a wave's second 32 keys wait for memory
+        // once more: 7.5 us for 512, in units of 256 8.0; 2048 9.7 and 8.5, since eight more parts are joined)
+        const long long team = 256ll * few_resident(d.rt, a.cache.dim, mx) / H;
+        if (mx && keys <= 512 && d.tiles * std::max(1ll, ceil_div(keys, 128)) <= team) d.unit_bits = 7;
+        const long long units = (d.tiles + 0ll) * std::max(1ll, ceil_div(keys, 1ll << d.unit_bits));
+        d.team = (int)std::max(1ll, std::min(team, units));
         if (d.team * H > (long long)(kAttentionCounters / 4)) return GPTQ_HIP_ERR_UNSUPPORTED;
         pl.own_rows = (size_t)(2 * d.team * H * d.rows());
     } else {
@@ -192,7 +196,7 @@ int attend(const gptq_hip_attention *a, const gptq_hip_cache_mx *mx, void *works
     while (p.block_bits < 31 && 1ll << p.block_bits < c.block_size) p.block_bits++;
     p.block_magic = (uint32_t)(((1ull << (29 + p.block_bits)) + (unsigned)c.block_size - 1) / (unsigned)c.block_size);
     auto launch = [&](const Division &d) {
-        p.tiles = d.tiles, p.splits = d.splits, p.chunk = d.chunk, p.team = d.team, p.most_units = d.most_units;
+        p.tiles = d.tiles, p.splits = d.splits, p.chunk = d.chunk, p.team = d.team, p.most_units = d.most_units, p.unit_bits = d.unit_bits;
         if (d.rt) return mx ? launch_attention_few_mx(p, c.type, d.rt, stream) : launch_attention_few(p, c.type, d.rt, stream);
         return mx ? launch_attention_tile_mx(p, c.type, stream) : launch_attention_tile(p, c.type, stream);
     };

@@ -72,6 +72,20 @@ __device__ __forceinline__ int sum_upto(int x)
     return x;
 }
 
+// the largest of the lanes' values, none of which is negative
+__device__ __forceinline__ int max_lanes(int x)
+{
+#define GPTQ_MAX(CONTROL, ROWS) x = max(x, __builtin_amdgcn_update_dpp(0, x, CONTROL, ROWS, 0xf, false))
+    GPTQ_MAX(0x111, 0xf);   // as above
+    GPTQ_MAX(0x112, 0xf);
+    GPTQ_MAX(0x114, 0xf);
+    GPTQ_MAX(0x118, 0xf);
+    GPTQ_MAX(0x142, 0xa);
+    GPTQ_MAX(0x143, 0xc);
+#undef GPTQ_MAX
+    return __builtin_amdgcn_readlane(x, 63);
+}
+
 // DP: compiled width, the dims past p.dim do not count; FULL: there are none; RT: 16-row operands a wave holds; SHARED: the parts of a
 // shared prefix; MX: a cache in MXFP4
 template <typename E, int DP, bool FULL, int RT, bool SHARED, bool MX>
@@ -100,8 +114,13 @@ __global__ __launch_bounds__(64 * kFewWaves, few_resident(RT, DP, MX)) void atte
         look = look_at<R, MX>(given, 0);
         clear_rest(given, given.starts[0], given.starts[given.requests], blockIdx.x * (64ll * kFewWaves) + threadIdx.x, gridDim.x * (64ll * kFewWaves));
         upto = sum_upto(look.total);
-        int total = __builtin_amdgcn_readlane(upto, 63);
-        for (int b = 64; b < given.requests; b += 64) total += __builtin_amdgcn_readlane(sum_upto(look_at<R, MX>(given, b).total), 63);
+        int total = __builtin_amdgcn_readlane(upto, 63), most = 0;       // units in all, and of a tile at most
+        if (MX) most = max_lanes(look.units);
+        for (int b = 64; b < given.requests; b += 64) {
+            const Requests x = look_at<R, MX>(given, b);
+            if (MX) most = max(most, max_lanes(x.units));
+            total += __builtin_amdgcn_readlane(sum_upto(x.total), 63);
+        }
         // (Whole tiles of two units rather than their halves, once every CU has a workgroup: the second unit costs less than
         // the join.  32 contexts of 300 tokens, 8 heads: 12.0 us, in halves 13.9; 4 of 512, where CUs are left, 10.4 in halves.)
         share = max((total + given.team - 1) / given.team, total * given.kv_heads > 256 && total <= 2 * given.requests ? 2 : 1);
@@ -111,7 +130,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_resident(RT, DP, MX)) void atte
             // bound, and whole tiles where each CU has two of them.  (8 key/value heads, us with the shortest parts and so: 1
             // context of 32768 29.2 / 17.6, of 8192 12.4 / 11.2; 4 of 32768 38.7 / 33.0, 16 of 8192 34.4 / 31.8; 64 of 1024 19.7 / 16.4.)
             const int tile_units = (total + given.requests - 1) / given.requests;
-            int least = (int)__builtin_sqrtf((float)(total / given.requests) * 0.125f);
+            int least = (int)__builtin_sqrtf((float)most * (1.0f / 6.0f));
             if ((long long)total * given.kv_heads >= 4096 && tile_units >= 8) least = max(least, 8);
             if ((long long)given.requests * given.kv_heads >= 512 && tile_units <= 4) least = max(least, tile_units);
             share = max(share, least);

@@ -190,9 +190,19 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
     // (Taken anew for every use: what follows from the thread would else stand in registers that the kernel does not have.)
     auto this_thread = [&]() {
         int t = threadIdx.x;
-        asm volatile("" : "+v"(t));
+        if constexpr (DP != 128 || DC == 128) asm volatile("" : "+v"(t));
         return t;
     };
+    // Where its part of a row goes, from a tile's beginning: keys in the lower half of the word, values in the upper.  (Dynamic LDS begins at 0,
+    // so that the swizzle is in the low bits of the sum.)
+    auto find_place = [&]() {
+        const int thread = this_thread(), code_row = thread / 4, chunk = thread % 4 * DW;
+        return (uint32_t)(code_row * (DP * 2) + (chunk ^ (code_row & (CH - 1))) * 16) |
+               (uint32_t)(code_row * (DP * 2) + (chunk ^ (2 * code_row & (CH - 1))) * 16) << 16;
+    };
+    static_assert(TILE <= 1 << 16, "");
+    const uint32_t kept_place = MX && DP <= 128 ? find_place() : 0;
+    auto place_of_part = [&]() { return DP <= 128 ? kept_place : find_place(); };
     auto fetch = [&](int n, const char *from, const void *scales) {
         const int thread = this_thread(), code_row = thread / 4, code_part = thread % 4;
         Coded x = {};
@@ -219,17 +229,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
         return x;
     };
     // (words [w0, w1) of a part)
-    auto put = [&](const Coded &x, int w0, int w1, uint32_t to, int twist) {
-        const int thread = this_thread(), code_row = thread / 4, code_part = thread % 4;
-        const int turned = (twist * code_row) & (CH - 1);
-        const uint32_t row = to + code_row * (DP * 2) + (((code_part * DW) ^ turned) * 16);
+    auto put = [&](const Coded &x, int w0, int w1, uint32_t row) {
 #pragma unroll
         for (int w = 0; w < DW; w++)
             if (w >= w0 && w < w1)
                 *(__attribute__((address_space(3))) u4 *)(uintptr_t)(row ^ (w * 16)) = mx_values<E>(x.codes[w], (w < 4 ? x.scales : x.scales >> 8) << 23);
     };
-    auto put_keys = [&](const Coded &x, int buf, int w0 = 0, int w1 = 8) { put(x, w0, w1, lds + buf * TILE, 1); };
-    auto put_values = [&](const Coded &x, int buf, int w0 = 0, int w1 = 8) { put(x, w0, w1, lds + (2 + buf) * TILE, 2); };
+    auto put_keys = [&](const Coded &x, int buf, int w0 = 0, int w1 = 8) { put(x, w0, w1, lds + buf * TILE + (place_of_part() & 0xffffu)); };
+    auto put_values = [&](const Coded &x, int buf, int w0 = 0, int w1 = 8) { put(x, w0, w1, lds + (2 + buf) * TILE + (place_of_part() >> 16)); };
     auto meet_lds = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
     float m = kNone, l = 0.0f;

@@ -345,3 +345,23 @@ def test_through_the_dispatcher():
         made = empty(4, 16, 2, 64)
         attention.cache_write(k, v, *made, slots)
     assert all(torch.equal(a, b) for a, b in zip(attention.cache_read(*made, slots, 64), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [True, False])
+def test_read_of_more_than_the_caches_hold(quantised):
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    rand = lambda shape: torch.randint(0, 256, shape, dtype=torch.uint8, device="cuda", generator=gen)
+    if quantised:
+        cache = attention.mxfp4_cache(300, 64, 4, 128)
+        for c in cache:
+            c.codes.copy_(rand(c.codes.shape))
+            c.scales.copy_(rand(c.scales.shape) % 20 + 117)
+    else:
+        cache = torch.randn(2, 300, 64, 4, 128, device="cuda", generator=gen).half().unbind()
+    slots = torch.randint(-50, 300 * 64 + 50, (17001,), device="cuda", generator=gen, dtype=torch.int32)
+    inside = (slots >= 0) & (slots < 300 * 64)
+    at = torch.where(inside, slots, 0).long()
+    for got, c in zip(attention.cache_read(*cache, slots, 128), cache):
+        want = decode(c.codes[at // 64, at % 64], c.scales[at // 64, at % 64], 128) if quantised else c[at // 64, at % 64].double()
+        assert torch.equal(got.double(), torch.where(inside[:, None, None], want, 0.0))

@@ -113,7 +113,11 @@ int plan(const gptq_hip_attention &a, bool mx, Plan &pl)
         Division &s = pl.shared;
         s.rt = few_operands(T * group, a.cache.dim);
         s.tiles = (int)ceil_div(T * group, s.rows());
-        divide(s, s.rt ? 2 * kPrefixWorkgroups : kPrefixWorkgroups, s.tiles * H, a.prefix_length, std::min(room, kMostPrefixParts));
+        // (MXFP4, us with 256 and 512 workgroups: few rows, 8 behind 16384 21.6 / 27.7, 4 behind 32768 22.2 / 26.5; tiles, where two share a CU's
+        // matrix pipes and its conversions, 128 behind 32768 119 / 107.5, behind 16384 73.6 / 71.0, in parts of 512 keys 64 behind 16384
+        // 49.0 / 52.3, 128 behind 8192 49.8 / 50.8.)
+        const bool two = mx ? !s.rt && a.cache.dim <= 128 && s.tiles * H * a.prefix_length >= 512ll * 1024 : s.rt != 0;
+        divide(s, two ? 2 * kPrefixWorkgroups : kPrefixWorkgroups, s.tiles * H, a.prefix_length, std::min(room, kMostPrefixParts));
         pl.prefix_rows = (size_t)(s.splits * all);
     } else {
         keys += a.prefix_length;

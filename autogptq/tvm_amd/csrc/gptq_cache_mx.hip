@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const CacheRead p)
 template <typename E, bool MX>
 static void launch_read(const CacheRead &p, unsigned grid, hipStream_t stream)
 {
-    const bool past = (unsigned long long)p.tokens * p.row_chunks * 32 > 32ull << 20;       // the second-level caches' 8 times 4 MiB
+    const bool past = (unsigned long long)p.tokens * p.row_chunks * 32 >= 32ull << 20;      // the second-level caches' 8 times 4 MiB
     if (past) hipLaunchKernelGGL((cache_read_kernel<E, MX, true>), dim3(grid), dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((cache_read_kernel<E, MX, false>), dim3(grid), dim3(256), 0, stream, p);
 }

@@ -163,10 +163,10 @@ class PagedCache:
         return attention.cache_read(self.k[layer], self.v[layer], slots)
 
     def _in_type(self, **tensors: torch.Tensor) -> None:
-        """(The codes of a quantised cache do not say which type they were written from.)"""
+        """(The codes of a quantised cache do not say which type they were written from, nor where a head's values end.)"""
         for name, t in tensors.items():
-            if self.quantize and t.dtype != self.dtype:
-                raise ValueError(f"{name} is {t.dtype}, the cache holds values of {self.dtype}")
+            if self.quantize and (t.dtype != self.dtype or t.shape[-1:] != (self.dim,)):
+                raise ValueError(f"{name} is {t.dtype} {tuple(t.shape)}, the cache holds values of {self.dtype}, {self.dim} of a head")
 
     def _forget(self, request: int, first: int, last: Optional[int] = None) -> None:
         """Takes entries out of a request's table.  (Steps keep theirs; the entries that later steps add lie past their contexts.)"""

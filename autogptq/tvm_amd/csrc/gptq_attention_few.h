@@ -115,10 +115,10 @@ __global__ __launch_bounds__(64 * kFewWaves, few_resident(RT, DP, MX)) void atte
         clear_rest(given, given.starts[0], given.starts[given.requests], blockIdx.x * (64ll * kFewWaves) + threadIdx.x, gridDim.x * (64ll * kFewWaves));
         upto = sum_upto(look.total);
         int total = __builtin_amdgcn_readlane(upto, 63), most = 0;       // units in all, and of a tile at most
-        if (MX) most = max_lanes(look.units);
+        if (MX) most = max_lanes(look.total ? look.units : 0);
         for (int b = 64; b < given.requests; b += 64) {
             const Requests x = look_at<R, MX>(given, b);
-            if (MX) most = max(most, max_lanes(x.units));
+            if (MX) most = max(most, max_lanes(x.total ? x.units : 0));
             total += __builtin_amdgcn_readlane(sum_upto(x.total), 63);
         }
         // (Whole tiles of two units rather than their halves, once every CU has a workgroup: the second unit costs less than

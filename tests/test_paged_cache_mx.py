@@ -43,6 +43,12 @@ def test_refusals():
     for call in (lambda: c.write(0, x.half(), x.bfloat16(), None), lambda: c.write(0, x, x, None), lambda: c.attend(0, x.bfloat16(), None)):
         with pytest.raises(ValueError, match="holds values of torch.float16"):
             call()
+    # (rows of 80 values and of 96 take the same bytes)
+    c = cache(device="cpu", dim=80)
+    for x in (torch.zeros(3, 2, 96).half(), torch.zeros(3, 2, 72).half()):
+        for call in (lambda: c.write(0, x, x, None), lambda: c.attend(0, x, None)):
+            with pytest.raises(ValueError, match="80 of a head"):
+                call()
     with pytest.raises(IndexError):
         c.read(0, 4)
     with pytest.raises(RuntimeError, match="no CPU fallback"):

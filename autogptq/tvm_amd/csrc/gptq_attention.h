@@ -66,6 +66,7 @@ struct AttentionParams {
     // the excess of the product, x times less than block_size, stays below 2^(29 + bits)
     uint32_t block_magic;
     int block_bits;
+    int even;                // kernel of tiles on a cache in MXFP4: the keys of a part follow from the lengths, see even_parts
     int unit_bits;           // few-rows kernel on a cache in MXFP4: log2 of the keys of a unit
 };
 
@@ -250,6 +251,34 @@ __device__ __forceinline__ void put_stats(float *to, float m, float l)
 {
     if constexpr (COHERENT) store_stats(to, m, l);
     else *(f2 *)to = (f2){m, l};
+}
+
+// the sum over the lanes up to this one
+__device__ __forceinline__ int sum_upto(int x)
+{
+#define GPTQ_ADD(CONTROL, ROWS) x += __builtin_amdgcn_update_dpp(0, x, CONTROL, ROWS, 0xf, false)
+    GPTQ_ADD(0x111, 0xf);   // within rows of 16: from 1, 2, 4, 8 lanes before
+    GPTQ_ADD(0x112, 0xf);
+    GPTQ_ADD(0x114, 0xf);
+    GPTQ_ADD(0x118, 0xf);
+    GPTQ_ADD(0x142, 0xa);   // the last lane of rows 0 and 2 into rows 1 and 3
+    GPTQ_ADD(0x143, 0xc);   // that of row 1 into rows 2 and 3
+#undef GPTQ_ADD
+    return x;
+}
+
+// the largest of the lanes' values, none of which is negative
+__device__ __forceinline__ int max_lanes(int x)
+{
+#define GPTQ_MAX(CONTROL, ROWS) x = max(x, __builtin_amdgcn_update_dpp(0, x, CONTROL, ROWS, 0xf, false))
+    GPTQ_MAX(0x111, 0xf);   // as above
+    GPTQ_MAX(0x112, 0xf);
+    GPTQ_MAX(0x114, 0xf);
+    GPTQ_MAX(0x118, 0xf);
+    GPTQ_MAX(0x142, 0xa);
+    GPTQ_MAX(0x143, 0xc);
+#undef GPTQ_MAX
+    return __builtin_amdgcn_readlane(x, 63);
 }
 
 // row r of a tile: its token (in the request) and query head

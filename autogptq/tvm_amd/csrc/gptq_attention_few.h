@@ -58,34 +58,6 @@ __device__ __forceinline__ Requests look_at(const AttentionParams &p, int base)
     r.total = (int)(((uint32_t)r.count * (uint32_t)p.group + R - 1) / R) * r.units;
     return r;
 }
-// the sum over the lanes up to this one
-__device__ __forceinline__ int sum_upto(int x)
-{
-#define GPTQ_ADD(CONTROL, ROWS) x += __builtin_amdgcn_update_dpp(0, x, CONTROL, ROWS, 0xf, false)
-    GPTQ_ADD(0x111, 0xf);   // within rows of 16: from 1, 2, 4, 8 lanes before
-    GPTQ_ADD(0x112, 0xf);
-    GPTQ_ADD(0x114, 0xf);
-    GPTQ_ADD(0x118, 0xf);
-    GPTQ_ADD(0x142, 0xa);   // the last lane of rows 0 and 2 into rows 1 and 3
-    GPTQ_ADD(0x143, 0xc);   // that of row 1 into rows 2 and 3
-#undef GPTQ_ADD
-    return x;
-}
-
-// the largest of the lanes' values, none of which is negative
-__device__ __forceinline__ int max_lanes(int x)
-{
-#define GPTQ_MAX(CONTROL, ROWS) x = max(x, __builtin_amdgcn_update_dpp(0, x, CONTROL, ROWS, 0xf, false))
-    GPTQ_MAX(0x111, 0xf);   // as above
-    GPTQ_MAX(0x112, 0xf);
-    GPTQ_MAX(0x114, 0xf);
-    GPTQ_MAX(0x118, 0xf);
-    GPTQ_MAX(0x142, 0xa);
-    GPTQ_MAX(0x143, 0xc);
-#undef GPTQ_MAX
-    return __builtin_amdgcn_readlane(x, 63);
-}
-
 // DP: compiled width, the dims past p.dim do not count; FULL: there are none; RT: 16-row operands a wave holds; SHARED: the parts of a
 // shared prefix; MX: a cache in MXFP4
 template <typename E, int DP, bool FULL, int RT, bool SHARED, bool MX>

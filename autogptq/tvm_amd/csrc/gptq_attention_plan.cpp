@@ -54,6 +54,7 @@ struct Division {
     int rt = 0;        // 16-row operands a wave of the few-rows kernel, 0: the tile kernel
     int tiles = 0;     // of rows: all there can be
     int splits = 1, chunk = 1;          // parts of a tile at most, keys of a part
+    int even = 0;      // kernel of tiles: the keys of a part follow from the lengths, for this many workgroups
     int team = 1, most_units = 1, unit_bits = 8;       // few-rows kernel on own contexts: see there
     int rows() const { return rt ? 16 * rt : kTileRows; }
 };
@@ -136,6 +137,13 @@ int plan(const gptq_hip_attention &a, bool mx, Plan &pl)
         pl.own_rows = (size_t)(2 * d.team * H * d.rows());
     } else {
         divide(d, kOwnWorkgroups, std::max(B, ceil_div(T * group, d.rows())) * H, keys, room);
+        // MXFP4: parts by the lengths on the GPU (even_parts), us by the longest context and so: 3 pieces of up to 300 tokens behind up to
+        // 20000 keys 184 / 142, 20 of up to 33 behind 16000 135 / 88, 4 of 40 behind 8000 65 / 57; 60 of up to 99 behind 16000 281 / 288
+        // (more tiles than workgroups), 16 of 20 behind 2068 48.0 / 51.9.
+        if (mx && d.splits > 1 && B > 1 && B <= 64 && keys >= 6144) {
+            d.even = (int)(a.cache.dim > 128 ? kOwnWorkgroups / 2 : kOwnWorkgroups);     // (as many as the card holds)
+            d.splits = (int)std::max(1ll, std::min({2ll * d.splits, ceil_div(keys, 256), room}));
+        }
         if (d.splits > 1 || pl.prefix) pl.own_rows = (size_t)(d.splits * all);
     }
     const size_t rows = pl.prefix_rows + pl.own_rows;
@@ -200,7 +208,7 @@ int attend(const gptq_hip_attention *a, const gptq_hip_cache_mx *mx, void *works
     while (p.block_bits < 31 && 1ll << p.block_bits < c.block_size) p.block_bits++;
     p.block_magic = (uint32_t)(((1ull << (29 + p.block_bits)) + (unsigned)c.block_size - 1) / (unsigned)c.block_size);
     auto launch = [&](const Division &d) {
-        p.tiles = d.tiles, p.splits = d.splits, p.chunk = d.chunk, p.team = d.team, p.most_units = d.most_units, p.unit_bits = d.unit_bits;
+        p.tiles = d.tiles, p.splits = d.splits, p.chunk = d.chunk, p.team = d.team, p.most_units = d.most_units, p.unit_bits = d.unit_bits, p.even = d.even;
         if (d.rt) return mx ? launch_attention_few_mx(p, c.type, d.rt, stream) : launch_attention_few(p, c.type, d.rt, stream);
         return mx ? launch_attention_tile_mx(p, c.type, stream) : launch_attention_tile(p, c.type, stream);
     };

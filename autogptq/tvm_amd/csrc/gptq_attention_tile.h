@@ -80,6 +80,40 @@ __device__ __forceinline__ int tile_parts(const AttentionParams &p, int seen, in
     return max(1, (seen + chunk - 1) / chunk);
 }
 
+// Up to 64 requests: the smallest parts, in steps of 64 keys, with which all tiles together have no more parts than run at once, if
+// those are not longer than 1.5 times an even share; else the host's.  (The host knows the longest context only and divides as
+// if all had it, and counts no tiles that are not full.)  Every workgroup finds them for itself, of the same numbers by the same
+// operations; that and the places for twice as many parts cost 4 us, so that it is for long contexts: measured beside the choice.
+__device__ __forceinline__ int even_parts(const AttentionParams &p, int seen, int &chunk)
+{
+    const int b = threadIdx.x & 63, last = p.requests - 1;
+    const int start = min(max(p.starts[min(b, last)], 0), p.tokens);
+    const int count = b > last ? 0 : min(max(p.starts[min(b, last) + 1] - start, 0), p.tokens - start);
+    const int context = p.contexts[min(b, last)];
+    const int hi = max(min(context, held_keys(p)), 0), lo = p.window > 0 ? min(max(context - count - p.window + 1, 0), hi) : 0;
+    const int keys = count > 0 ? p.front + min(p.sinks, lo) + hi - lo : 0;
+    const int tiles = (int)(((uint32_t)count * (uint32_t)p.group + kTileRows - 1) / kTileRows);
+    const int steps = (keys + kTileKeys - 1) / kTileKeys, most = max_lanes(steps);
+    // (of wrong lengths the sums may be anything: every choice is a right one, and the same in every workgroup)
+    const float all = (float)__builtin_amdgcn_readlane(sum_upto(tiles * ((steps + 63) / 64)), 63) * 64.0f;
+    const int share = (int)min(all * 1.5f * (float)p.kv_heads / (float)p.even, 1e6f), least = max(4, (most + p.splits - 1) / p.splits);
+    auto fit = [&](int part) {
+        const int parts = tiles * (int)ceilf((float)steps * __builtin_amdgcn_rcpf((float)part));
+        return (long long)__builtin_amdgcn_readlane(sum_upto(parts), 63) * p.kv_heads <= p.even;
+    };
+    int few = least, many = max(least, min(most, share));      // steps of a part
+    if (!fit(many)) few = many = max(least, p.chunk / kTileKeys);
+    while (few < many) {
+        const int mid = (few + many) / 2;
+        if (fit(mid)) many = mid;
+        else few = mid + 1;
+    }
+    chunk = max(few * kTileKeys, ((seen + p.splits - 1) / p.splits + kTileKeys - 1) / kTileKeys * kTileKeys);
+    const int parts = max(1, (seen + chunk - 1) / chunk);
+    chunk = max(kTileKeys, ((seen + parts - 1) / parts + kTileKeys - 1) / kTileKeys * kTileKeys);     // the last one no shorter
+    return max(1, (seen + chunk - 1) / chunk);
+}
+
 // 16 bytes of `src` to LDS at lds + 16 * lane.  Inline assembly, so that the compiler does not wait for every outstanding
 // request before each read of LDS; the kernel waits for them at its barrier.
 __device__ __forceinline__ void request16(const char *src, uint32_t lds)
@@ -121,7 +155,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
     if (!p.shared) clear_rest(p, first_token, end_token, (blockIdx.y * (long long)gridDim.x + blockIdx.x) * 256 + threadIdx.x, 256ll * gridDim.x * gridDim.y);
     if (!found) return;
     int chunk;
-    const int parts = tile_parts(p, q.seen, KT, chunk);
+    const int parts = MX && p.even ? even_parts(p, q.seen, chunk) : tile_parts(p, q.seen, KT, chunk);
     if (split >= parts) return;
     const int begin = split * chunk, end = min(q.seen, begin + chunk);
     const int32_t *table = p.tables + (long long)q.b * p.table_stride;

@@ -11,7 +11,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionPara
     QueryTile q;
     if (!find_tile<kTileRows>(p, tile, q) || r0 >= q.rows) return;
     int chunk;
-    const int parts = tile_parts(p, q.seen, kTileKeys, chunk);
+    const int parts = p.even ? even_parts(p, q.seen, chunk) : tile_parts(p, q.seen, kTileKeys, chunk);
     if (parts == 1 && p.prefix_parts == 0) return;
     const long long all = (long long)p.tokens * p.heads;
     const int quads = p.dim / 4;

@@ -29,6 +29,11 @@ MORE = {     # widths whose last group is not whole, or that leave groups of the
                                                       4, 2, 128, 16, HALF, "head", 0, 0),
     "one long context alone": ([(20000, 1)], 4, 1, 128, 64, HALF, "head", 0, 0),
     "two operands": ([(900, 1), (1300, 1), (40, 1)], 24, 1, 128, 16, BF16, "head", 0, 0),
+    "ragged pieces behind long contexts": ([(7000, 60), (300, 40), (2500, 130), (6500, 1), (0, 0)], 4, 1, 128, 16, HALF, "head", 0, 0),
+    "ragged pieces behind long contexts, dim 64": ([(9000, 33), (9000, 32), (128, 128), (5000, 70)], 8, 2, 64, 64, BF16, "head", 0, 0),
+    "ragged pieces behind long contexts, dim 256": ([(6200, 50), (640, 40), (6300, 30)], 4, 1, 256, 16, HALF, "head", 0, 0),
+    "ragged pieces under a long window": ([(9000, 60), (300, 40), (12000, 130)], 4, 1, 128, 24, HALF, "head", 7000, 5),
+    "more tiles than workgroups behind long contexts": ([(6400 - 700 * (i % 9), 64) for i in range(40)], 32, 4, 64, 64, HALF, "head", 0, 0),
     "two operands, dim 64": ([(900, 7), (1300, 5), (40, 7)], 4, 1, 64, 16, HALF, "head", 0, 0),
 }
 
@@ -43,10 +48,16 @@ def test_attention(name):
     assert torch.equal(got, attend(s)), "a second call on the same inputs differs"
 
 
+LONG_PREFIXES = {
+    "ragged pieces behind long contexts": ([(6500, 40), (300, 40), (2500, 130)], 4, 1, 128, 16, HALF, 700),
+    "tiles in two a CU": ([(1 + i % 7, 1) for i in range(64)], 64, 8, 64, 64, HALF, 16500),
+}
+
+
 @pytest.mark.gpu
-@pytest.mark.parametrize("name", list(PREFIXES))
+@pytest.mark.parametrize("name", list(PREFIXES) + ["long: " + n for n in LONG_PREFIXES])
 def test_shared_prefix(name):
-    requests, heads, kv_heads, dim, block, dtype, prefix = PREFIXES[name]
+    requests, heads, kv_heads, dim, block, dtype, prefix = PREFIXES[name] if name in PREFIXES else LONG_PREFIXES[name[6:]]
     s = MxStep(12, requests, heads, kv_heads, dim, block, dtype, prefix=prefix)
     got = attend(s)
     assert_attention(got, s, name)

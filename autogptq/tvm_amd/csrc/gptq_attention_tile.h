@@ -18,14 +18,20 @@
 //             the parts, 16 rows a workgroup.  (The last workgroup of a tile doing it, one for up to 128 rows: 16 pieces of
 //             20 tokens behind 2048 keys, dim 128, 73.6 us against 54.5; 5 of up to 333 behind up to 9001, dim 80, 77.7
 //             against 66.6.)
-//   LDS       rows as they lie in the cache; the 16-byte chunks of row r stand at chunk ^ r (keys) and chunk ^ 2 r (values),
-//             without which all lanes of a read would stand on the same banks.  Some still do: a third of the cycles of LDS are
-//             conflicts.  The swizzle is in the requests' source addresses.
+//   LDS       rows as they lie in the cache; the 16-byte chunk c of row r stands at c ^ t(r), the four low bits of r turned by two.
+//             Sixteen lanes read the same chunk of 16 keys at a time, and 32 lanes four chunks of four rows of values: t puts each on banks of
+//             its own (c ^ r and c ^ 2 r, which served sixteen lanes of the latter, cost a third of the cycles of LDS and 1 % of the
+//             time).  The swizzle is in the requests' source addresses.
 //
-// Measured (32 heads in groups of 4, dim 128): a prompt of 8192 tokens 587 to 613 us on different cards, 897 to 937 TFLOP/s; the matrix
+// Measured (32 heads in groups of 4, dim 128): a prompt of 8192 tokens 587 to 619 us on different cards, 889 to 937 TFLOP/s; the matrix
 // pipes are busy in half of the cycles, at 1.8 GHz; a wave waits for data or the barrier 31 % of its time, and 31 % to issue.  Without
 // the exponentials it takes 6 % less, without the requests 18 %, without the reads of values 3 %.  Not better: 64 rows a wave (spills,
 // 1537 us), eight waves a workgroup (the same), a wave's priority raised around its products (fewer cycles, the same time).
+//
+// A cache in MXFP4 (MX).  LDS holds the same values at the same places.  A tile's codes come into registers a tile ahead, four threads a
+// row, and are turned into values (two an instruction, exactly) and written to LDS between the products, whose pipe they leave alone.
+// Measured as above: a prompt of 8192 tokens 573 to 586 us, 938 to 960 TFLOP/s; 128 single tokens behind a prefix of 16384 67 us, two launches and
+// the parts between them; 5 pieces of up to 333 behind up to 9001, dim 80, 75 us.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -199,19 +205,22 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
         }
     };
     typedef uint32_t Rows __attribute__((ext_vector_type(PASSES)));
+    // the swizzle of a row.  (Rows of 64 dims alternate between the halves of the banks, so that three bits do; the lowest two, of which
+    // rows of values differ, must both count.)
+    auto turn = [](int row) { return DP == 64 ? ((row ^ row >> 1) << 2 & 4) | (row >> 2 & 3) : (row << 2 & 12) | (row >> 2 & 3); };
     // this thread's chunk of the rows it requests
     const int myrow = threadIdx.x / CH, place = threadIdx.x % CH;
     auto rows_of = [&](int n) { return *(const Rows *)(list + (n & 7) * KT + myrow * PASSES); };
-    auto request = [&](const Rows &rows, const char *from, uint32_t to, int twist) {
+    auto request = [&](const Rows &rows, const char *from, uint32_t to) {
 #pragma unroll
         for (int j = 0; j < PASSES; j++) {
-            const int c = place ^ ((twist * (j * RP + myrow)) & (CH - 1));
+            const int c = place ^ turn(j * RP + myrow);
             if (p.dim == DP || c * 8 < p.dim)
                 request16(from + (unsigned long long)rows[j] * 16 + c * 16, __builtin_amdgcn_readfirstlane(to + wave * 1024 + j * 4096));
         }
     };
-    auto request_keys = [&](const Rows &rows, int buf) { request(rows, kbase, lds + buf * TILE, 1); };
-    auto request_values = [&](const Rows &rows, int buf) { request(rows, vbase, lds + (2 + buf) * TILE, 2); };
+    auto request_keys = [&](const Rows &rows, int buf) { request(rows, kbase, lds + buf * TILE); };
+    auto request_values = [&](const Rows &rows, int buf) { request(rows, vbase, lds + (2 + buf) * TILE); };
     auto meet = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
     // MX: four threads hold a row of a tile, DP / 4 dims each, and write them to LDS as values.  (Rows end with a group: what of a
@@ -227,18 +236,20 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
         if constexpr (DP != 128 || DC == 128) asm volatile("" : "+v"(t));
         return t;
     };
+    // MX: the row whose codes a thread holds: the eight lanes that LDS takes at a time write eight chunks whose lowest bits differ
+    auto row_of_codes = [](int thread) { return thread >> 6 << 4 | (thread << 2 & 12) | (thread >> 2 & 3); };
     // Where its part of a row goes, from a tile's beginning: keys in the lower half of the word, values in the upper.  (Dynamic LDS begins at 0,
     // so that the swizzle is in the low bits of the sum.)
     auto find_place = [&]() {
-        const int thread = this_thread(), code_row = thread / 4, chunk = thread % 4 * DW;
-        return (uint32_t)(code_row * (DP * 2) + (chunk ^ (code_row & (CH - 1))) * 16) |
-               (uint32_t)(code_row * (DP * 2) + (chunk ^ (2 * code_row & (CH - 1))) * 16) << 16;
+        const int thread = this_thread(), code_row = row_of_codes(thread), chunk = (thread >> 4 & 3) * DW;
+        return (uint32_t)(code_row * (DP * 2) + (chunk ^ turn(code_row)) * 16) |
+               (uint32_t)(code_row * (DP * 2) + (chunk ^ turn(code_row)) * 16) << 16;
     };
     static_assert(TILE <= 1 << 16, "");
     const uint32_t kept_place = MX && DP <= 128 ? find_place() : 0;
     auto place_of_part = [&]() { return DP <= 128 ? kept_place : find_place(); };
     auto fetch = [&](int n, const char *from, const void *scales) {
-        const int thread = this_thread(), code_row = thread / 4, code_part = thread % 4;
+        const int thread = this_thread(), code_row = row_of_codes(thread), code_part = thread >> 4 & 3;
         Coded x = {};
         const int first = code_part * DP / 128;              // the thread's first group
         x.scales = 0x7f7fu;
@@ -282,15 +293,15 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
     // values, leave the swizzle as it is.
     uint32_t kat[SX], vat[2][DT];
 #pragma unroll
-    for (int x = 0; x < SX; x++) kat[x] = lds + col * (DP * 2) + (((2 * x + hh) ^ (col & (CH - 1))) * 16);
+    for (int x = 0; x < SX; x++) kat[x] = lds + col * (DP * 2) + (((2 * x + hh) ^ turn(col)) * 16);
 #pragma unroll
     for (int up = 0; up < 2; up++)
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
             const int key = 8 * up + 4 * hh + (col & 15) / 4, c = 4 * dt + 2 * (col >> 4) + (col & 3) / 2;
-            vat[up][dt] = lds + 2 * TILE + key * (DP * 2) + ((c ^ ((2 * key) & (CH - 1))) * 16) + (col & 1) * 8;
+            vat[up][dt] = lds + 2 * TILE + key * (DP * 2) + ((c ^ turn(key)) * 16) + (col & 1) * 8;
         }
-    static_assert(CH <= 32, "the swizzle repeats every 32 rows, of keys, and every 16, of values");
+    static_assert(CH >= 8, "the swizzle repeats every 16 rows");
 
     f16 s[KA];
     // S^T for the keys in the buffer BUF

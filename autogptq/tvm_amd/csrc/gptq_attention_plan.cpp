@@ -84,8 +84,9 @@ constexpr long long kOwnWorkgroups = 512, kPrefixWorkgroups = 256;
 constexpr long long kMostPrefixParts = 1024;
 
 struct Plan {
-    Division own, shared;
+    Division own, shared, few;
     bool prefix = false;             // a launch of its own for the shared prefix
+    bool mixed = false;              // `few` for requests of up to few.rows() rows, `own` for the others
     size_t prefix_rows = 0, own_rows = 0, bytes = 0;     // rows of the parts in the workspace
 };
 
@@ -123,7 +124,8 @@ int plan(const gptq_hip_attention &a, bool mx, Plan &pl)
     } else {
         keys += a.prefix_length;
     }
-    if (d.rt) {
+    // the few-rows kernel on own contexts, with d.tiles tiles
+    auto by_units = [&](Division &d) {
         const long long most = B * (T * group / d.rows() + 1);    // tiles, whatever the lengths on the GPU say
         if (most > 1ll << 30) return GPTQ_HIP_ERR_UNSUPPORTED;
         d.most_units = (int)std::min((1ll << 30) / most, 1ll << 20);
@@ -134,17 +136,33 @@ int plan(const gptq_hip_attention &a, bool mx, Plan &pl)
         const long long units = (d.tiles + 0ll) * std::max(1ll, ceil_div(keys, 1ll << d.unit_bits));
         d.team = (int)std::max(1ll, std::min(team, units));
         if (d.team * H > (long long)(kAttentionCounters / 4)) return GPTQ_HIP_ERR_UNSUPPORTED;
-        pl.own_rows = (size_t)(2 * d.team * H * d.rows());
+        pl.own_rows = std::max(pl.own_rows, (size_t)(2 * d.team * H * d.rows()));
+        return GPTQ_HIP_OK;
+    };
+    if (d.rt) {
+        const int rc = by_units(d);
+        if (rc != GPTQ_HIP_OK) return rc;
     } else {
-        divide(d, kOwnWorkgroups, std::max(B, ceil_div(T * group, d.rows())) * H, keys, room);
+        // MXFP4: single tokens that a batch of pieces may hold have a launch of the few-rows kernel to themselves, where they would cost
+        // the kernel of tiles more than such a launch finds nothing in.  (us without and with it: 63 up to 32768 and a piece of 512 behind
+        // 4096 646 / 126, 7 up to 8192 and 256 behind 2044 72 / 59, 63 up to 4000 and a prompt of 2048 151 / 102, with 2 key/value
+        // heads 7 up to 16384 and 512 behind 4096 58.0 / 55.4; nothing in it: 32 of 64 behind 4096 225 / 227; below the bound 8 of
+        // 128 behind 4096 102 / 104, 3 up to 2500 and 256 behind 2044, 2 heads, 25 / 34.  Long pieces among so many single tokens that
+        // the mean fits the few-rows kernel stay there: 255 up to 1000 and 1024 behind 7168 236, in two launches 259.)
+        Division &f = pl.few;
+        f.rt = few_operands(group, a.cache.dim);
+        f.tiles = (int)B;
+        pl.mixed = mx && f.rt && B > 1 && B * H * keys >= 512ll * 1024 && by_units(f) == GPTQ_HIP_OK;
+        const bool even = mx && B > 1 && B <= kEvenRequests && keys >= 6144;
+        divide(d, kOwnWorkgroups, std::max(pl.mixed && even ? 1 : B, ceil_div(T * group, d.rows())) * H, keys, room);
         // MXFP4: parts by the lengths on the GPU (even_parts), us by the longest context and so: 3 pieces of up to 300 tokens behind up to
         // 20000 keys 184 / 142, 20 of up to 33 behind 16000 135 / 88, 4 of 40 behind 8000 65 / 57; 60 of up to 99 behind 16000 281 / 288
         // (more tiles than workgroups), 16 of 20 behind 2068 48.0 / 51.9.
-        if (mx && d.splits > 1 && B > 1 && B <= 64 && keys >= 6144) {
+        if (even && d.splits > 1) {
             d.even = (int)(a.cache.dim > 128 ? kOwnWorkgroups / 2 : kOwnWorkgroups);     // (as many as the card holds)
             d.splits = (int)std::max(1ll, std::min({2ll * d.splits, ceil_div(keys, 256), room}));
         }
-        if (d.splits > 1 || pl.prefix) pl.own_rows = (size_t)(d.splits * all);
+        if (d.splits > 1 || pl.prefix) pl.own_rows = std::max(pl.own_rows, (size_t)(d.splits * all));
     }
     const size_t rows = pl.prefix_rows + pl.own_rows;
     pl.bytes = rows ? kAttentionCounters + (rows * 8 + 255) / 256 * 256 + rows * a.cache.dim * 4 : 0;
@@ -208,7 +226,7 @@ int attend(const gptq_hip_attention *a, const gptq_hip_cache_mx *mx, void *works
     while (p.block_bits < 31 && 1ll << p.block_bits < c.block_size) p.block_bits++;
     p.block_magic = (uint32_t)(((1ull << (29 + p.block_bits)) + (unsigned)c.block_size - 1) / (unsigned)c.block_size);
     auto launch = [&](const Division &d) {
-        p.tiles = d.tiles, p.splits = d.splits, p.chunk = d.chunk, p.team = d.team, p.most_units = d.most_units, p.unit_bits = d.unit_bits, p.even = d.even;
+        p.tiles = d.tiles, p.splits = d.splits, p.chunk = d.chunk, p.team = d.team, p.most_units = d.most_units, p.unit_bits = d.unit_bits | (&d == &pl.few ? 32 : 0), p.even = d.even;
         if (d.rt) return mx ? launch_attention_few_mx(p, c.type, d.rt, stream) : launch_attention_few(p, c.type, d.rt, stream);
         return mx ? launch_attention_tile_mx(p, c.type, stream) : launch_attention_tile(p, c.type, stream);
     };
@@ -224,6 +242,11 @@ int attend(const gptq_hip_attention *a, const gptq_hip_cache_mx *mx, void *works
     p.tables = a->tables, p.table_width = a->table_width, p.table_stride = a->table_stride;
     p.starts = a->starts, p.contexts = a->contexts;
     p.window = std::min(a->window, kMostKeys), p.sinks = std::min(a->sinks, kMostKeys);
+    if (pl.mixed) {      // (both keep their parts at the same place, one after the other)
+        p.few_rows = pl.few.rows();
+        rc = launch(pl.few);
+        if (rc != GPTQ_HIP_OK) return rc;
+    }
     return launch(pl.own);
 }
 

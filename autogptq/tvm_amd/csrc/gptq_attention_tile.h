@@ -71,7 +71,7 @@ __device__ __forceinline__ bool find_tile(const AttentionParams &p, int tile, Qu
         q.row0 = (tile - ((int)((uint32_t)q.start * (uint32_t)p.group / R) + q.b)) * R;
     }
     const int all = q.count * p.group;
-    if (q.row0 < 0 || q.row0 >= all) return false;
+    if (q.row0 < 0 || q.row0 >= all || all <= p.few_rows) return false;
     q.rows = min(R, all - q.row0);
     if (p.shared) set_tile<true>(p, q, context);
     else set_tile<false>(p, q, context);
@@ -86,25 +86,38 @@ __device__ __forceinline__ int tile_parts(const AttentionParams &p, int seen, in
     return max(1, (seen + chunk - 1) / chunk);
 }
 
-// Up to 64 requests: the smallest parts, in steps of 64 keys, with which all tiles together have no more parts than run at once, if
+// Up to kEvenRequests requests: the smallest parts, in steps of 64 keys, with which all tiles together have no more parts than run at once, if
 // those are not longer than 1.5 times an even share; else the host's.  (The host knows the longest context only and divides as
 // if all had it, and counts no tiles that are not full.)  Every workgroup finds them for itself, of the same numbers by the same
 // operations; that and the places for twice as many parts cost 4 us, so that it is for long contexts: measured beside the choice.
-__device__ __forceinline__ int even_parts(const AttentionParams &p, int seen, int &chunk)
+template <int N>
+__device__ __forceinline__ int even_parts_of(const AttentionParams &p, int seen, int &chunk)
 {
-    const int b = threadIdx.x & 63, last = p.requests - 1;
-    const int start = min(max(p.starts[min(b, last)], 0), p.tokens);
-    const int count = b > last ? 0 : min(max(p.starts[min(b, last) + 1] - start, 0), p.tokens - start);
-    const int context = p.contexts[min(b, last)];
-    const int hi = max(min(context, held_keys(p)), 0), lo = p.window > 0 ? min(max(context - count - p.window + 1, 0), hi) : 0;
-    const int keys = count > 0 ? p.front + min(p.sinks, lo) + hi - lo : 0;
-    const int tiles = (int)(((uint32_t)count * (uint32_t)p.group + kTileRows - 1) / kTileRows);
-    const int steps = (keys + kTileKeys - 1) / kTileKeys, most = max_lanes(steps);
-    // (of wrong lengths the sums may be anything: every choice is a right one, and the same in every workgroup)
-    const float all = (float)__builtin_amdgcn_readlane(sum_upto(tiles * ((steps + 63) / 64)), 63) * 64.0f;
+    const int lane = threadIdx.x & 63, last = p.requests - 1;
+    int steps[N], tiles[N], most = 0;      // of the requests 64 n + lane: steps of a tile, and tiles
+    float all = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        steps[n] = tiles[n] = 0;
+        if (n && 64 * n > last) continue;
+        const int b = min(64 * n + lane, last), start = min(max(p.starts[b], 0), p.tokens);
+        int count = min(max(p.starts[b + 1] - start, 0), p.tokens - start);
+        if (64 * n + lane > last || (uint32_t)count * (uint32_t)p.group <= (uint32_t)p.few_rows) count = 0;
+        const int context = p.contexts[b];
+        const int hi = max(min(context, held_keys(p)), 0), lo = p.window > 0 ? min(max(context - count - p.window + 1, 0), hi) : 0;
+        const int keys = count > 0 ? p.front + min(p.sinks, lo) + hi - lo : 0;
+        tiles[n] = (int)(((uint32_t)count * (uint32_t)p.group + kTileRows - 1) / kTileRows);
+        steps[n] = (keys + kTileKeys - 1) / kTileKeys;
+        most = max(most, max_lanes(steps[n]));
+        // (of wrong lengths the sums may be anything: every choice is a right one, and the same in every workgroup)
+        all += (float)__builtin_amdgcn_readlane(sum_upto(tiles[n] * ((steps[n] + 63) / 64)), 63) * 64.0f;
+    }
     const int share = (int)min(all * 1.5f * (float)p.kv_heads / (float)p.even, 1e6f), least = max(4, (most + p.splits - 1) / p.splits);
     auto fit = [&](int part) {
-        const int parts = tiles * (int)ceilf((float)steps * __builtin_amdgcn_rcpf((float)part));
+        const float per = __builtin_amdgcn_rcpf((float)part);
+        int parts = 0;
+#pragma unroll
+        for (int n = 0; n < N; n++) parts += tiles[n] * (int)ceilf((float)steps[n] * per);
         return (long long)__builtin_amdgcn_readlane(sum_upto(parts), 63) * p.kv_heads <= p.even;
     };
     int few = least, many = max(least, min(most, share));      // steps of a part
@@ -118,6 +131,10 @@ __device__ __forceinline__ int even_parts(const AttentionParams &p, int seen, in
     const int parts = max(1, (seen + chunk - 1) / chunk);
     chunk = max(kTileKeys, ((seen + parts - 1) / parts + kTileKeys - 1) / kTileKeys * kTileKeys);     // the last one no shorter
     return max(1, (seen + chunk - 1) / chunk);
+}
+__device__ __forceinline__ int even_parts(const AttentionParams &p, int seen, int &chunk)
+{
+    return p.requests <= 64 ? even_parts_of<1>(p, seen, chunk) : even_parts_of<kEvenRequests / 64>(p, seen, chunk);
 }
 
 // 16 bytes of `src` to LDS at lds + 16 * lane.  Inline assembly, so that the compiler does not wait for every outstanding

@@ -34,6 +34,12 @@ MORE = {     # widths whose last group is not whole, or that leave groups of the
     "ragged pieces behind long contexts, dim 256": ([(6200, 50), (640, 40), (6300, 30)], 4, 1, 256, 16, HALF, "head", 0, 0),
     "ragged pieces under a long window": ([(9000, 60), (300, 40), (12000, 130)], 4, 1, 128, 24, HALF, "head", 7000, 5),
     "more tiles than workgroups behind long contexts": ([(6400 - 700 * (i % 9), 64) for i in range(40)], 32, 4, 64, 64, HALF, "head", 0, 0),
+    "single tokens beside a piece": ([(1 + 397 * i % 6000, 1) for i in range(40)] + [(3000, 300), (50, 50), (0, 0), (2000, 4), (2000, 5)], 8, 2, 64, 16, HALF, "head", 0, 0),
+    "single tokens beside a piece, dim 128": ([(7000, 70)] + [(8100 - 97 * i, 1) for i in range(20)] + [(6300, 3), (0, 0)], 16, 4, 128, 64, BF16, "head", 0, 0),
+    "single tokens beside a piece, window": ([(9000, 1)] * 6 + [(9000, 200), (200, 200)] + [(7777, 1)] * 3, 24, 8, 80, 24, HALF, "head", 6500, 3),
+    "single tokens beside a piece, dim 256": ([(6200 - 211 * i, 1) for i in range(20)] + [(6400, 2), (6300, 60), (6500, 1)], 8, 4, 256, 16, HALF, "head", 0, 0),
+    "single tokens beside pieces, many requests": ([(2500 - 7 * i, 1) for i in range(80)] + [(2000, 400), (64, 64)] + [(1, 1)] * 10 + [(900, 700)], 16, 4, 64, 16, HALF, "head", 0, 0),
+    "heads that fit no few rows": ([(8200, 1)] * 12 + [(3000, 40)], 35, 1, 64, 16, HALF, "head", 0, 0),
     "two operands, dim 64": ([(900, 7), (1300, 5), (40, 7)], 4, 1, 64, 16, HALF, "head", 0, 0),
 }
 
@@ -50,6 +56,7 @@ def test_attention(name):
 
 LONG_PREFIXES = {
     "ragged pieces behind long contexts": ([(6500, 40), (300, 40), (2500, 130)], 4, 1, 128, 16, HALF, 700),
+    "single tokens beside a piece": ([(3000 + 61 * i, 1) for i in range(30)] + [(2000, 200), (300, 300)], 16, 4, 128, 16, BF16, 5000),
     "tiles in two a CU": ([(1 + i % 7, 1) for i in range(64)], 64, 8, 64, 64, HALF, 16500),
 }
 

@@ -44,37 +44,69 @@ namespace gptq {
 constexpr int kTileKeys = 64;   // keys of a step
 constexpr int kJoinRows = 16;
 
-// The tile of a workgroup.  Request b owns the tiles from first_tile(b) = floor(starts[b] * group / R) + b: the floors of two
-// neighbours lie at least floor(rows / R) apart, and the + b adds the tile of a remainder.  So the bound
-// floor(tokens * group / R) + requests on the number of tiles, and the request of a tile, follow without any sum over
-// requests.  False for a tile past its request's rows.
+// The tile of a workgroup: the requests' tiles one after the other, the last rows of a request first (they see the most keys).  There are
+// at most floor(tokens * group / R) + requests of them.  Workgroups without a tile are the last ones: between others they cost more than
+// themselves, since workgroups go to the parts of the card in turn, whichever have room (64 requests of 32 tokens behind 4096, 32 heads in groups of
+// 4, every second workgroup without a tile: EVERY2).  False for a tile that no request has.
 template <int R>
-__device__ __forceinline__ bool find_tile(const AttentionParams &p, int tile, QueryTile &q)
+__device__ __forceinline__ bool find_tile(const AttentionParams &p, int tile, QueryTile &q, int &split)
 {
-    const int lane = threadIdx.x & 63;
-    int context = p.prefix;
     if (p.shared) {
         q.b = 0, q.start = 0, q.count = p.tokens, q.row0 = tile * R;
-    } else {
-        // what the tensors say is cut to what the other arguments allow: wrong lengths give wrong sums, not wrong addresses
-        int before = 0;
-#pragma unroll 4
-        for (int b0 = 0; b0 < p.requests; b0 += 64) {
-            const int b = b0 + lane;
-            const int s = min(max(p.starts[min(b, p.requests)], 0), p.tokens);
-            before += __popcll(__ballot(b < p.requests && (int)((uint32_t)s * (uint32_t)p.group / R) + b <= tile));
-        }
-        q.b = __builtin_amdgcn_readfirstlane(max(before, 1) - 1);
-        q.start = min(max(p.starts[q.b], 0), p.tokens);
-        q.count = min(max(p.starts[q.b + 1] - q.start, 0), p.tokens - q.start);
-        context = p.contexts[q.b];
-        q.row0 = (tile - ((int)((uint32_t)q.start * (uint32_t)p.group / R) + q.b)) * R;
+        if (q.row0 >= q.count * p.group) return false;
+        q.rows = min(R, q.count * p.group - q.row0);
+        set_tile<true>(p, q, p.prefix);
+        return true;
     }
-    const int all = q.count * p.group;
-    if (q.row0 < 0 || q.row0 >= all || all <= p.few_rows) return false;
-    q.rows = min(R, all - q.row0);
-    if (p.shared) set_tile<true>(p, q, context);
-    else set_tile<false>(p, q, context);
+    const int lane = threadIdx.x & 63, last = p.requests - 1;
+    int context = 0;
+    // what the tensors say is cut to what the other arguments allow: wrong lengths give wrong sums, not wrong addresses
+    auto look = [&](int b0, auto chunks) {
+        constexpr int N = decltype(chunks)::value;
+        int start[N], count[N], contexts[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int b = min(b0 + 64 * n + lane, last);
+            start[n] = p.starts[b], count[n] = p.starts[b + 1], contexts[n] = p.contexts[b];
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int s = min(max(start[n], 0), p.tokens), c = min(max(count[n] - s, 0), p.tokens - s);
+            const uint32_t rows = b0 + 64 * n + lane > last ? 0u : (uint32_t)c * (uint32_t)p.group;
+            int own = rows <= (uint32_t)p.few_rows ? 0 : (int)((rows + R - 1) / R), upto = sum_upto(own), from = lane;
+            const int total = __builtin_amdgcn_readlane(upto, 63);
+            if (N == 1 && p.splits > 1 && split >= 0 && total > 0) {
+                const int at = split * p.tiles + tile;
+                split = at / total, tile = at - split * total;
+                if (split >= p.splits) tile = total;
+            }
+            if (N == 1 && total * p.kv_heads > 512) {      // more than run at once: the longest contexts first
+                const uint32_t key = (uint32_t)min(max(contexts[n], 0), (1 << 25) - 1) << 6 | (63 - lane);
+                int longer = 0;
+                for (int j = 0; j <= last; j++) longer += (uint32_t)__builtin_amdgcn_readlane((int)key, j) > key;
+                if (lane > last) longer = lane;
+                from = __builtin_amdgcn_ds_permute(4 * longer, lane);
+                own = __builtin_amdgcn_ds_permute(4 * longer, own);
+                upto = sum_upto(own);
+            }
+            if (tile >= 0 && tile < total) {
+                const int place = __popcll(__ballot(upto <= tile)), owner = __builtin_amdgcn_readlane(from, place);
+                q.b = b0 + 64 * n + owner;
+                q.start = __builtin_amdgcn_readlane(s, owner), q.count = __builtin_amdgcn_readlane(c, owner);
+                context = __builtin_amdgcn_readlane(contexts[n], owner);
+                q.row0 = (__builtin_amdgcn_readlane(upto, place) - 1 - tile) * R;
+                tile = -1;
+            } else if (tile >= 0) {
+                tile -= total;
+            }
+        }
+    };
+    if (last < 64) look(0, std::integral_constant<int, 1>{});
+    else
+        for (int b0 = 0; b0 <= last && tile >= 0; b0 += 256) look(b0, std::integral_constant<int, 4>{});
+    if (tile >= 0) return false;
+    q.rows = min(R, q.count * p.group - q.row0);
+    set_tile<false>(p, q, context);
     return true;
 }
 
@@ -170,11 +202,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
 
     const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    // the last rows of a request see the most keys: they come first
-    const int h = blockIdx.x % p.kv_heads, tile = p.tiles - 1 - blockIdx.x / p.kv_heads, split = blockIdx.y;
+    const int h = blockIdx.x % p.kv_heads, tile = blockIdx.x / p.kv_heads;
+    int split = blockIdx.y;
     QueryTile q;
     const int first_token = p.shared ? 0 : p.starts[0], end_token = p.shared ? p.tokens : p.starts[p.requests];
-    const bool found = find_tile<kTileRows>(p, tile, q);
+    const bool found = find_tile<kTileRows>(p, tile, q, split);
     if (!p.shared) clear_rest(p, first_token, end_token, (blockIdx.y * (long long)gridDim.x + blockIdx.x) * 256 + threadIdx.x, 256ll * gridDim.x * gridDim.y);
     if (!found) return;
     int chunk;

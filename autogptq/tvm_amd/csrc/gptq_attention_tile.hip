@@ -9,7 +9,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionPara
 {
     const int h = blockIdx.x % p.kv_heads, tile = blockIdx.x / p.kv_heads, r0 = blockIdx.y * kJoinRows;
     QueryTile q;
-    if (!find_tile<kTileRows>(p, tile, q) || r0 >= q.rows) return;
+    int split = -1;
+    if (!find_tile<kTileRows>(p, tile, q, split) || r0 >= q.rows) return;
     int chunk;
     const int parts = p.even ? even_parts(p, q.seen, chunk) : tile_parts(p, q.seen, kTileKeys, chunk);
     if (parts == 1 && p.prefix_parts == 0) return;

@@ -27,7 +27,7 @@
 namespace gptq {
 
 constexpr int kTileRows = 128;       // of a tile at most
-constexpr int kEvenRequests = 256;   // that even_parts looks at, at most
+constexpr int kEvenRequests = 256;   // that even_keys looks at, at most
 constexpr int kMostKeys = 1 << 29;   // of a request, a prefix, a window: sums of positions and widths stay within 32 bits
 
 // Workgroups of the few-rows kernel that a CU holds, by its registers: rt 16-row operands a wave, heads of up to `dim`.
@@ -67,7 +67,7 @@ struct AttentionParams {
     // the excess of the product, x times less than block_size, stays below 2^(29 + bits)
     uint32_t block_magic;
     int block_bits;
-    int even;                // kernel of tiles on a cache in MXFP4: the keys of a part follow from the lengths, see even_parts
+    int even;                // kernel of tiles on a cache in MXFP4: the keys of a part follow from the lengths, see even_keys
     int few_rows;            // kernel of tiles: requests of up to this many rows have a launch of the few-rows kernel
     int unit_bits;           // few-rows kernel on a cache in MXFP4: log2 of the keys of a unit, and 32 if requests of more than a tile are not its own
 };

@@ -155,7 +155,7 @@ int plan(const gptq_hip_attention &a, bool mx, Plan &pl)
         pl.mixed = mx && f.rt && B > 1 && B * H * keys >= 512ll * 1024 && by_units(f) == GPTQ_HIP_OK;
         const bool even = mx && B > 1 && B <= kEvenRequests && keys >= 6144;
         divide(d, kOwnWorkgroups, std::max(pl.mixed && even ? 1 : B, ceil_div(T * group, d.rows())) * H, keys, room);
-        // MXFP4: parts by the lengths on the GPU (even_parts), us by the longest context and so: 3 pieces of up to 300 tokens behind up to
+        // MXFP4: parts by the lengths on the GPU (even_keys), us by the longest context and so: 3 pieces of up to 300 tokens behind up to
         // 20000 keys 184 / 142, 20 of up to 33 behind 16000 135 / 88, 4 of 40 behind 8000 65 / 57; 60 of up to 99 behind 16000 281 / 288
         // (more tiles than workgroups), 16 of 20 behind 2068 48.0 / 51.9.
         if (even && d.splits > 1) {

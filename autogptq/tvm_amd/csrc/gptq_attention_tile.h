@@ -44,112 +44,50 @@ namespace gptq {
 constexpr int kTileKeys = 64;   // keys of a step
 constexpr int kJoinRows = 16;
 
-// The tile of a workgroup: the requests' tiles one after the other, the last rows of a request first (they see the most keys).  There are
-// at most floor(tokens * group / R) + requests of them.  Workgroups without a tile are the last ones: between others they cost more than
-// themselves, since workgroups go to the parts of the card in turn, whichever have room (64 requests of 32 tokens behind 4096, 32 heads in groups of
-// 4, every second workgroup without a tile: EVERY2).  False for a tile that no request has.
-template <int R>
-__device__ __forceinline__ bool find_tile(const AttentionParams &p, int tile, QueryTile &q, int &split)
+// Requests [base, base + 64), one a lane, as the kernel of tiles sees them.
+struct TileRequests {
+    int start, count, context;
+    int tiles, keys;       // tiles, and the keys that any of its tokens sees: no tile's list is longer
+};
+__device__ __forceinline__ TileRequests look_at_tiles(const AttentionParams &p, int base)
 {
-    if (p.shared) {
-        q.b = 0, q.start = 0, q.count = p.tokens, q.row0 = tile * R;
-        if (q.row0 >= q.count * p.group) return false;
-        q.rows = min(R, q.count * p.group - q.row0);
-        set_tile<true>(p, q, p.prefix);
-        return true;
-    }
-    const int lane = threadIdx.x & 63, last = p.requests - 1;
-    int context = 0;
     // what the tensors say is cut to what the other arguments allow: wrong lengths give wrong sums, not wrong addresses
-    auto look = [&](int b0, auto chunks) {
-        constexpr int N = decltype(chunks)::value;
-        int start[N], count[N], contexts[N];
-#pragma unroll
-        for (int n = 0; n < N; n++) {
-            const int b = min(b0 + 64 * n + lane, last);
-            start[n] = p.starts[b], count[n] = p.starts[b + 1], contexts[n] = p.contexts[b];
-        }
-#pragma unroll
-        for (int n = 0; n < N; n++) {
-            const int s = min(max(start[n], 0), p.tokens), c = min(max(count[n] - s, 0), p.tokens - s);
-            const uint32_t rows = b0 + 64 * n + lane > last ? 0u : (uint32_t)c * (uint32_t)p.group;
-            int own = rows <= (uint32_t)p.few_rows ? 0 : (int)((rows + R - 1) / R), upto = sum_upto(own), from = lane;
-            const int total = __builtin_amdgcn_readlane(upto, 63);
-            if (N == 1 && p.splits > 1 && split >= 0 && total > 0) {
-                const int at = split * p.tiles + tile;
-                split = at / total, tile = at - split * total;
-                if (split >= p.splits) tile = total;
-            }
-            if (N == 1 && total * p.kv_heads > 512) {      // more than run at once: the longest contexts first
-                const uint32_t key = (uint32_t)min(max(contexts[n], 0), (1 << 25) - 1) << 6 | (63 - lane);
-                int longer = 0;
-                for (int j = 0; j <= last; j++) longer += (uint32_t)__builtin_amdgcn_readlane((int)key, j) > key;
-                if (lane > last) longer = lane;
-                from = __builtin_amdgcn_ds_permute(4 * longer, lane);
-                own = __builtin_amdgcn_ds_permute(4 * longer, own);
-                upto = sum_upto(own);
-            }
-            if (tile >= 0 && tile < total) {
-                const int place = __popcll(__ballot(upto <= tile)), owner = __builtin_amdgcn_readlane(from, place);
-                q.b = b0 + 64 * n + owner;
-                q.start = __builtin_amdgcn_readlane(s, owner), q.count = __builtin_amdgcn_readlane(c, owner);
-                context = __builtin_amdgcn_readlane(contexts[n], owner);
-                q.row0 = (__builtin_amdgcn_readlane(upto, place) - 1 - tile) * R;
-                tile = -1;
-            } else if (tile >= 0) {
-                tile -= total;
-            }
-        }
-    };
-    if (last < 64) look(0, std::integral_constant<int, 1>{});
-    else
-        for (int b0 = 0; b0 <= last && tile >= 0; b0 += 256) look(b0, std::integral_constant<int, 4>{});
-    if (tile >= 0) return false;
-    q.rows = min(R, q.count * p.group - q.row0);
-    set_tile<false>(p, q, context);
-    return true;
+    const int b = base + (threadIdx.x & 63), last = p.requests - 1;
+    const int first = p.starts[min(b, last)], end = p.starts[min(b, last) + 1];
+    TileRequests r;
+    r.context = p.contexts[min(b, last)];
+    r.start = min(max(first, 0), p.tokens);
+    r.count = b > last ? 0 : min(max(end - r.start, 0), p.tokens - r.start);
+    const uint32_t rows = (uint32_t)r.count * (uint32_t)p.group;
+    r.tiles = rows <= (uint32_t)p.few_rows ? 0 : (int)((rows + kTileRows - 1) / kTileRows);
+    const int hi = max(min(r.context, held_keys(p)), 0), lo = p.window > 0 ? min(max(r.context - r.count - p.window + 1, 0), hi) : 0;
+    r.keys = p.front + min(p.sinks, lo) + hi - lo;
+    return r;
 }
 
-// The keys of a part, and how many parts the tile has.  A list that is longer than the host expected (splits * chunk) has
-// longer parts.
-__device__ __forceinline__ int tile_parts(const AttentionParams &p, int seen, int unit, int &chunk)
-{
-    chunk = max(p.chunk, ((seen + p.splits - 1) / p.splits + unit - 1) / unit * unit);
-    return max(1, (seen + chunk - 1) / chunk);
-}
-
-// Up to kEvenRequests requests: the smallest parts, in steps of 64 keys, with which all tiles together have no more parts than run at once, if
-// those are not longer than 1.5 times an even share; else the host's.  (The host knows the longest context only and divides as
-// if all had it, and counts no tiles that are not full.)  Every workgroup finds them for itself, of the same numbers by the same
-// operations; that and the places for twice as many parts cost 4 us, so that it is for long contexts: measured beside the choice.
+// Keys of a part, before they are cut to the tile's list.  Up to kEvenRequests requests: the smallest parts, in steps of 64 keys, with which all tiles
+// together have no more parts than run at once, if those are not longer than 1.5 times an even share; else the host's.  (The host knows the
+// longest context only and divides as if all had it, and counts no tiles that are not full.)  Every workgroup finds them for itself, of the
+// same numbers by the same operations; that and the places for twice as many parts cost 4 us, so that it is for long contexts:
+// measured beside the choice.
 template <int N>
-__device__ __forceinline__ int even_parts_of(const AttentionParams &p, int seen, int &chunk)
+__device__ __forceinline__ int even_keys(const AttentionParams &p, const TileRequests (&r)[N])
 {
-    const int lane = threadIdx.x & 63, last = p.requests - 1;
-    int steps[N], tiles[N], most = 0;      // of the requests 64 n + lane: steps of a tile, and tiles
+    int steps[N], most = 0;      // of a tile
     float all = 0.0f;
 #pragma unroll
     for (int n = 0; n < N; n++) {
-        steps[n] = tiles[n] = 0;
-        if (n && 64 * n > last) continue;
-        const int b = min(64 * n + lane, last), start = min(max(p.starts[b], 0), p.tokens);
-        int count = min(max(p.starts[b + 1] - start, 0), p.tokens - start);
-        if (64 * n + lane > last || (uint32_t)count * (uint32_t)p.group <= (uint32_t)p.few_rows) count = 0;
-        const int context = p.contexts[b];
-        const int hi = max(min(context, held_keys(p)), 0), lo = p.window > 0 ? min(max(context - count - p.window + 1, 0), hi) : 0;
-        const int keys = count > 0 ? p.front + min(p.sinks, lo) + hi - lo : 0;
-        tiles[n] = (int)(((uint32_t)count * (uint32_t)p.group + kTileRows - 1) / kTileRows);
-        steps[n] = (keys + kTileKeys - 1) / kTileKeys;
+        steps[n] = r[n].tiles ? (r[n].keys + kTileKeys - 1) / kTileKeys : 0;
         most = max(most, max_lanes(steps[n]));
         // (of wrong lengths the sums may be anything: every choice is a right one, and the same in every workgroup)
-        all += (float)__builtin_amdgcn_readlane(sum_upto(tiles[n] * ((steps[n] + 63) / 64)), 63) * 64.0f;
+        all += (float)__builtin_amdgcn_readlane(sum_upto(r[n].tiles * ((steps[n] + 63) / 64)), 63) * 64.0f;
     }
     const int share = (int)min(all * 1.5f * (float)p.kv_heads / (float)p.even, 1e6f), least = max(4, (most + p.splits - 1) / p.splits);
     auto fit = [&](int part) {
         const float per = __builtin_amdgcn_rcpf((float)part);
         int parts = 0;
 #pragma unroll
-        for (int n = 0; n < N; n++) parts += tiles[n] * (int)ceilf((float)steps[n] * per);
+        for (int n = 0; n < N; n++) parts += r[n].tiles * (int)ceilf((float)steps[n] * per);
         return (long long)__builtin_amdgcn_readlane(sum_upto(parts), 63) * p.kv_heads <= p.even;
     };
     int few = least, many = max(least, min(most, share));      // steps of a part
@@ -159,14 +97,85 @@ __device__ __forceinline__ int even_parts_of(const AttentionParams &p, int seen,
         if (fit(mid)) many = mid;
         else few = mid + 1;
     }
-    chunk = max(few * kTileKeys, ((seen + p.splits - 1) / p.splits + kTileKeys - 1) / kTileKeys * kTileKeys);
-    const int parts = max(1, (seen + chunk - 1) / chunk);
-    chunk = max(kTileKeys, ((seen + parts - 1) / parts + kTileKeys - 1) / kTileKeys * kTileKeys);     // the last one no shorter
-    return max(1, (seen + chunk - 1) / chunk);
+    return __builtin_amdgcn_readfirstlane(few * kTileKeys);
 }
-__device__ __forceinline__ int even_parts(const AttentionParams &p, int seen, int &chunk)
+
+// The tile and the part of workgroup `at` of those of a key/value head, or (JOIN) tile `at`; the keys of a part, and how many parts the tile has.
+// The requests come one after the other, the last rows of a request first (they see the most keys), and of up to 64 the longest contexts
+// first where not all workgroups run at once.  Workgroups without work are the last ones:
+// between others they cost more than themselves, since workgroups go to the parts of the card in turn, whichever have room (64
+// pieces of 32 tokens behind 4096, 32 heads in groups of 4, every second workgroup without a tile: 278 us, 175 so).  There are at
+// most floor(tokens * group / kTileRows) + requests tiles.  A list that is longer than the host expected (splits * chunk) has longer parts.
+// False for a workgroup without work.
+template <bool EVEN, bool JOIN>
+__device__ __forceinline__ bool find_tile(const AttentionParams &p, int at, QueryTile &q, int &split, int &chunk, int &parts)
 {
-    return p.requests <= 64 ? even_parts_of<1>(p, seen, chunk) : even_parts_of<kEvenRequests / 64>(p, seen, chunk);
+    const int lane = threadIdx.x & 63;
+    int base = p.chunk, context = p.prefix;
+    split = 0, q.row0 = -1;
+    // a request's tiles, each of as many parts as its longest list has
+    auto places = [&](const TileRequests &r) {
+        return r.tiles * (JOIN || p.splits == 1 ? 1 : r.keys > (long long)p.splits * base ? p.splits : max(1, (r.keys + base - 1) / base));
+    };
+    // workgroup `at` of those of request b, the `owner` of r
+    auto take = [&](const TileRequests &r, int b, int owner, int at) {
+        q.b = b, q.start = __builtin_amdgcn_readlane(r.start, owner), q.count = __builtin_amdgcn_readlane(r.count, owner);
+        context = __builtin_amdgcn_readlane(r.context, owner);
+        const int tiles = max(1, __builtin_amdgcn_readlane(r.tiles, owner));
+        if (!JOIN && p.splits > 1) split = __builtin_amdgcn_readfirstlane(at / tiles);
+        q.row0 = (tiles - 1 - (at - split * tiles)) * kTileRows;
+    };
+    if (p.shared) {
+        split = at / p.tiles;
+        q.b = 0, q.start = 0, q.count = p.tokens, q.row0 = (at - split * p.tiles) * kTileRows;
+    } else if (p.requests <= 64) {
+        const TileRequests r[1] = {look_at_tiles(p, 0)};
+        if (EVEN && p.even) base = even_keys(p, r);
+        int own = places(r[0]), from = lane, upto = sum_upto(own);
+        const int total = __builtin_amdgcn_readlane(upto, 63);
+        if (at >= total) return false;
+        if (!JOIN && total * p.kv_heads > (p.dim > 128 ? 256 : 512)) {
+            const uint32_t key = (uint32_t)min(max(r[0].context, 0), (1 << 25) - 1) << 6 | (63 - lane);
+            int longer = 0;
+            for (int j = 0; j < p.requests; j++) longer += (uint32_t)__builtin_amdgcn_readlane((int)key, j) > key;
+            if (lane >= p.requests) longer = lane;
+            from = __builtin_amdgcn_ds_permute(4 * longer, lane);
+            own = __builtin_amdgcn_ds_permute(4 * longer, own);
+            upto = sum_upto(own);
+        }
+        const int place = __popcll(__ballot(upto <= at)), owner = __builtin_amdgcn_readlane(from, place);
+        take(r[0], owner, owner, at - (__builtin_amdgcn_readlane(upto, place) - __builtin_amdgcn_readlane(own, place)));
+    } else {
+        constexpr int N = kEvenRequests / 64;
+        for (int b0 = 0; b0 < p.requests && q.row0 < 0; b0 += 64 * N) {
+            TileRequests r[N];
+#pragma unroll
+            for (int n = 0; n < N; n++) r[n] = look_at_tiles(p, b0 + 64 * n);
+            if (EVEN && p.even) base = even_keys(p, r);      // (there are no more requests)
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                const int own = places(r[n]), upto = sum_upto(own), total = __builtin_amdgcn_readlane(upto, 63);
+                if (q.row0 < 0 && at < total) {
+                    const int owner = __popcll(__ballot(upto <= at));
+                    take(r[n], b0 + 64 * n + owner, owner, at - (__builtin_amdgcn_readlane(upto, owner) - __builtin_amdgcn_readlane(own, owner)));
+                }
+                at -= total;
+            }
+        }
+    }
+    const int all = q.row0 < 0 ? 0 : q.count * p.group;
+    if (q.row0 < 0 || q.row0 >= all) return false;
+    q.rows = min(kTileRows, all - q.row0);
+    if (p.shared) set_tile<true>(p, q, context);
+    else set_tile<false>(p, q, context);
+    chunk = max(base, ((q.seen + p.splits - 1) / p.splits + kTileKeys - 1) / kTileKeys * kTileKeys);
+    parts = max(1, (q.seen + chunk - 1) / chunk);
+    if (EVEN && p.even) {      // the last one no shorter
+        chunk = max(kTileKeys, ((q.seen + parts - 1) / parts + kTileKeys - 1) / kTileKeys * kTileKeys);
+        parts = max(1, (q.seen + chunk - 1) / chunk);
+    }
+    chunk = __builtin_amdgcn_readfirstlane(chunk), parts = __builtin_amdgcn_readfirstlane(parts);
+    return JOIN || split < parts;
 }
 
 // 16 bytes of `src` to LDS at lds + 16 * lane.  Inline assembly, so that the compiler does not wait for every outstanding
@@ -202,16 +211,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
 
     const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int h = blockIdx.x % p.kv_heads, tile = blockIdx.x / p.kv_heads;
-    int split = blockIdx.y;
+    const int h = blockIdx.x % p.kv_heads;
+    int split, chunk, parts;
     QueryTile q;
     const int first_token = p.shared ? 0 : p.starts[0], end_token = p.shared ? p.tokens : p.starts[p.requests];
-    const bool found = find_tile<kTileRows>(p, tile, q, split);
+    const bool found = find_tile<MX, false>(p, blockIdx.y * p.tiles + blockIdx.x / p.kv_heads, q, split, chunk, parts);
     if (!p.shared) clear_rest(p, first_token, end_token, (blockIdx.y * (long long)gridDim.x + blockIdx.x) * 256 + threadIdx.x, 256ll * gridDim.x * gridDim.y);
     if (!found) return;
-    int chunk;
-    const int parts = MX && p.even ? even_parts(p, q.seen, chunk) : tile_parts(p, q.seen, KT, chunk);
-    if (split >= parts) return;
     const int begin = split * chunk, end = min(q.seen, begin + chunk);
     const int32_t *table = p.tables + (long long)q.b * p.table_stride;
     const char *kbase = (const char *)p.k + (long long)h * p.head_stride * (MX ? 1 : 2);
@@ -282,7 +288,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
     // (Taken anew for every use: what follows from the thread would else stand in registers that the kernel does not have.)
     auto this_thread = [&]() {
         int t = threadIdx.x;
-        if constexpr (DP != 128 || DC == 128) asm volatile("" : "+v"(t));
+        asm volatile("" : "+v"(t));
         return t;
     };
     // MX: the row whose codes a thread holds: the eight lanes that LDS takes at a time write eight chunks whose lowest bits differ
@@ -538,15 +544,8 @@ template <typename E, bool MX>
 static void launch_tile(const AttentionParams &p, hipStream_t stream)
 {
     const dim3 grid((unsigned)(p.kv_heads * p.tiles), (unsigned)p.splits);
-    // A CU holds three workgroups of rows of 64.  Where those that have rows are two a CU at most (and not many others run beside them) three
-    // would stand on some and one on others; LDS for two keeps it even.  Behind 4096 keys, 32 heads in groups of 4, us with LDS for two and
-    // for three: 8 pieces of 128 tokens (512 with rows of 640, two parts) 62 / 72, of 256 (512 of 576) 94 / 114, of 288 (576 of 640) 141 / 117,
-    // of 320 (640 of 704) 155 / 124; 16 of 64 behind 1000 (512 of 768, two parts) 39 / 30.  With 8 heads: 8 of 512 (512 of 544, two
-    // parts) 61 / 71, of 288 (576 of 640) 54 / 45; on the wrong side 8 of 256 (512 of 576, four parts) 52 / 43.
-    const long long groups = (long long)p.kv_heads * p.splits, full = ((long long)p.tokens * p.group + kTileRows - 1) / kTileRows;
-    const int least = groups * full <= 512 && groups * p.tiles <= 640 ? 56 * 1024 : 0;
 #define GPTQ_TILE(DP, DC) \
-    hipLaunchKernelGGL((attention_tile_kernel<E, DP, DC, MX>), grid, dim3(256), std::max(4 * kTileKeys * DP * 2 + (MX ? 16 : 8) * kTileKeys * 4, least), stream, p)
+    hipLaunchKernelGGL((attention_tile_kernel<E, DP, DC, MX>), grid, dim3(256), 4 * kTileKeys * DP * 2 + (MX ? 16 : 8) * kTileKeys * 4, stream, p)
     if (p.dim <= 64) GPTQ_TILE(64, 64);
     else if (p.dim <= 80) GPTQ_TILE(128, 80);
     else if (p.dim <= 96) GPTQ_TILE(128, 96);

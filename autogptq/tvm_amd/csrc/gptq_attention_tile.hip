@@ -9,10 +9,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionPara
 {
     const int h = blockIdx.x % p.kv_heads, tile = blockIdx.x / p.kv_heads, r0 = blockIdx.y * kJoinRows;
     QueryTile q;
-    int split = -1;
-    if (!find_tile<kTileRows>(p, tile, q, split) || r0 >= q.rows) return;
-    int chunk;
-    const int parts = p.even ? even_parts(p, q.seen, chunk) : tile_parts(p, q.seen, kTileKeys, chunk);
+    int split, chunk, parts;
+    if (!find_tile<true, true>(p, tile, q, split, chunk, parts) || r0 >= q.rows) return;
     if (parts == 1 && p.prefix_parts == 0) return;
     const long long all = (long long)p.tokens * p.heads;
     const int quads = p.dim / 4;

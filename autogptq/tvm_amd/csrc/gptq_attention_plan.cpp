@@ -75,8 +75,8 @@ void divide(Division &d, long long want, long long busy, long long keys, long lo
     d.splits = (int)std::max(1ll, ceil_div(keys, d.chunk));
 }
 // Own contexts on the tile kernel: two workgroups a CU (also where it holds three: 768 for dim 64 bring nothing), since they differ in length (32 heads in groups of 4; us with 256, 512 and
-// 1024 workgroups: 16 pieces of 20 tokens behind 2048 keys, dim 128: 51, 54, 62, dim 256: 136, 124, 140; 8 of 256 behind 4096: dim
-// 128: 182, 181, 216, dim 256: 462, 464, 542; 723 tokens of 7 heads behind up to 9001, dim 80: 107, 87, 90).  A shared prefix: parts of one length, which the
+// 1024 workgroups: 16 pieces of 20 tokens behind 2048 keys, dim 128: 43, 40, 53, dim 256: 85, 100, 127; 8 of 256 behind 4096: dim
+// 128: 161, 160, 190, dim 256: 431, 431, 510; 723 tokens of 7 heads behind up to 9001, dim 80: 94, 71, 81).  A shared prefix: parts of one length, which the
 // next launch reads again, so one a CU (512 rows behind 16384 keys: 256 workgroups 80 us, 512 84, 1024 111); rows that fit the
 // few-rows kernel two.
 constexpr long long kOwnWorkgroups = 512, kPrefixWorkgroups = 256;
@@ -154,10 +154,24 @@ int plan(const gptq_hip_attention &a, bool mx, Plan &pl)
         f.tiles = (int)B;
         pl.mixed = mx && f.rt && B > 1 && B * H * keys >= 512ll * 1024 && by_units(f) == GPTQ_HIP_OK;
         const bool even = mx && B > 1 && B <= kEvenRequests && keys >= 6144;
-        divide(d, kOwnWorkgroups, std::max(pl.mixed && even ? 1 : B, ceil_div(T * group, d.rows())) * H, keys, room);
+        long long busy = std::max(pl.mixed && even ? 1 : B, ceil_div(T * group, d.rows())) * H;
+        // MXFP4: no more parts than the card holds workgroups (512, of rows of more than 128 dims 256), and none where every CU has a tile of up
+        // to 2048 keys, since the parts' way through memory and their join cost some 17 us.  (8 key/value heads, us so and in parts for 512
+        // workgroups: 32 pieces of 32 tokens behind 512 22 / 39, 1024 35 / 47, 2048 61 / 66, 4096 103 / 102; 20 of 20, two parts or four,
+        // behind 1024 32 / 40, 4096 65 / 78; dim 256, 24 of 20 behind 1024 71 / 105, 4096 245 / 297, 40 of 20 behind 512 83 / 101,
+        // 4096, where 320 tiles would wait for one another, in two parts 445, undivided 535.)
+        long long want = kOwnWorkgroups;
+        if (mx && !even) {
+            busy = B * ceil_div(T * group, B * d.rows()) * H;      // (as many as requests of one length have)
+            if (a.cache.dim > 128) want /= 2;
+            if (busy >= 256 && keys <= 2048) want = 1;
+            else if (a.cache.dim > 128 && busy > want) want = 2 * want;
+            else want = std::max(1ll, want / busy) * busy;
+        }
+        divide(d, want, busy, keys, room);
         // MXFP4: parts by the lengths on the GPU (even_keys), us by the longest context and so: 3 pieces of up to 300 tokens behind up to
-        // 20000 keys 184 / 142, 20 of up to 33 behind 16000 135 / 88, 4 of 40 behind 8000 65 / 57; 60 of up to 99 behind 16000 281 / 288
-        // (more tiles than workgroups), 16 of 20 behind 2068 48.0 / 51.9.
+        // 20000 keys 230 / 198, 10 of up to 64 143 / 100, 20 of up to 33 behind 16000 138 / 85, 200 of 20 to 60 behind 8000, 2 heads, 174 / 165;
+        // 30 of 30 to 60 behind 7000, nearly a tile a workgroup as they are, 134 / 161; from 2048 keys on 24 of 50 behind 3000 75 / 79.
         if (even && d.splits > 1) {
             d.even = (int)(a.cache.dim > 128 ? kOwnWorkgroups / 2 : kOwnWorkgroups);     // (as many as the card holds)
             d.splits = (int)std::max(1ll, std::min({2ll * d.splits, ceil_div(keys, 256), room}));

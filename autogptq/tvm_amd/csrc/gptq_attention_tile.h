@@ -15,9 +15,8 @@
 //             rows' places come from a ring of lists in LDS, filled every four tiles by all waves at once, a tile each (one
 //             wave doing it for every tile held the others up at every barrier).
 //   parts     where a batch has fewer tiles than the card holds workgroups, each tile's keys are divided; a second launch joins
-//             the parts, 16 rows a workgroup.  (The last workgroup of a tile doing it, one for up to 128 rows: 16 pieces of
-//             20 tokens behind 2048 keys, dim 128, 73.6 us against 54.5; 5 of up to 333 behind up to 9001, dim 80, 77.7
-//             against 66.6.)
+//             the parts, 16 rows a workgroup.  (The last workgroup of a tile doing it, one for up to 128 rows, cost 16 pieces of
+//             20 tokens behind 2048 keys, dim 128, a third more, 5 of up to 333 behind up to 9001, dim 80, a sixth.)
 //   LDS       rows as they lie in the cache; the 16-byte chunk c of row r stands at c ^ t(r), the four low bits of r turned by two.
 //             Sixteen lanes read the same chunk of 16 keys at a time, and 32 lanes four chunks of four rows of values: t puts each on banks of
 //             its own (c ^ r and c ^ 2 r, which served sixteen lanes of the latter, cost a third of the cycles of LDS and 1 % of the
@@ -31,7 +30,7 @@
 // A cache in MXFP4 (MX).  LDS holds the same values at the same places.  A tile's codes come into registers a tile ahead, four threads a
 // row, and are turned into values (two an instruction, exactly) and written to LDS between the products, whose pipe they leave alone.
 // Measured as above: a prompt of 8192 tokens 573 to 586 us, 938 to 960 TFLOP/s; 128 single tokens behind a prefix of 16384 67 us, two launches and
-// the parts between them; 5 pieces of up to 333 behind up to 9001, dim 80, 75 us.
+// the parts between them; 5 pieces of up to 333 behind up to 9001, dim 80, 68 us.
 #pragma once
 #include <algorithm>
 #include <type_traits>

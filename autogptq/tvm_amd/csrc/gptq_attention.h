@@ -37,6 +37,7 @@ constexpr int few_resident(int rt, int dim, bool mx)
     return dim > 128 ? 1 : (rt == 1 ? 3 : 2) + (dim <= 64);
 }
 
+// (What a workgroup asks for before it has keys stands in the first three lines of 64 bytes: a fourth on that way costs a small call 0.2 us.)
 struct AttentionParams {
     const void *q, *k, *v;
     void *out;
@@ -52,6 +53,8 @@ struct AttentionParams {
     int prefix;
     int front;         // keys of a prefix that stands in front of every list
     int tiles, splits, chunk;   // tiles (bound), parts of a tile at most, keys of a part
+    int even;          // kernel of tiles on a cache in MXFP4: the keys of a part follow from the lengths, see even_keys
+    int few_rows;      // kernel of tiles: requests of up to this many rows have a launch of the few-rows kernel
     int prefix_parts;  // parts of a shared prefix to be joined with a tile's own
     int team, most_units;       // few-rows kernel: workgroups of a key/value head, units of a tile at most
     long long q_token, q_head, head_stride, table_stride;   // in elements
@@ -67,8 +70,6 @@ struct AttentionParams {
     // the excess of the product, x times less than block_size, stays below 2^(29 + bits)
     uint32_t block_magic;
     int block_bits;
-    int even;                // kernel of tiles on a cache in MXFP4: the keys of a part follow from the lengths, see even_keys
-    int few_rows;            // kernel of tiles: requests of up to this many rows have a launch of the few-rows kernel
     int unit_bits;           // few-rows kernel on a cache in MXFP4: log2 of the keys of a unit, and 32 if requests of more than a tile are not its own
 };
 

@@ -106,6 +106,8 @@ __device__ __forceinline__ int even_keys(const AttentionParams &p, const TileReq
 // pieces of 32 tokens behind 4096, 32 heads in groups of 4, every second workgroup without a tile: 278 us, 175 so).  There are at
 // most floor(tokens * group / kTileRows) + requests tiles.  A list that is longer than the host expected (splits * chunk) has longer parts.
 // False for a workgroup without work.
+// What small calls have no use for stands out of their way, and is short: all of it is on the way of code into an empty cache (16 bits, a chunk of 17 tokens, dim 64,
+// 6.9 to 6.6 us with the order of the arguments, 100 pieces of 20 tokens 16.8 to 16.1 with 64 requests at a time).
 template <bool EVEN, bool JOIN>
 __device__ __forceinline__ bool find_tile(const AttentionParams &p, int at, QueryTile &q, int &split, int &chunk, int &parts)
 {
@@ -127,13 +129,13 @@ __device__ __forceinline__ bool find_tile(const AttentionParams &p, int at, Quer
     if (p.shared) {
         split = at / p.tiles;
         q.b = 0, q.start = 0, q.count = p.tokens, q.row0 = (at - split * p.tiles) * kTileRows;
-    } else if (p.requests <= 64) {
+    } else if (__builtin_expect(p.requests <= 64, 1)) {
         const TileRequests r[1] = {look_at_tiles(p, 0)};
         if (EVEN && p.even) base = even_keys(p, r);
         int own = places(r[0]), from = lane, upto = sum_upto(own);
         const int total = __builtin_amdgcn_readlane(upto, 63);
         if (at >= total) return false;
-        if (!JOIN && total * p.kv_heads > (p.dim > 128 ? 256 : 512)) {
+        if (!JOIN && __builtin_expect(total * p.kv_heads > (p.dim > 128 ? 256 : 512), 0)) {
             const uint32_t key = (uint32_t)min(max(r[0].context, 0), (1 << 25) - 1) << 6 | (63 - lane);
             int longer = 0;
             for (int j = 0; j < p.requests; j++) longer += (uint32_t)__builtin_amdgcn_readlane((int)key, j) > key;
@@ -145,7 +147,7 @@ __device__ __forceinline__ bool find_tile(const AttentionParams &p, int at, Quer
         const int place = __popcll(__ballot(upto <= at)), owner = __builtin_amdgcn_readlane(from, place);
         take(r[0], owner, owner, at - (__builtin_amdgcn_readlane(upto, place) - __builtin_amdgcn_readlane(own, place)));
     } else {
-        constexpr int N = kEvenRequests / 64;
+        constexpr int N = EVEN ? kEvenRequests / 64 : 1;     // (waves of requests at a time)
         for (int b0 = 0; b0 < p.requests && q.row0 < 0; b0 += 64 * N) {
             TileRequests r[N];
 #pragma unroll

@@ -3,14 +3,15 @@
 
 namespace gptq {
 
-// Joins the parts of tiles that are divided, or stand behind a shared prefix: kJoinRows rows of a tile a workgroup.
-template <typename E>
+// Joins the parts of tiles that are divided, or stand behind a shared prefix: kJoinRows rows of a tile a workgroup.  EVEN: the parts' keys follow from the
+// lengths.
+template <typename E, bool EVEN>
 __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionParams p)
 {
     const int h = blockIdx.x % p.kv_heads, tile = blockIdx.x / p.kv_heads, r0 = blockIdx.y * kJoinRows;
     QueryTile q;
     int split, chunk, parts;
-    if (!find_tile<true, true>(p, tile, q, split, chunk, parts) || r0 >= q.rows) return;
+    if (!find_tile<EVEN, true>(p, tile, q, split, chunk, parts) || r0 >= q.rows) return;
     if (parts == 1 && p.prefix_parts == 0) return;
     const long long all = (long long)p.tokens * p.heads;
     const int quads = p.dim / 4;
@@ -28,8 +29,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionPara
 void launch_attention_join(const AttentionParams &p, int type, unsigned tiles, void *stream)
 {
     const dim3 grid(tiles, kTileRows / kJoinRows);
-    if (type == GPTQ_HIP_TYPE_FP16) hipLaunchKernelGGL(attention_join_kernel<_Float16>, grid, dim3(256), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(attention_join_kernel<__bf16>, grid, dim3(256), 0, (hipStream_t)stream, p);
+    auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, p); };
+    if (type == GPTQ_HIP_TYPE_FP16) p.even ? join(attention_join_kernel<_Float16, true>) : join(attention_join_kernel<_Float16, false>);
+    else p.even ? join(attention_join_kernel<__bf16, true>) : join(attention_join_kernel<__bf16, false>);
 }
 
 int launch_attention_tile(const AttentionParams &p, int type, void *stream) { return launch_tile_of<false>(p, type, stream); }

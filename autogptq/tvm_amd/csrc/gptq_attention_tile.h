@@ -101,9 +101,11 @@ __device__ __forceinline__ int even_keys(const AttentionParams &p, const TileReq
 
 // The tile and the part of workgroup `at` of those of a key/value head, or (JOIN) tile `at`; the keys of a part, and how many parts the tile has.
 // The requests come one after the other, the last rows of a request first (they see the most keys), and of up to 64 the longest contexts
-// first where not all workgroups run at once.  Workgroups without work are the last ones:
-// between others they cost more than themselves, since workgroups go to the parts of the card in turn, whichever have room (64
-// pieces of 32 tokens behind 4096, 32 heads in groups of 4, every second workgroup without a tile: 278 us, 175 so).  There are at
+// first where not all workgroups run at once.  If all tiles of up to 64 requests have as many parts, the first parts come before the second
+// ones: the last ones are the shortest, and share a CU where there are more workgroups than CUs (4 pieces of 64 tokens behind 1000, five parts,
+// 320 workgroups, us a request after the other and so: 16 bits, dim 64 18.4 / 17.1, dim 128 25.8 / 24.0, MXFP4 28.5 / 25.3).  Workgroups
+// without work are the last ones: between others they cost more than themselves, since workgroups go to the parts of the card in turn,
+// whichever have room (64 pieces of 32 tokens behind 4096, 32 heads in groups of 4, every second workgroup without a tile: 278 us, 175 so).  There are at
 // most floor(tokens * group / kTileRows) + requests tiles.  A list that is longer than the host expected (splits * chunk) has longer parts.
 // False for a workgroup without work.
 // What small calls have no use for stands out of their way, and is short: all of it is on the way of code into an empty cache (16 bits, a chunk of 17 tokens, dim 64,
@@ -114,17 +116,17 @@ __device__ __forceinline__ bool find_tile(const AttentionParams &p, int at, Quer
     const int lane = threadIdx.x & 63;
     int base = p.chunk, context = p.prefix;
     split = 0, q.row0 = -1;
-    // a request's tiles, each of as many parts as its longest list has
-    auto places = [&](const TileRequests &r) {
-        return r.tiles * (JOIN || p.splits == 1 ? 1 : r.keys > (long long)p.splits * base ? p.splits : max(1, (r.keys + base - 1) / base));
+    // parts of a request's tiles: as many as its longest list has
+    auto parts_of = [&](const TileRequests &r) {
+        return JOIN || p.splits == 1 ? 1 : r.keys > (long long)p.splits * base ? p.splits : max(1, (r.keys + base - 1) / base);
     };
     // workgroup `at` of those of request b, the `owner` of r
-    auto take = [&](const TileRequests &r, int b, int owner, int at) {
+    auto take = [&](const TileRequests &r, int b, int owner, int at, bool known) {
         q.b = b, q.start = __builtin_amdgcn_readlane(r.start, owner), q.count = __builtin_amdgcn_readlane(r.count, owner);
         context = __builtin_amdgcn_readlane(r.context, owner);
         const int tiles = max(1, __builtin_amdgcn_readlane(r.tiles, owner));
-        if (!JOIN && p.splits > 1) split = __builtin_amdgcn_readfirstlane(at / tiles);
-        q.row0 = (tiles - 1 - (at - split * tiles)) * kTileRows;
+        if (!JOIN && p.splits > 1 && !known) split = __builtin_amdgcn_readfirstlane(at / tiles), at -= split * tiles;
+        q.row0 = (tiles - 1 - at) * kTileRows;
     };
     if (p.shared) {
         split = at / p.tiles;
@@ -132,7 +134,23 @@ __device__ __forceinline__ bool find_tile(const AttentionParams &p, int at, Quer
     } else if (__builtin_expect(p.requests <= 64, 1)) {
         const TileRequests r[1] = {look_at_tiles(p, 0)};
         if (EVEN && p.even) base = even_keys(p, r);
-        int own = places(r[0]), from = lane, upto = sum_upto(own);
+        int own = r[0].tiles, from = lane;
+        bool alike = false;
+        if (!JOIN && p.splits > 1) {
+            const int mine = parts_of(r[0]);
+            const unsigned long long with = __ballot(own > 0);
+            if (!with) return false;
+            const int each = __builtin_amdgcn_readlane(mine, __builtin_ctzll(with));
+            alike = !__ballot(own > 0 && mine != each);
+            if (alike) {
+                const int all = __builtin_amdgcn_readlane(sum_upto(own), 63);
+                split = __builtin_amdgcn_readfirstlane(at / all), at -= split * all;
+                if (split >= each) return false;
+            } else {
+                own *= mine;
+            }
+        }
+        int upto = sum_upto(own);
         const int total = __builtin_amdgcn_readlane(upto, 63);
         if (at >= total) return false;
         if (!JOIN && __builtin_expect(total * p.kv_heads > (p.dim > 128 ? 256 : 512), 0)) {
@@ -145,7 +163,7 @@ __device__ __forceinline__ bool find_tile(const AttentionParams &p, int at, Quer
             upto = sum_upto(own);
         }
         const int place = __popcll(__ballot(upto <= at)), owner = __builtin_amdgcn_readlane(from, place);
-        take(r[0], owner, owner, at - (__builtin_amdgcn_readlane(upto, place) - __builtin_amdgcn_readlane(own, place)));
+        take(r[0], owner, owner, at - (__builtin_amdgcn_readlane(upto, place) - __builtin_amdgcn_readlane(own, place)), alike);
     } else {
         constexpr int N = EVEN ? kEvenRequests / 64 : 1;     // (waves of requests at a time)
         for (int b0 = 0; b0 < p.requests && q.row0 < 0; b0 += 64 * N) {
@@ -155,10 +173,10 @@ __device__ __forceinline__ bool find_tile(const AttentionParams &p, int at, Quer
             if (EVEN && p.even) base = even_keys(p, r);      // (there are no more requests)
 #pragma unroll
             for (int n = 0; n < N; n++) {
-                const int own = places(r[n]), upto = sum_upto(own), total = __builtin_amdgcn_readlane(upto, 63);
+                const int own = r[n].tiles * parts_of(r[n]), upto = sum_upto(own), total = __builtin_amdgcn_readlane(upto, 63);
                 if (q.row0 < 0 && at < total) {
                     const int owner = __popcll(__ballot(upto <= at));
-                    take(r[n], b0 + 64 * n + owner, owner, at - (__builtin_amdgcn_readlane(upto, owner) - __builtin_amdgcn_readlane(own, owner)));
+                    take(r[n], b0 + 64 * n + owner, owner, at - (__builtin_amdgcn_readlane(upto, owner) - __builtin_amdgcn_readlane(own, owner)), false);
                 }
                 at -= total;
             }

@@ -106,8 +106,7 @@ struct CacheRead {
     int block_size, blocks;
 };
 
-// MX: rows of codes, given as values of E; else rows of 16-bit values as they are.  PAST: results go past the caches, where there are
-// more of them than the caches hold (32768 tokens of 8 heads of 128, 170 MB in and out: 27.6 us, 6.2 TB/s; 43 through them).
+// MX: rows of codes, given as values of E; else rows of 16-bit values as they are.  PAST: results go past the caches.
 template <typename E, bool MX, bool PAST>
 __global__ __launch_bounds__(256) void cache_read_kernel(const CacheRead p)
 {
@@ -144,7 +143,10 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const CacheRead p)
 template <typename E, bool MX>
 static void launch_read(const CacheRead &p, unsigned grid, hipStream_t stream)
 {
-    const bool past = (unsigned long long)p.tokens * p.row_chunks * 32 >= 32ull << 20;      // the second-level caches' 8 times 4 MiB
+    // MiB of results, us past the caches and through them, 8 heads of 128: MXFP4 8 5.4 / 5.4, 12 5.4 / 5.3, 16 5.4 / 5.9, 20 5.3 / 6.7, 24 6.8 / 7.7, 32 8.8 / 9.2, 128
+    // 27.8 / 28.5 (6.2 TB/s), 256 53 / 83; 16 bits, whose rows are read in as much, 8 5.4 / 5.4, 12 5.6 / 5.9, 16 7.2 / 7.1, 24 9.2 / 9.4, 32 11.9 / 11.8, 64 21.3 / 22.7,
+    // 80 25.8 / 28.6, 128 48.5 / 41.7 (three calls' rows and results in turn, of which the last cache then keeps a part), 256 96 / 104
+    const bool past = (unsigned long long)p.tokens * p.row_chunks * 32 > 12ull << 20;
     if (past) hipLaunchKernelGGL((cache_read_kernel<E, MX, true>), dim3(grid), dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((cache_read_kernel<E, MX, false>), dim3(grid), dim3(256), 0, stream, p);
 }

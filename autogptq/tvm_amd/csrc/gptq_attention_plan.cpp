@@ -129,10 +129,12 @@ int plan(const gptq_hip_attention &a, bool mx, Plan &pl)
         const long long most = B * (T * group / d.rows() + 1);    // tiles, whatever the lengths on the GPU say
         if (most > 1ll << 30) return GPTQ_HIP_ERR_UNSUPPORTED;
         d.most_units = (int)std::min((1ll << 30) / most, 1ll << 20);
-        // (MXFP4: up to 512 keys in units of 128 where there are workgroups for all of them, since a wave's second 32 keys wait for memory
-        // once more: 7.5 us for 512, in units of 256 8.0; 2048 9.7 and 8.5, since eight more parts are joined)
+        // MXFP4: units of 128 keys in place of 256 where each of them has a CU to itself, since a wave's second 32 keys wait for memory once more; not
+        // for one unit, which needs no join, nor for more than eight.  (Contexts of single tokens, 8 key/value heads, us in units of 128 and 256: one of 200 7.5 / 6.5,
+        // 300 7.5 / 8.1, 512 7.5 / 8.1, 640 7.6 / 8.1, 768 7.8 / 8.2, 1024 8.0 / 8.2, 1536 8.8 / 8.3; four of 1024, 256 units, 8.1 / 8.3; eight of 512, 256 units, 7.8 / 8.2, of
+        // 520, 320 units, 8.4 / 8.2; sixteen of 300, 384 units, 8.5 / 8.3; dim 256, three of 768 9.0 / 9.5.)
         const long long team = 256ll * few_resident(d.rt, a.cache.dim, mx) / H;
-        if (mx && keys <= 512 && d.tiles * std::max(1ll, ceil_div(keys, 128)) <= team) d.unit_bits = 7;
+        if (mx && keys > 256 && keys <= 1024 && B * H * ceil_div(keys, 128) <= 256) d.unit_bits = 7;
         const long long units = (d.tiles + 0ll) * std::max(1ll, ceil_div(keys, 1ll << d.unit_bits));
         d.team = (int)std::max(1ll, std::min(team, units));
         if (d.team * H > (long long)(kAttentionCounters / 4)) return GPTQ_HIP_ERR_UNSUPPORTED;

@@ -1,7 +1,10 @@
 """The order in which the tiles and parts of a step are dealt: tiles that all have as many parts, and tiles that do not."""
+import ctypes
+
 import pytest
 import torch
 
+from autogptq.tvm_amd import _lib
 from tests.attention_util import Step, assert_attention
 from tests.mxfp4_util import MxStep
 from tests.test_attention import attend
@@ -41,3 +44,35 @@ def test_lengths_that_the_host_did_not_expect(made):
     s = made(42, [(3000, 40), (2900, 40), (2950, 33)], 8, 2, 64, 16)
     for hint in (600, 1500, 100000):
         assert_attention(attend(s, max_context=hint), s, f"max_context={hint}")
+
+
+def mx_workspace(requests, tokens, context, heads, kv_heads, dim, window=0, prefix=0):
+    """Bytes that a call over a cache in MXFP4 needs (blocks of 16 tokens, a table as wide as the context)."""
+    p = 0x1000
+    groups, scale = -(-dim // 32), 2 if dim <= 64 else 4 if dim <= 128 else 8
+    cache = _lib.CacheMx(k=p, v=p, k_scales=p, v_scales=p, type=0, blocks=1000, block_size=16, heads=kv_heads, dim=dim,
+                         block_stride=256 * groups * kv_heads, slot_stride=16 * groups, head_stride=256 * groups,
+                         scale_block_stride=16 * scale * kv_heads, scale_slot_stride=scale, scale_head_stride=16 * scale)
+    a = _lib.Attention()
+    a.q = a.out = a.tables = a.starts = a.contexts = a.prefix_blocks = p
+    a.tokens, a.requests, a.heads, a.max_context, a.window, a.prefix_length, a.scale = tokens, requests, heads, context, window, prefix, 0.1
+    a.table_width = a.table_stride = -(-context // 16)
+    a.q_token_stride, a.q_head_stride = heads * dim, dim
+    return _lib.lib().gptq_hip_attention_mx_workspace_bytes(ctypes.byref(cache), ctypes.byref(a))
+
+
+def size_of(rows, dim):
+    """... that the parts of so many rows take: counters, two statistics and dim values a row."""
+    return 65536 + -(-rows * 8 // 256) * 256 + rows * dim * 4
+
+
+@pytest.mark.parametrize("requests, context, kv_heads, dim, units", [
+    (1, 128, 8, 128, 1), (1, 200, 8, 128, 1), (1, 256, 8, 128, 1), (16, 256, 8, 128, 1),       # one of 256: no parts to join
+    (1, 257, 8, 128, 3), (1, 512, 8, 128, 4), (1, 768, 8, 128, 6), (1, 1024, 8, 128, 8), (4, 1024, 8, 64, 8), (3, 700, 2, 256, 6),
+    (8, 512, 8, 128, 4), (1, 1025, 8, 128, 5), (1, 2048, 8, 128, 8),
+    (8, 520, 8, 128, 3), (16, 300, 8, 128, 2), (33, 129, 8, 128, 1)])                          # more than a CU each
+def test_units_of_short_contexts(requests, context, kv_heads, dim, units):
+    """A single token's keys are dealt in units of 128 where those are up to eight, more than one of 256, and have a CU each; else of 256."""
+    tiles = requests * 4 // 16 + requests
+    rows = 2 * min(256 * (2 if dim > 128 else 4) // kv_heads, tiles * units) * kv_heads * 16
+    assert mx_workspace(requests, requests, context, 4 * kv_heads, kv_heads, dim) == size_of(rows, dim)

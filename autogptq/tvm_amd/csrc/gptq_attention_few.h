@@ -14,7 +14,7 @@
 //                           two keys' dwords by one byte permute.  Operand row i of tile t is then dim 8 i + t, and a
 //                           result lane holds eight neighbouring dims of a row.
 //
-// The division.  Two to four workgroups fill a CU's registers, so a grid with a workgroup for every part that
+// The division.  One to four workgroups fill a CU's registers, so a grid with a workgroup for every part that
 // a request might have spends its time on those that find none (16 contexts of up to 32768 tokens: 146 us, with the
 // division below 70).  Instead a head has `team` workgroups, as many as run at once, and each takes the same number of units
 // of up to 256 keys of the requests' tiles, one after the other, in the order of the requests: a workgroup ends one tile, takes
@@ -80,7 +80,6 @@ __global__ __launch_bounds__(64 * kFewWaves, few_resident(RT, DP, MX)) void atte
     constexpr int VH = DP / 16 / VE;               // ... that many times
     constexpr int VW = VE / 2;                     // dwords of that
     constexpr int OD = DP + 4;                     // row of O in LDS
-    constexpr int GW = DP > 128 ? 2 : 1;           // MX: words of a row's scales
     __shared__ uint32_t list[MX ? 1 : NW][2][64];
     __shared__ float stat_m[NW][16 * RT], stat_l[NW][16 * RT];
     __shared__ __align__(16) float join[NW * 16 * OD];

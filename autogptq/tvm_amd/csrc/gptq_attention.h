@@ -54,7 +54,7 @@ struct AttentionParams {
     int front;         // keys of a prefix that stands in front of every list
     int tiles, splits, chunk;   // tiles (bound), parts of a tile at most, keys of a part
     int even;          // kernel of tiles on a cache in MXFP4: the keys of a part follow from the lengths, see even_keys
-    int few_rows;      // kernel of tiles: requests of up to this many rows have a launch of the few-rows kernel
+    int few_rows;      // requests of up to this many rows (a tile of it) are the few-rows kernel's, others the kernel of tiles'; 0: all are one kernel's
     int prefix_parts;  // parts of a shared prefix to be joined with a tile's own
     int team, most_units;       // few-rows kernel: workgroups of a key/value head, units of a tile at most
     long long q_token, q_head, head_stride, table_stride;   // in elements
@@ -70,7 +70,7 @@ struct AttentionParams {
     // the excess of the product, x times less than block_size, stays below 2^(29 + bits)
     uint32_t block_magic;
     int block_bits;
-    int unit_bits;           // few-rows kernel on a cache in MXFP4: log2 of the keys of a unit, and 32 if requests of more than a tile are not its own
+    int unit_bits;           // few-rows kernel on a cache in MXFP4: log2 of the keys of a unit
 };
 
 // x / group for the rows of a tile, counted from its first token's

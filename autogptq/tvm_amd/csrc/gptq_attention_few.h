@@ -61,10 +61,10 @@ __device__ __forceinline__ Requests look_at(const AttentionParams &p, int base)
     const int hi = max(min(r.context, held_keys(p)), 0);
     const int lo = p.window > 0 ? min(max(r.context - r.count - p.window + 1, 0), hi) : 0;
     const int seen = p.front + min(p.sinks, lo) + hi - lo;
-    r.units = min(max(1, MX ? (seen + (1 << (p.unit_bits & 31)) - 1) >> (p.unit_bits & 31) : (seen + kFewUnit - 1) / kFewUnit), p.most_units);
+    r.units = min(max(1, MX ? (seen + (1 << p.unit_bits) - 1) >> p.unit_bits : (seen + kFewUnit - 1) / kFewUnit), p.most_units);
     r.keys = max(32, ((seen + r.units - 1) / r.units + 31) / 32 * 32);
     const int tiles = (int)(((uint32_t)r.count * (uint32_t)p.group + R - 1) / R);
-    r.total = MX && p.unit_bits & 32 && tiles > 1 ? 0 : tiles * r.units;
+    r.total = MX && p.few_rows && tiles > 1 ? 0 : tiles * r.units;
     return r;
 }
 // DP: compiled width, the dims past p.dim do not count; FULL: there are none; RT: 16-row operands a wave holds; SHARED: the parts of a

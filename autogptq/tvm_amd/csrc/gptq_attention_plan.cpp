@@ -242,7 +242,7 @@ int attend(const gptq_hip_attention *a, const gptq_hip_cache_mx *mx, void *works
     while (p.block_bits < 31 && 1ll << p.block_bits < c.block_size) p.block_bits++;
     p.block_magic = (uint32_t)(((1ull << (29 + p.block_bits)) + (unsigned)c.block_size - 1) / (unsigned)c.block_size);
     auto launch = [&](const Division &d) {
-        p.tiles = d.tiles, p.splits = d.splits, p.chunk = d.chunk, p.team = d.team, p.most_units = d.most_units, p.unit_bits = d.unit_bits | (&d == &pl.few ? 32 : 0), p.even = d.even;
+        p.tiles = d.tiles, p.splits = d.splits, p.chunk = d.chunk, p.team = d.team, p.most_units = d.most_units, p.unit_bits = d.unit_bits, p.even = d.even;
         if (d.rt) return mx ? launch_attention_few_mx(p, c.type, d.rt, stream) : launch_attention_few(p, c.type, d.rt, stream);
         return mx ? launch_attention_tile_mx(p, c.type, stream) : launch_attention_tile(p, c.type, stream);
     };

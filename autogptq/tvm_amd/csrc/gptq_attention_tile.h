@@ -312,14 +312,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
     };
     // MX: the row whose codes a thread holds: the eight lanes that LDS takes at a time write eight chunks whose lowest bits differ
     auto row_of_codes = [](int thread) { return thread >> 6 << 4 | (thread << 2 & 12) | (thread >> 2 & 3); };
-    // Where its part of a row goes, from a tile's beginning: keys in the lower half of the word, values in the upper.  (Dynamic LDS begins at 0,
-    // so that the swizzle is in the low bits of the sum.)
+    // Where its part of a row goes, from a tile's beginning.  (Dynamic LDS begins at 0, so that the swizzle is in the low bits of the sum.)
     auto find_place = [&]() {
         const int thread = this_thread(), code_row = row_of_codes(thread), chunk = (thread >> 4 & 3) * DW;
-        return (uint32_t)(code_row * (DP * 2) + (chunk ^ turn(code_row)) * 16) |
-               (uint32_t)(code_row * (DP * 2) + (chunk ^ turn(code_row)) * 16) << 16;
+        return (uint32_t)(code_row * (DP * 2) + (chunk ^ turn(code_row)) * 16);
     };
-    static_assert(TILE <= 1 << 16, "");
     const uint32_t kept_place = MX && DP <= 128 ? find_place() : 0;
     auto place_of_part = [&]() { return DP <= 128 ? kept_place : find_place(); };
     auto fetch = [&](int n, const char *from, const void *scales) {
@@ -354,8 +351,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DP == 128 ? 2 : 3) void attent
             if (w >= w0 && w < w1)
                 *(__attribute__((address_space(3))) u4 *)(uintptr_t)(row ^ (w * 16)) = mx_values<E>(x.codes[w], (w < 4 ? x.scales : x.scales >> 8) << 23);
     };
-    auto put_keys = [&](const Coded &x, int buf, int w0 = 0, int w1 = 8) { put(x, w0, w1, lds + buf * TILE + (place_of_part() & 0xffffu)); };
-    auto put_values = [&](const Coded &x, int buf, int w0 = 0, int w1 = 8) { put(x, w0, w1, lds + (2 + buf) * TILE + (place_of_part() >> 16)); };
+    auto put_keys = [&](const Coded &x, int buf, int w0 = 0, int w1 = 8) { put(x, w0, w1, lds + buf * TILE + place_of_part()); };
+    auto put_values = [&](const Coded &x, int buf, int w0 = 0, int w1 = 8) { put(x, w0, w1, lds + (2 + buf) * TILE + place_of_part()); };
     auto meet_lds = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
     float m = kNone, l = 0.0f;

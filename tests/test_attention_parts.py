@@ -46,7 +46,7 @@ def test_lengths_that_the_host_did_not_expect(made):
         assert_attention(attend(s, max_context=hint), s, f"max_context={hint}")
 
 
-def mx_workspace(requests, tokens, context, heads, kv_heads, dim, window=0, prefix=0):
+def mx_workspace(tokens, requests, context, heads, kv_heads, dim, window=0, sinks=0, prefix=0):
     """Bytes that a call over a cache in MXFP4 needs (blocks of 16 tokens, a table as wide as the context)."""
     p = 0x1000
     groups, scale = -(-dim // 32), 2 if dim <= 64 else 4 if dim <= 128 else 8
@@ -55,7 +55,8 @@ def mx_workspace(requests, tokens, context, heads, kv_heads, dim, window=0, pref
                          scale_block_stride=16 * scale * kv_heads, scale_slot_stride=scale, scale_head_stride=16 * scale)
     a = _lib.Attention()
     a.q = a.out = a.tables = a.starts = a.contexts = a.prefix_blocks = p
-    a.tokens, a.requests, a.heads, a.max_context, a.window, a.prefix_length, a.scale = tokens, requests, heads, context, window, prefix, 0.1
+    a.tokens, a.requests, a.heads, a.max_context, a.scale = tokens, requests, heads, context, 0.1
+    a.window, a.sinks, a.prefix_length = window, sinks, prefix
     a.table_width = a.table_stride = -(-context // 16)
     a.q_token_stride, a.q_head_stride = heads * dim, dim
     return _lib.lib().gptq_hip_attention_mx_workspace_bytes(ctypes.byref(cache), ctypes.byref(a))

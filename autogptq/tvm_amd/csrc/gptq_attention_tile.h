@@ -65,8 +65,10 @@ __device__ __forceinline__ TileRequests look_at_tiles(const AttentionParams &p, 
 }
 
 // Keys of a part, before they are cut to the tile's list.  Up to kEvenRequests requests: the smallest parts, in steps of 64 keys, with which all tiles
-// together have no more parts than run at once, if those are not longer than 1.5 times an even share; else the host's.  (The host knows the
-// longest context only and divides as if all had it, and counts no tiles that are not full.)  Every workgroup finds them for itself, of the
+// together have no more parts than run at once, if those are not longer than 1.5 times an even share, or than the host's; else the host's.  (The host
+// knows the longest context only and divides as if all had it, and counts no tiles that are not full.  Where tiles of short lists leave the
+// long ones no parts, the host's take several rounds, but are done sooner: dim 256, 5 pieces of up to 333 tokens behind up to 9001 keys 510 us as they
+// fit at once, 367 so, 8 behind up to 9000 533 / 393.)  Every workgroup finds them for itself, of the
 // same numbers by the same operations; that and the places for twice as many parts cost 4 us, so that it is for long contexts:
 // measured beside the choice.
 template <int N>
@@ -79,7 +81,7 @@ __device__ __forceinline__ int even_keys(const AttentionParams &p, const TileReq
         steps[n] = r[n].tiles ? (r[n].keys + kTileKeys - 1) / kTileKeys : 0;
         most = max(most, max_lanes(steps[n]));
         // (of wrong lengths the sums may be anything: every choice is a right one, and the same in every workgroup)
-        all += (float)__builtin_amdgcn_readlane(sum_upto(r[n].tiles * ((steps[n] + 63) / 64)), 63) * 64.0f;
+        all += (float)__builtin_amdgcn_readlane(sum_upto(r[n].tiles * ((steps[n] + 7) / 8)), 63) * 8.0f;
     }
     const int share = (int)min(all * 1.5f * (float)p.kv_heads / (float)p.even, 1e6f), least = max(4, (most + p.splits - 1) / p.splits);
     auto fit = [&](int part) {
@@ -89,8 +91,9 @@ __device__ __forceinline__ int even_keys(const AttentionParams &p, const TileReq
         for (int n = 0; n < N; n++) parts += r[n].tiles * (int)ceilf((float)steps[n] * per);
         return (long long)__builtin_amdgcn_readlane(sum_upto(parts), 63) * p.kv_heads <= p.even;
     };
-    int few = least, many = max(least, min(most, share));      // steps of a part
-    if (!fit(many)) few = many = max(least, p.chunk / kTileKeys);
+    const int given = max(least, p.chunk / kTileKeys);
+    int few = least, many = max(least, min(most, max(share, given)));      // steps of a part
+    if (!fit(many)) few = many = given;
     while (few < many) {
         const int mid = (few + many) / 2;
         if (fit(mid)) many = mid;

@@ -21,6 +21,8 @@ CASES = {
     "two parts each, more than run at once": ([(2000 - 11 * (i % 7), 9) for i in range(38)], 32, 8, 64, 64, HALF, 0, 0),
     "one request of fewer parts": ([(2100, 30)] * 5 + [(200, 30)], 8, 2, 64, 16, HALF, 0, 0),
     "as many parts under a window": ([(4000 + 100 * i, 40) for i in range(6)], 8, 2, 128, 16, BF16, 900, 4),
+    "few long lists among short ones, wide heads": ([(6300, 300), (298, 298), (72, 72), (1000, 17), (122, 4)], 32, 8, 256, 24, BF16, 0, 0),
+    "few long lists among short ones": ([(9000, 200)] + [(130 + i, 129) for i in range(20)], 32, 8, 128, 16, HALF, 0, 0),
     "no part is seen": ([(0, 5)] * 7 + [(0, 0)], 8, 2, 64, 16, HALF, 0, 0),
 }
 

@@ -15,7 +15,7 @@ captured by ``torch.cuda.graph``: a capture gets a workspace of its own from the
 (the graph clears its counters, one small launch a replay); what the kernels need loaded, a call on any stream before it loads.  Caches are float16 or bfloat16
 [blocks, block_size, kv_heads, dim] in any order of memory whose last dimension is contiguous; dim is a multiple of 8 up to 256.
 
-A cache may also be held in MXFP4, 4.25 bits a value: pass an ``Mxfp4`` (see there, and ``mxfp4_cache``) wherever a cache is asked for; the
+A cache may also be held in MXFP4, 4.25 bits a value where dim is 64, 128 or 256: pass an ``Mxfp4`` (see there, and ``mxfp4_cache``) wherever a cache is asked for; the
 write quantises, the attention reads the codes.  The operators of these are ``torch.ops.gptq_hip.<name>_mx``, with codes and scales as
 two arguments each.
 """

@@ -171,9 +171,10 @@ int plan(const gptq_hip_attention &a, bool mx, Plan &pl)
             else want = std::max(1ll, want / busy) * busy;
         }
         divide(d, want, busy, keys, room);
-        // MXFP4: parts by the lengths on the GPU (even_keys), us by the longest context and so: 3 pieces of up to 300 tokens behind up to
-        // 20000 keys 230 / 198, 10 of up to 64 143 / 100, 20 of up to 33 behind 16000 138 / 85, 200 of 20 to 60 behind 8000, 2 heads, 174 / 165;
-        // 30 of 30 to 60 behind 7000, nearly a tile a workgroup as they are, 134 / 161; from 2048 keys on 24 of 50 behind 3000 75 / 79.
+        // MXFP4: parts by the lengths on the GPU (even_keys).  8 key/value heads, us by the longest context and so: lengths of all sizes, 3 pieces of up to 300 tokens
+        // behind up to 20000 keys 163 / 110, 10 of up to 64 161 / 74, 20 of up to 33 behind 16000 134 / 73, 200 of 20 to 60 behind 8000, 2 heads, 245 / 157, 30 of
+        // 30 to 60 behind 7000 166 / 105; the same from half the longest on 216 / 215, all alike 229 / 242; 12 of 130 behind 12000, alike, 393 / 407.  From 2048 keys
+        // on: 24 of 50 behind 3000, of all sizes 79 / 54, from half on 99 / 106, alike 108 / 119: there the finding costs too large a share.
         if (even && d.splits > 1) {
             d.even = (int)(a.cache.dim > 128 ? kOwnWorkgroups / 2 : kOwnWorkgroups);     // (as many as the card holds)
             d.splits = (int)std::max(1ll, std::min({2ll * d.splits, ceil_div(keys, 256), room}));

@@ -398,7 +398,7 @@ int gptq_hip_cache_write(const gptq_hip_cache *cache, const void *k, const void 
 int gptq_hip_cache_read(const gptq_hip_cache *cache, const int32_t *slots, int tokens, void *k, void *v, void *stream);
 
 /*
- * The same cache held in 4.25 bits (MXFP4).  A head's dim values of a token, padded with zeros to a multiple of 32, are groups of 32: each
+ * The same cache held in MXFP4, 4.25 bits a value where dim is 64, 128 or 256.  A head's dim values of a token, padded with zeros to a multiple of 32, are groups of 32: each
  * has a power of two 2^e, kept as the byte e + 127, and 32 codes of a sign and one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (value 2 j in the
  * low half of byte j, 2 j + 1 in the high one).  A row of codes has 16 ceil(dim / 32) bytes; a row of scales has 2 bytes up to
  * dim 64, 4 up to 128, 8 above, of which the first ceil(dim / 32) count.  A write takes the e that puts the group's largest magnitude m

@@ -41,6 +41,25 @@ def test_parts(name, made):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("made", [Step, MxStep])
+@pytest.mark.parametrize("request_, window, prefix", [((0, 0), 0, 0), ((900, 0), 0, 0), ((40, 40), 0, 0), ((2500, 70), 0, 0), ((2500, 70), 300, 0), ((3, 50), 0, 0),
+                                                      ((700, 60), 0, 2500)])
+@pytest.mark.parametrize("ahead, behind", [(0, 0), (0, 90), (7, 61)])
+def test_one_request(made, request_, window, prefix, ahead, behind):
+    """Alone in its step, with or without tokens, some of them before its context, in a step that is padded."""
+    s = made(43, [request_], 8, 2, 64, 16, HALF, "head", window, 3 if window else 0, prefix)
+    want, size = s.expected()
+    n = s.tokens
+    nan = lambda rows: torch.full((rows, 8, 64), float("nan"), device="cuda").half()
+    s.q = torch.cat([nan(ahead), s.q, nan(behind)])
+    s.starts = s.starts + ahead
+    nan(len(s.q))      # what the result's memory holds
+    got = attend(s)
+    assert bool((got[:ahead] == 0).all()) and bool((got[ahead + n:] == 0).all())
+    assert bool(((got[ahead:ahead + n].double() - want).abs() <= 2.25 * 2.0 ** -11 * size + 2.0 ** -24).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("made", [Step, MxStep])
 def test_lengths_that_the_host_did_not_expect(made):
     """Contexts behind the longest that the host knows: longer parts, as many for every tile."""
     s = made(42, [(3000, 40), (2900, 40), (2950, 33)], 8, 2, 64, 16)
